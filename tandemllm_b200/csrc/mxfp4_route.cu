@@ -1,0 +1,181 @@
+// Around the routed experts' products of a step that is too large for the two-kernel form (mxfp4_few.cu): which pairs (row, slot) an expert
+// has, its token rows side by side, and the weighed sum of what the experts made of a row.
+#include "mxfp4.cuh"
+
+namespace tl {
+namespace mx {
+
+constexpr int PLAN_THREADS = 1024;
+constexpr int PLAN_EXPERTS = 1024;
+constexpr int SUM_TOP = 32;
+
+// The sum of `v` over the threads before this one; `total` gets all of it. `scratch`: 33 integers.
+__device__ __forceinline__ int before_me(int v, int* scratch, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int run = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, run, o);
+    if (lane >= o) run += a;
+  }
+  __syncthreads();
+  if (lane == 31) scratch[warp] = run;
+  __syncthreads();
+  if (warp == 0) {
+    const int mine = scratch[lane];
+    int sum = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += a;
+    }
+    scratch[lane] = sum - mine;
+    if (lane == 31) scratch[32] = sum;
+  }
+  __syncthreads();
+  total = scratch[32];
+  return scratch[warp] + run - v;
+}
+
+// One block. Pairs of an expert lie together, in any order among themselves: a row's products do not depend on the rows beside it, so the
+// order, which the atomics leave open, changes no result. Pairs without an expert come last and are in no tile.
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restrict__ ids, int pairs, int experts, int tile_rows_at_most,
+                                                            int* __restrict__ counts, int* __restrict__ sorted, int* __restrict__ place,
+                                                            int* __restrict__ tile_group, int* __restrict__ tile_row0, int* __restrict__ tile_rows,
+                                                            int* __restrict__ n_tiles, int* status) {
+  __shared__ int at[PLAN_EXPERTS + 1];
+  __shared__ int scratch[33];
+  chain_next();
+  chain_wait();
+  const int tid = threadIdx.x;
+  for (int e = tid; e <= experts; e += PLAN_THREADS) at[e] = 0;
+  __syncthreads();
+  for (int p = tid; p < pairs; p += PLAN_THREADS) {
+    const int id = ids[p];
+    const bool ok = (unsigned)id < (unsigned)experts;
+    atomicAdd(&at[ok ? id : experts], 1);
+    if (!ok) atomicExch(status, 6);
+  }
+  __syncthreads();
+  const int mine = tid < experts ? at[tid] : 0, tiles = (mine + tile_rows_at_most - 1) / tile_rows_at_most;
+  int all, all_tiles;
+  const int first = before_me(mine, scratch, all);
+  const int first_tile = before_me(tiles, scratch, all_tiles);
+  if (tid < experts) {
+    counts[tid] = mine;
+    at[tid] = first;
+    for (int t = 0; t < tiles; ++t) {
+      tile_group[first_tile + t] = tid;
+      tile_row0[first_tile + t] = first + t * tile_rows_at_most;
+      tile_rows[first_tile + t] = min(tile_rows_at_most, mine - t * tile_rows_at_most);
+    }
+  }
+  if (tid == 0) {
+    at[experts] = all;
+    *n_tiles = all_tiles;
+  }
+  __syncthreads();
+  for (int p = tid; p < pairs; p += PLAN_THREADS) {
+    const int id = ids[p];
+    const int to = atomicAdd(&at[(unsigned)id < (unsigned)experts ? id : experts], 1);
+    sorted[to] = p;
+    place[p] = to;
+  }
+}
+
+// to[i] = from[sorted[i] / top], 16 bytes a thread.
+__global__ void __launch_bounds__(256) gather_kernel(const uint4* __restrict__ from, long long ld, const int* __restrict__ sorted, int top,
+                                                     uint4* __restrict__ to, int pieces, long long total) {
+  chain_next();
+  chain_wait();
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const long long row = i / pieces;
+  to[i] = from[(long long)(sorted[row] / top) * ld + (i - row * pieces)];
+}
+
+// out[r] = sum over r's slots, one after the other, of wts * y[place]; without weights the rows as they are. Four outputs a thread.
+template <bool WHOLE, typename TOut>
+__global__ void __launch_bounds__(256) sum_kernel(const float* __restrict__ y, long long ldy, const int* __restrict__ place,
+                                                  const int* __restrict__ ids, const float* __restrict__ wts, TOut* __restrict__ out, int N, int top,
+                                                  int experts) {
+  __shared__ int s_place[SUM_TOP];
+  __shared__ float s_weight[SUM_TOP];
+  chain_next();
+  chain_wait();
+  const long long r = blockIdx.x;
+  if (threadIdx.x < top) {
+    const long long p = r * top + threadIdx.x;
+    s_place[threadIdx.x] = (unsigned)ids[p] < (unsigned)experts ? place[p] : -1;
+    s_weight[threadIdx.x] = wts ? wts[p] : 1.f;
+  }
+  __syncthreads();
+  const int n = (blockIdx.y * 256 + threadIdx.x) * 4;
+  if (n >= N) return;
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int j = 0; j < top; ++j) {
+    if (s_place[j] < 0) continue;
+    const float* from = y + s_place[j] * ldy + n;
+    const float w = s_weight[j];
+    if (WHOLE) {
+      const float4 f = *reinterpret_cast<const float4*>(from);
+      v[0] = fmaf(w, f.x, v[0]), v[1] = fmaf(w, f.y, v[1]), v[2] = fmaf(w, f.z, v[2]), v[3] = fmaf(w, f.w, v[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < N) v[i] = fmaf(w, from[i], v[i]);
+    }
+  }
+  TOut* to = out + r * N + n;
+  if (WHOLE) {
+    store4(to, v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i < N) to[i] = from_f32<TOut>(v[i]);
+  }
+}
+
+}  // namespace mx
+}  // namespace tl
+
+using namespace tl;
+
+extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_rows_at_most, int* counts, int* sorted, int* place, int* tile_group,
+                             int* tile_row0, int* tile_rows, int* n_tiles, int* status, cudaStream_t stream) {
+  if (pairs == 0) return 0;
+  TL_REQUIRE(pairs > 0 && experts >= 1 && experts <= mx::PLAN_EXPERTS && tile_rows_at_most >= 1, "mxfp4 experts: %d pairs of %d experts", pairs,
+             experts);
+  return (int)launch_chained(mx::plan_kernel, dim3(1), dim3(mx::PLAN_THREADS), 0, stream, ids, pairs, experts, tile_rows_at_most, counts, sorted,
+                             place, tile_group, tile_row0, tile_rows, n_tiles, status);
+}
+
+// x [*, width] bfloat16 (row stride ldx), to [pairs, width]; width and ldx multiples of 8, pointers of 16 bytes.
+extern "C" int tl_mxfp4_gather(const void* x, long long ldx, const int* sorted, int top, void* to, int pairs, int width, cudaStream_t stream) {
+  if (pairs == 0 || width == 0) return 0;
+  TL_REQUIRE(pairs > 0 && top >= 1 && width % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)to % 16) == 0,
+             "mxfp4 experts: rows of %d numbers, %lld apart", width, ldx);
+  const long long total = (long long)pairs * (width / 8), blocks = ceil_div64(total, 256);
+  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4 experts: %d pairs of %d numbers are too many", pairs, width);
+  return (int)launch_chained(mx::gather_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const uint4*)x, ldx / 8, sorted, top, (uint4*)to,
+                             width / 8, total);
+}
+
+// y [pairs, N] 32-bit, out [rows, N] contiguous, bfloat16 or 32-bit.
+extern "C" int tl_mxfp4_sum(const float* y, const int* place, const int* ids, const float* wts, void* out, int out_dtype, int rows, int N, int top,
+                            int experts, cudaStream_t stream) {
+  if (rows == 0 || N == 0) return 0;
+  TL_REQUIRE(rows > 0 && N > 0 && top >= 1 && top <= mx::SUM_TOP, "mxfp4 experts: %d rows of %d, top-%d", rows, N, top);
+  TL_REQUIRE(N <= 65535 * 1024, "mxfp4 experts: %d outputs exceed the grid limit", N);
+  const bool whole = N % 4 == 0 && ((uintptr_t)y % 16) == 0 && ((uintptr_t)out % 16) == 0;
+  const dim3 grid(rows, ceil_div(N, 1024));
+#define TL_SUM(W_, T_) \
+  return (int)launch_chained(mx::sum_kernel<W_, T_>, grid, dim3(256), 0, stream, y, (long long)N, place, ids, wts, (T_*)out, N, top, experts)
+  if (out_dtype == TL_FP32) {
+    if (whole) TL_SUM(true, float);
+    TL_SUM(false, float);
+  }
+  if (whole) TL_SUM(true, bf16);
+  TL_SUM(false, bf16);
+#undef TL_SUM
+}

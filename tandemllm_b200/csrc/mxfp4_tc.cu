@@ -1,0 +1,478 @@
+// Products of bfloat16 rows with MXFP4 weights (mxfp4.cuh) on the 5th-generation tensor cores, for more rows than mxfp4_few.cu takes:
+//
+//   C[m, n] = sum_k X[m, k] * W[n, k] (+ bias[n])      or, gated:  C[m, n] = act(X . G[n] + b_g[n]) * (X . U[n] + b_u[n])
+//
+// A CTA computes 128 weight rows (gated: 64 outputs, 8 gate rows and the 8 up rows of the same outputs in turn) by BN token rows. The
+// weights are the MMA's M side and come from tensor memory: lane r of it is weight row r, so the thread that owns a lane loads that
+// row's 64 values of a k-block (32 bytes of codes and two scales), makes them bfloat16 numbers in its registers and stores them to its
+// lane with one tcgen05.st. The 4-bit weights thus cross from L2 once, as they are, and no shared memory is spent on them. The token rows are the N
+// side: boxes of 64 k-elements that TMA brings into a ring of stages (128-byte swizzle, no multicast).
+//
+//   warp 0       one thread keeps the ring of token boxes full
+//   warp 1       one thread issues the MMAs (kind::f16, A in tensor memory, B in shared memory) and releases both operands' stages
+//   warps 2..9   two groups of four that take every other k-block of weights; then the epilogue, each group every other 16 columns
+//
+// An MMA of 128 x 128 x 64 takes 256 cycles of the tensor pipe and its weights 134 issue cycles of each scheduler, so with tiles of 128
+// token rows the conversion runs under the products; two CTAs an SM run under each other's ends.
+//
+// SPLIT: a cluster of CTAs shares a tile, each with a run of k; each leaves its accumulator in its shared memory, the cluster meets, and
+// every CTA adds the sums of some of the tokens in rank order and stores them, so the result does not depend on timing.
+//
+// Every wait on an mbarrier is bounded: when a bound is hit the CTA records status 11, stops issuing work, waits (bounded again) for the
+// copies and products in flight, meets its cluster, frees its tensor memory and returns.
+#include "mxfp4.cuh"
+#include "tma.cuh"
+
+namespace tl {
+namespace mx {
+
+constexpr int ROWS = 128;                   // weight rows a CTA: the MMA's M side
+constexpr int KB = TMA_BOX_COLS;            // k-elements a block
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = 64 + 32 * EPI_WARPS;
+constexpr int MAX_SPLITS = 8;
+
+struct TcParams {
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;
+  void* C;
+  long long ldc;
+  int M, N, K;                // tokens, outputs, reduction length
+  int matrices;               // matrices a group: 1, or 2 where gate and up matrix come in turn
+  int tiles_a_split;          // tiles of 128 k a CTA of a cluster takes
+  const int* tile_group;      // grouped (or null): per token tile its group, first row and rows; tiles past *n_tiles leave
+  const int* tile_row0;
+  const int* tile_rows;
+  const int* n_tiles;
+  int act;                    // the gate's activation (TL_ACT_*), 0 for a plain product; negated: an activation on a plain product's results
+  float ga0, ga1;
+  const float* row_weight;    // grouped (or null): a (row, slot) pair's own weight on its sums, see `pair_weight`
+  const int* weight_index;
+  int* status;
+};
+
+template <int BN>
+struct Tc {
+  static constexpr int B_BYTES = BN * KB * 2;
+  static constexpr int B_STAGES = BN >= 128 ? 6 : 8;
+  static constexpr int A_COLS = KB / 2;                         // columns of tensor memory a k-block of weights takes
+  static constexpr int A_STAGES = BN >= 128 ? 4 : 6;
+  static constexpr int TMEM_COLS = 256;
+  static constexpr int AHEAD = BN >= 128 ? 2 : 4;               // k-blocks of codes a thread has on their way
+  static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+  // What a launch with clusters asks for at least. A CTA of a cluster that waits for tensor memory keeps the others waiting, who keep
+  // theirs; beside another kernel of clusters that could close a circle. With this much shared memory no SM has room for more CTAs of such kernels
+  // (tc_gemm_pair.cu: 90 KB and more with half of tensor memory, 192 KB and more with all of it) than its tensor memory has.
+  static constexpr int SPLIT_TOTAL = TOTAL > 72 * 1024 ? TOTAL : 72 * 1024;
+  static_assert(BN + A_STAGES * A_COLS <= TMEM_COLS, "accumulator and weights share half of tensor memory");
+  static_assert(B_STAGES * B_BYTES >= BN * ROWS * 4, "an accumulator fits the ring of token boxes");
+};
+
+__device__ __forceinline__ uint64_t desc(uint32_t smem_addr) {  // K-major, 128-byte rows and swizzle: 8-row groups 1024 bytes apart
+  uint64_t d = 0;
+  d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
+  d |= (uint64_t)1 << 16;
+  d |= (uint64_t)(1024 >> 4) << 32;
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)2 << 61;
+  return d;
+}
+
+__device__ __forceinline__ void mma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, "
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
+      "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+__device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
+  uint32_t r[16];
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ float load_from(const float* p, uint32_t rank) {     // `p` in the shared memory of the cluster's CTA `rank`
+  uint32_t a;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// The codes and scales of a thread's row in one k-block.
+struct RowBlock {
+  uint4 c[2];
+  uint32_t s;                 // the two blocks' scales, the first in the low byte
+};
+__device__ __forceinline__ void load_row_block(RowBlock& q, const uint8_t* codes, const uint8_t* scales, int tile, bool valid) {
+  asm volatile(
+      "{\n\t.reg .pred ok;\n\t"
+      "setp.ne.b32 ok, %11, 0;\n\t"
+      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+      "mov.b32 %4, 0;\n\tmov.b32 %5, 0;\n\tmov.b32 %6, 0;\n\tmov.b32 %7, 0;\n\tmov.b32 %8, 0;\n\t"
+      "@ok ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%9];\n\t"
+      "@ok ld.global.nc.v4.u32 {%4, %5, %6, %7}, [%9 + 128];\n\t"
+      "@ok ld.global.nc.u16 %8, [%10];\n\t}"
+      : "=r"(q.c[0].x), "=r"(q.c[0].y), "=r"(q.c[0].z), "=r"(q.c[0].w), "=r"(q.c[1].x), "=r"(q.c[1].y), "=r"(q.c[1].z), "=r"(q.c[1].w), "=r"(q.s)
+      : "l"(codes + (long long)tile * TILE_CODES), "l"(scales + (long long)tile * TILE_SCALES), "r"((int)valid));
+}
+
+__device__ __forceinline__ void convert(const RowBlock& q, uint32_t (&v)[32]) {
+  const uint32_t s[2] = {q.s & 255u, q.s >> 8};
+  const bool far = __any_sync(0xffffffffu, max(s[0], s[1]) > 128u);
+#pragma unroll
+  for (int b = 0; b < 2; ++b) {
+    const uint32_t f = factor(s[b]), w[4] = {q.c[b].x, q.c[b].y, q.c[b].z, q.c[b].w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x[4];
+      values(w[i], f, x);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[b * 16 + i * 4 + j] = x[j];
+    }
+    if (far) {
+      const uint32_t left = factor_left(s[b]);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) v[b * 16 + j] = mul2(v[b * 16 + j], left);
+    }
+  }
+}
+
+template <typename TOut> __device__ __forceinline__ void store_one(TOut* p, float v) { *p = from_f32<TOut>(v); }
+
+template <int BN, bool GATED, bool SPLIT, typename TOut>
+__global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ CUtensorMap tmX, TcParams p) {
+  using S = Tc<BN>;
+  constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
+  chain_next();
+  chain_wait();
+  int tok0, tok_rows, group = 0;
+  if (p.tile_group) {
+    const int t = blockIdx.y;
+    if (t >= *p.n_tiles) return;
+    tok0 = p.tile_row0[t];
+    tok_rows = min(p.tile_rows[t], BN);
+    group = p.tile_group[t];
+  } else {
+    tok0 = blockIdx.y * BN;
+    tok_rows = min(BN, p.M - tok0);
+  }
+  const int n0 = blockIdx.x * OUTS;
+  const int k_tiles = ceil_div(p.K, TILE_K);
+  const int tile0 = SPLIT ? (int)blockIdx.z * p.tiles_a_split : 0;              // first tile of 128 k
+  const int kb0 = 2 * tile0, num_kb = min(ceil_div(p.K, KB), SPLIT ? kb0 + 2 * p.tiles_a_split : 0x7fffffff) - kb0;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
+  uint64_t* b_empty = b_full + S::B_STAGES;
+  uint64_t* a_full = b_empty + S::B_STAGES;
+  uint64_t* a_empty = a_full + S::A_STAGES;
+  uint64_t* acc_full = a_empty + S::A_STAGES;
+  uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
+  volatile uint32_t* aborted = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::B_STAGES; ++s) {
+      mbar_init(&b_full[s], 1);
+      mbar_init(&b_empty[s], 1);
+    }
+    for (int s = 0; s < S::A_STAGES; ++s) {
+      mbar_init(&a_full[s], 4);                                 // one arrival a warp of the group whose k-block it is
+      mbar_init(&a_empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    *aborted = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)S::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  auto give_up = [&]() {
+    *aborted = 1;
+    atomicExch(p.status, 11);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      // ---- token rows ----
+      int issued = 0;
+      for (int i = 0; i < num_kb; ++i) {
+        const int s = i % S::B_STAGES;
+        if (i >= S::B_STAGES && !mbar_wait(&b_empty[s], ((i / S::B_STAGES) - 1) & 1)) give_up();
+        if (*aborted) break;
+        mbar_expect_tx(&b_full[s], S::B_BYTES);
+        tma_load_2d(boxes + s * S::B_BYTES, &tmX, &b_full[s], (kb0 + i) * KB, tok0);
+        issued = i + 1;
+      }
+      if (*aborted)            // copies already started must land before the CTA's shared memory goes away
+        for (int i = max(0, issued - S::B_STAGES); i < issued; ++i) mbar_wait(&b_full[i % S::B_STAGES], (i / S::B_STAGES) & 1);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
+      constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+      for (int i = 0; i < num_kb; ++i) {
+        const int sa = i % S::A_STAGES, sb = i % S::B_STAGES;
+        if (!mbar_wait(&b_full[sb], (i / S::B_STAGES) & 1) || !mbar_wait(&a_full[sa], (i / S::A_STAGES) & 1)) give_up();
+        if (*aborted) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const uint32_t b = smem_u32(boxes + sb * S::B_BYTES), a = tmem_base + BN + sa * S::A_COLS;
+#pragma unroll
+        for (int k = 0; k < KB / 16; ++k) mma_a_tmem(tmem_base, a + k * 8, desc(b + k * 32), idesc, (i > 0 || k > 0) ? 1u : 0u);
+        commit(&b_empty[sb]);
+        commit(&a_empty[sa]);
+      }
+      commit(acc_full);
+    }
+  } else {
+    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, k-blocks of this group's parity ----
+    const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+    const int eight = r >> 3, row_tiles = ceil_div(p.N, TILE_ROWS);
+    const int row_tile = (n0 >> 3) + (GATED ? eight >> 1 : eight);
+    const bool valid = row_tile < row_tiles;
+    const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (valid ? row_tile : 0)) * k_tiles + tile0;
+    const uint8_t* codes = p.codes + first * TILE_CODES + (2 * half * TILE_ROWS + (r & 7)) * 16;
+    const uint8_t* scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK) + 2 * half;
+    RowBlock q[S::AHEAD];
+#pragma unroll
+    for (int u = 0; u < S::AHEAD; ++u) load_row_block(q[u], codes, scales, u, valid && 2 * u + half < num_kb);
+    bool ok = true;
+    for (int i0 = half; i0 < num_kb && ok; i0 += 2 * S::AHEAD) {
+#pragma unroll
+      for (int u = 0; u < S::AHEAD; ++u) {
+        const int i = i0 + 2 * u;
+        if (i < num_kb && ok) {
+          uint32_t v[32];
+          convert(q[u], v);
+          load_row_block(q[u], codes, scales, (i >> 1) + S::AHEAD, valid && i + 2 * S::AHEAD < num_kb);
+          const int s = i % S::A_STAGES;
+          if (i >= S::A_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], ((i / S::A_STAGES) - 1) & 1)) && *aborted == 0;
+          ok = __all_sync(0xffffffffu, ok);
+          if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            tmem_store32(t_lane + BN + s * S::A_COLS, v);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&a_full[s]);
+          } else if (lane == 0) {
+            give_up();
+          }
+        }
+      }
+    }
+    // ---- epilogue ----
+    if (!__all_sync(0xffffffffu, mbar_wait(acc_full, 0))) {
+      if (lane == 0) give_up();
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    ok = __all_sync(0xffffffffu, *aborted == 0);
+    if (ok) {
+      float* part = (float*)boxes;                              // SPLIT: [BN][128]; the products have read the boxes
+      TOut* C = (TOut*)p.C;
+      const int n = n0 + (GATED ? (r >> 4) * 8 + (r & 7) : r);
+      const bool mine = n < p.N, up = GATED && (eight & 1);
+      float bias = 0.f;
+      if (!SPLIT && p.bias && mine) bias = p.bias[up ? p.N + n : n];
+#pragma unroll 1
+      for (int c0 = half * 16; c0 < min(BN, tok_rows); c0 += 32) {
+        float v[16];
+        tmem_load16(t_lane + c0, v);
+        const int left = tok_rows - c0;
+        if constexpr (SPLIT) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) part[(c0 + j) * ROWS + r] = v[j];
+          continue;
+        }
+        if (p.row_weight) {
+          const float w = (lane & 15) < left ? pair_weight(p.row_weight, p.weight_index, (long long)tok0 + c0 + (lane & 15)) : 1.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] *= __shfl_sync(0xffffffffu, w, j);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] += bias;
+        if constexpr (GATED) {
+          // of two tokens the lane with the gate row finishes the first and the one with the up row the second
+#pragma unroll
+          for (int j = 0; j < 16; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 8);
+            const float out = gated(up ? other : v[j], up ? v[j + 1] : other, p.act, p.ga0, p.ga1);
+            const int m = up ? j + 1 : j;
+            if (mine && m < left) store_one(C + (long long)(tok0 + c0 + m) * p.ldc + n, out);
+          }
+        } else {
+          if (p.act < 0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = gate_activation(v[j], -p.act);
+          }
+          if (mine) {
+            TOut* to = C + (long long)(tok0 + c0) * p.ldc + n;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j < left) store_one(to + (long long)j * p.ldc, v[j]);
+          }
+        }
+      }
+    }
+  }
+  if constexpr (SPLIT) {
+    __syncthreads();
+    __syncwarp();
+    cluster_sync();
+    if (warp >= 2 && *aborted == 0) {
+      const float* part = (const float*)boxes;
+      TOut* C = (TOut*)p.C;
+      const int rank = (int)cluster_rank(), ranks = gridDim.z, at = threadIdx.x - 64;
+      const int o = at & (OUTS - 1), n = n0 + o;
+      const int r = GATED ? (o >> 3) * 16 + (o & 7) : o;
+      if (n < p.N) {
+        for (int m = rank + ranks * (at / OUTS); m < tok_rows; m += ranks * (32 * EPI_WARPS / OUTS)) {
+          float v = 0.f, u = 0.f;
+          for (int s = 0; s < ranks; ++s) {
+            v += load_from(part + m * ROWS + r, s);
+            if (GATED) u += load_from(part + m * ROWS + r + 8, s);
+          }
+          if (p.row_weight) {
+            const float w = pair_weight(p.row_weight, p.weight_index, (long long)tok0 + m);
+            v *= w, u *= w;
+          }
+          if (p.bias) {
+            v += p.bias[n];
+            if (GATED) u += p.bias[p.N + n];
+          }
+          const float out = GATED ? gated(v, u, p.act, p.ga0, p.ga1) : p.act < 0 ? gate_activation(v, -p.act) : v;
+          store_one(C + (long long)(tok0 + m) * p.ldc + n, out);
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();                                             // no CTA leaves while another reads its sums
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::TMEM_COLS));
+  }
+}
+
+template <int BN, bool GATED, bool SPLIT, typename TOut>
+int launch_tc(const CUtensorMap& tmX, const TcParams& p, dim3 grid, cudaStream_t stream) {
+  constexpr int BYTES = SPLIT ? Tc<BN>::SPLIT_TOTAL : Tc<BN>::TOTAL;
+  auto kernel = tc_kernel<BN, GATED, SPLIT, TOut>;
+  static thread_local int set_on = -1;              // the device whose function has its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (set_on != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES);
+    if (e != cudaSuccess) return (int)e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    if (e != cudaSuccess) return (int)e;
+    set_on = dev;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = grid.z;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = BYTES;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = SPLIT ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, tmX, p);
+}
+
+}  // namespace mx
+}  // namespace tl
+
+using namespace tl;
+
+// x [x_rows, K] bfloat16 (row stride ldx); the matrix N x K, or with `matrices` 2 a gate and an up matrix; grouped (tile_group ...): as many for
+// every group, x in the plan's order, tiles of at most `bn` rows. bias [N] (gated: [2 N]) 32-bit or null. out [M, N] (row stride ldc). `act`
+// as in tl_mxfp4_few. `bn`: token rows a tile, 16, 32, 64 or 128. `splits`: CTAs that share a tile's k, 1 to 8, none of them without any.
+extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const void* codes, const void* scales, const float* bias, void* out,
+                           long long ldc, int M, int N, int K, int act, float a0, float a1, int out_dtype, int bn, int splits,
+                           const int* tile_group, const int* tile_row0, const int* tile_rows, const int* n_tiles, int max_tiles,
+                           const float* row_weight, const int* weight_index, int* status, cudaStream_t stream) {
+  if (M == 0 || N == 0 || (tile_group && max_tiles == 0)) return 0;
+  TL_REQUIRE(M >= 1 && N >= 1 && K >= 1 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0, "mxfp4 product: %d rows x (%d x %d), row stride %lld",
+             M, N, K, ldx);
+  TL_REQUIRE(act <= 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 product: gate activation %d is none (nor an ungated one, negated)", act);
+  TL_REQUIRE(act <= 0 || out_dtype == TL_BF16, "mxfp4 product: gated outputs of type %d", out_dtype);
+  const int k_tiles = ceil_div(K, mx::TILE_K);
+  TL_REQUIRE(splits >= 1 && splits <= mx::MAX_SPLITS && splits <= k_tiles, "mxfp4 product: k %d in %d runs", K, splits);
+  TL_REQUIRE(!tile_group || (tile_row0 && tile_rows && n_tiles), "mxfp4 product: an incomplete plan (%d tiles)", max_tiles);
+  mx::TcParams p = {};
+  p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.bias = bias, p.C = out, p.ldc = ldc, p.M = M, p.N = N, p.K = K;
+  p.matrices = act > 0 ? 2 : 1;
+  p.tiles_a_split = ceil_div(k_tiles, splits);
+  splits = ceil_div(k_tiles, p.tiles_a_split);                  // (rounding up may leave the last ones nothing)
+  p.tile_group = tile_group, p.tile_row0 = tile_row0, p.tile_rows = tile_rows, p.n_tiles = n_tiles;
+  p.act = act, p.ga0 = a0, p.ga1 = a1, p.row_weight = row_weight, p.weight_index = weight_index, p.status = status;
+  const dim3 grid(ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS), tile_group ? max_tiles : ceil_div(M, bn), splits);
+  TL_REQUIRE(grid.y <= 65535, "mxfp4 product: %d token tiles exceed the grid limit", (int)grid.y);
+  CUtensorMap tmX;
+  const int r = tensor_map(x, x_rows, K, ldx, bn, &tmX);
+  if (r) return r;
+#define TL_MX_TC_(BN_, S_)                                                                            \
+  do {                                                                                                \
+    if (act > 0) return mx::launch_tc<BN_, true, S_, bf16>(tmX, p, grid, stream);                     \
+    if (out_dtype == TL_FP32) return mx::launch_tc<BN_, false, S_, float>(tmX, p, grid, stream);      \
+    return mx::launch_tc<BN_, false, S_, bf16>(tmX, p, grid, stream);                                 \
+  } while (0)
+#define TL_MX_TC(BN_)                 \
+  do {                                \
+    if (splits > 1) TL_MX_TC_(BN_, true); \
+    TL_MX_TC_(BN_, false);            \
+  } while (0)
+  if (bn == 16) TL_MX_TC(16);
+  if (bn == 32) TL_MX_TC(32);
+  if (bn == 64) TL_MX_TC(64);
+  TL_REQUIRE(bn == 128, "mxfp4 product: token tiles of %d rows; 16, 32, 64 or 128", bn);
+  TL_MX_TC(128);
+#undef TL_MX_TC
+#undef TL_MX_TC_
+}

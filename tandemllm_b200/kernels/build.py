@@ -45,7 +45,7 @@ LIBRARIES: dict[str, list[str]] = {
     "tensorcore": ["tc_gemm.cu", "tc_gemm_pair.cu", "attention_mma.cu", "attention_tc.cu", "attention_headmix_mma.cu",
                    "attention_latent_mma.cu", "attention_flex_mma.cu", "head_linear_mma.cu", "gemm_skinny_mma.cu"],
     # feed-forwards with 4-bit weights; loaded by a model that has some
-    "mxfp4": ["mxfp4.cu", "mxfp4_few.cu"],
+    "mxfp4": ["mxfp4.cu", "mxfp4_few.cu", "mxfp4_tc.cu", "mxfp4_route.cu"],
 }
 HEADERS = ["common.cuh", "route.cuh", "add_rmsnorm.cuh", "recurrence.cuh", "attention_noalloc.h", "tma.cuh", "mxfp4.cuh"]
 

@@ -36,6 +36,11 @@ _SIGNATURES = {
                                c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p],
     "tl_mxfp4_experts_second": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int,
                                 c_void_p, c_void_p],
+    "tl_mxfp4_tc": [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_float,
+                    c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
+    "tl_mxfp4_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "tl_mxfp4_gather": [c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p],
+    "tl_mxfp4_sum": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
 }
 _lib = None
 
@@ -148,9 +153,30 @@ def _output(out, rows: int, n: int, dtype: torch.dtype, device) -> torch.Tensor:
     return out
 
 
-def _few(x, w: Mxfp4Matrix, bias, out, act: int, constants) -> None:
-    _check(lib().tl_mxfp4_few(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops.ptr(bias), out.data_ptr(), out.stride(0),
-                              x.shape[0], w.n, x.shape[1], act, *constants, ops.dtype_code(out.dtype), ops.stream()), "mxfp4_few")
+def token_tile(rows: float) -> int:
+    """Token rows of a tile of the tensor-core product for `rows` rows side by side."""
+    return 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+
+
+def splits_of(ctas: int, k: int, sms: int) -> int:
+    """CTAs that share a tile's k where `ctas` alone leave SMs idle (two CTAs an SM, each with at least two tiles of 128)."""
+    return max(1, min(2 * sms // ctas, -(-k // TILE_K) // 2, 8))
+
+
+def _product(runtime, x, w: Mxfp4Matrix, bias, out, act: int, constants) -> None:
+    """out = the product of x's rows with w: act 0 plain, a gate's code gated, negated an activation on a plain product."""
+    M = x.shape[0]
+    if M == 0:
+        return
+    if M <= FEW_ROWS:
+        _check(lib().tl_mxfp4_few(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops.ptr(bias), out.data_ptr(), out.stride(0),
+                                  M, w.n, x.shape[1], act, *constants, ops.dtype_code(out.dtype), ops.stream()), "mxfp4_few")
+        return
+    bn = token_tile(M)
+    ctas = -(-w.n // (64 if act > 0 else 128)) * -(-M // bn)
+    _check(lib().tl_mxfp4_tc(x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), ops.ptr(bias), out.data_ptr(), out.stride(0),
+                             M, w.n, x.shape[1], act, *constants, ops.dtype_code(out.dtype), bn, splits_of(ctas, x.shape[1], ops.sm_count()),
+                             None, None, None, None, 0, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
 
 
 def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
@@ -161,8 +187,7 @@ def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None =
     x = _rows(x, w)
     _vector(bias, w.n, "the bias", x.device)
     out = _output(out, x.shape[0], w.n, out_dtype or (out.dtype if out is not None else x.dtype), x.device)
-    for r in range(0, x.shape[0], FEW_ROWS):
-        _few(x[r:r + FEW_ROWS], w, bias, out[r:r + FEW_ROWS], 0, (0.0, 0.0))
+    _product(runtime, x, w, bias, out, 0, (0.0, 0.0))
     return out
 
 
@@ -176,8 +201,9 @@ def gated(runtime, x: torch.Tensor, w: Mxfp4Matrix, act: str | int = "silu", bia
     _vector(bias, 2 * w.n, "the bias", x.device)
     code = ops.activation_code(act) if isinstance(act, str) else int(act)
     out = torch.empty(x.shape[0], w.n, dtype=torch.bfloat16, device=x.device)
-    for r in range(0, x.shape[0], FEW_ROWS):
-        _few(x[r:r + FEW_ROWS], w, bias, out[r:r + FEW_ROWS], code, constants)
+    if code <= 0:
+        raise ops.KernelError(f"mxfp4 gated product: activation {act!r} is no gate")
+    _product(runtime, x, w, bias, out, code, constants)
     return out
 
 
@@ -203,9 +229,10 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
     if not 1 <= top <= EXPERT_TOP or not 1 <= E <= 1024:
         raise ops.KernelError(f"mxfp4 experts: top-{top} of {E}; up to top-{EXPERT_TOP} of 1024 are implemented")
     out = torch.empty(rows, w_down.n, dtype=out_dtype or x.dtype, device=x.device)
-    for r in range(0, rows, EXPERT_ROWS):
-        _two_kernels(runtime, x[r:r + EXPERT_ROWS], ids[r:r + EXPERT_ROWS], wts[r:r + EXPERT_ROWS], w_first, w_down,
-                     code if gates == 2 else -code, weigh == "input", constants, out[r:r + EXPERT_ROWS])
+    if rows == 0:
+        return out
+    form = _two_kernels if rows <= EXPERT_ROWS and rows * top <= EXPERT_PAIRS else _sorted
+    form(runtime, x, ids, wts, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants, out)
     return out
 
 
@@ -220,3 +247,32 @@ def _two_kernels(runtime, x, ids, wts, w_first, w_down, act: int, before: bool, 
     _check(lib().tl_mxfp4_experts_second(a.data_ptr(), ld, w_down.codes.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), out.stride(0), rows,
                                          w_down.n, inter, ids.data_ptr(), top, E, ops.dtype_code(out.dtype), runtime.status.data_ptr(),
                                          ops.stream()), "mxfp4_experts_second")
+
+
+def _sorted(runtime, x, ids, wts, w_first, w_down, act: int, before: bool, constants, out) -> None:
+    """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
+    rows, top = ids.shape
+    E, inter, hidden, pairs, k = w_down.groups, w_down.k, w_down.n, rows * top, x.shape[1]
+    tile = token_tile(1.4 * pairs / E)
+    tiles = min(pairs // tile + E, pairs)
+    ints = torch.empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32, device=x.device)
+    counts = ints.data_ptr()
+    order = counts + 4 * E
+    place = order + 4 * pairs
+    group, row0, n_rows = (place + 4 * (pairs + i * tiles) for i in range(3))
+    n_tiles = n_rows + 4 * tiles
+    _check(lib().tl_mxfp4_plan(ids.data_ptr(), pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, runtime.status.data_ptr(),
+                               ops.stream()), "mxfp4_plan")
+    xs = torch.empty(pairs, k, dtype=torch.bfloat16, device=x.device)
+    _check(lib().tl_mxfp4_gather(x.data_ptr(), x.stride(0), order, top, xs.data_ptr(), pairs, k, ops.stream()), "mxfp4_gather")
+    ld = -(-inter // 8) * 8
+    a = torch.empty(pairs, ld, dtype=torch.bfloat16, device=x.device)
+    y = torch.empty(pairs, hidden, dtype=torch.float32, device=x.device)
+    tail = (tile, 1, group, row0, n_rows, n_tiles, tiles)
+    _check(lib().tl_mxfp4_tc(xs.data_ptr(), k, pairs, w_first.codes.data_ptr(), w_first.scales.data_ptr(), None, a.data_ptr(), ld, pairs, inter, k,
+                             act, *constants, ops.BF16, *tail, wts.data_ptr() if before else None, order if before else None,
+                             runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
+    _check(lib().tl_mxfp4_tc(a.data_ptr(), ld, pairs, w_down.codes.data_ptr(), w_down.scales.data_ptr(), None, y.data_ptr(), hidden, pairs, hidden,
+                             inter, 0, 0.0, 0.0, ops.FP32, *tail, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
+    _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids.data_ptr(), None if before else wts.data_ptr(), out.data_ptr(), ops.dtype_code(out.dtype),
+                              rows, hidden, top, E, ops.stream()), "mxfp4_sum")
