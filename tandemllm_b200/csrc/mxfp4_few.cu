@@ -36,7 +36,21 @@ __device__ __forceinline__ uint4 load16(const void* p, bool valid) {
       : "l"(p), "r"((int)valid));
   return v;
 }
-// The same for weights, which no kernel writes and no other CTA reads.
+// Eight numbers of a token row from its element k on, zeros past K and where not valid. WHOLE: rows begin at multiples of 16 bytes and K is a
+// multiple of 8, so the eight are in or out; else they are fetched one by one.
+template <bool WHOLE>
+__device__ __forceinline__ uint4 load_row(const bf16* row, int k, int K, bool valid) {
+  if constexpr (WHOLE) return load16(row + k, valid && k < K);
+  uint32_t v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const bool lo = valid && k + 2 * i < K, hi = valid && k + 2 * i + 1 < K;
+    const uint32_t a = lo ? __bfloat16_as_ushort(row[k + 2 * i]) : 0u, b = hi ? __bfloat16_as_ushort(row[k + 2 * i + 1]) : 0u;
+    v[i] = a | b << 16;
+  }
+  return make_uint4(v[0], v[1], v[2], v[3]);
+}
+// 16 bytes of weights, which no kernel writes and no other CTA reads.
 __device__ __forceinline__ uint4 load_codes(const uint8_t* p, bool valid) {
   uint4 v;
   asm volatile(
@@ -112,7 +126,7 @@ __device__ __forceinline__ void keep(float (&part)[RT][16][8 * NT + 1], const fl
 }
 
 // 16 outputs a CTA for up to 8 NT rows. `gate` != 0: the second matrix holds the up rows, and `bias` its numbers behind the gate's.
-template <int NT, bool GATED, int UNROLL, typename TOut>
+template <int NT, bool GATED, bool WHOLE, int UNROLL, typename TOut>
 __global__ void __launch_bounds__(WARPS * 32) few_kernel(const bf16* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
                                                          const uint8_t* __restrict__ scales, const float* __restrict__ bias, TOut* __restrict__ out,
                                                          long long ldc, int M, int N, int K, int act, float ga0, float ga1) {
@@ -139,9 +153,9 @@ __global__ void __launch_bounds__(WARPS * 32) few_kernel(const bf16* __restrict_
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
         const int m = j * 8 + g, k = c * TILE_K + t * BLOCK;
-        const bf16* row = x + (long long)(m < M ? m : 0) * ldx + k;
+        const bf16* row = x + (long long)(m < M ? m : 0) * ldx;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[u][j][i] = load16(row + 8 * i, m < M && k + 8 * i < K);       // (K a multiple of 8: all or none)
+        for (int i = 0; i < 4; ++i) b[u][j][i] = load_row<WHOLE>(row, k + 8 * i, K, m < M);
       }
     }
 #pragma unroll
@@ -240,7 +254,7 @@ __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids
 
 // grid (16 outputs, items at most): a CTA takes an item's expert and the rows that chose it. `out` [pairs, ldc], outputs up to ldc (those
 // past N come from rows of zeros). `before`: the pair's weight multiplies the sums, in front of the activation, else what comes of them.
-template <bool GATED, int UNROLL>
+template <bool GATED, bool WHOLE, int UNROLL>
 __global__ void __launch_bounds__(WARPS * 32) first_kernel(const bf16* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
                                                            const uint8_t* __restrict__ scales, bf16* __restrict__ out, int ldc, int N, int K,
                                                            const int* __restrict__ ids, const float* __restrict__ wts, int before, int pairs,
@@ -273,7 +287,7 @@ __global__ void __launch_bounds__(WARPS * 32) first_kernel(const bf16* __restric
         load_fragment(f[u][r], codes, scales, at, ok_hi ? at + k_tiles : at, g, t, in, in && ok_hi);
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) b[u][0][i] = load16(row + k + 8 * i, pair >= 0 && k + 8 * i < K);
+      for (int i = 0; i < 4; ++i) b[u][0][i] = load_row<WHOLE>(row, k + 8 * i, K, pair >= 0);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u)
@@ -358,24 +372,29 @@ using namespace tl;
 extern "C" int tl_mxfp4_few(const void* x, long long ldx, const void* codes, const void* scales, const float* bias, void* out, long long ldc,
                             int M, int N, int K, int act, float a0, float a1, int out_dtype, cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
-  TL_REQUIRE(M >= 1 && M <= 32 && N >= 1 && K >= 1 && K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0,
-             "mxfp4 product of few rows: %d rows x (%d x %d), row stride %lld", M, N, K, ldx);
+  TL_REQUIRE(M >= 1 && M <= 32 && N >= 1 && K >= 1, "mxfp4 product of few rows: %d rows x (%d x %d)", M, N, K);
   TL_REQUIRE(act <= 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 product: gate activation %d is none (nor an ungated one, negated)", act);
   TL_REQUIRE(act <= 0 || out_dtype == TL_BF16, "mxfp4 product: gated outputs of type %d", out_dtype);
   const dim3 grid(ceil_div(N, 16)), block(mx::WARPS * 32);
   const int nt = ceil_div(M, 8);
-#define TL_FEW(NT_, G_, U_, T_)                                                                                               \
-  return (int)launch_chained(mx::few_kernel<NT_, G_, U_, T_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes, \
+  const bool whole = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
+#define TL_FEW(NT_, G_, W_, U_, T_)                                                                                               \
+  return (int)launch_chained(mx::few_kernel<NT_, G_, W_, U_, T_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes, \
                              (const uint8_t*)scales, bias, (T_*)out, ldc, M, N, K, act, a0, a1)
-#define TL_FEW_(NT_, U_, G_U_)                            \
-  do {                                                    \
-    if (act > 0) TL_FEW(NT_, true, G_U_, bf16);           \
-    if (out_dtype == TL_FP32) TL_FEW(NT_, false, U_, float); \
-    TL_FEW(NT_, false, U_, bf16);                         \
+#define TL_FEW_(NT_, W_, U_)                                     \
+  do {                                                           \
+    if (act > 0) TL_FEW(NT_, true, W_, U_, bf16);                \
+    if (out_dtype == TL_FP32) TL_FEW(NT_, false, W_, U_, float); \
+    TL_FEW(NT_, false, W_, U_, bf16);                            \
   } while (0)
-  if (nt == 1) TL_FEW_(1, 2, 2);
-  if (nt == 2) TL_FEW_(2, 1, 1);
-  TL_FEW_(4, 1, 1);
+  if (whole) {
+    if (nt == 1) TL_FEW_(1, true, 2);
+    if (nt == 2) TL_FEW_(2, true, 1);
+    TL_FEW_(4, true, 1);
+  }
+  if (nt == 1) TL_FEW_(1, false, 1);
+  if (nt == 2) TL_FEW_(2, false, 1);
+  TL_FEW_(4, false, 1);
 #undef TL_FEW_
 #undef TL_FEW
 }
@@ -388,16 +407,19 @@ extern "C" int tl_mxfp4_experts_first(const void* x, long long ldx, const void* 
   if (rows == 0 || N == 0) return 0;
   TL_REQUIRE(rows >= 1 && rows <= mx::MAX_ROWS && top >= 1 && rows * top <= mx::MAX_PAIRS && top <= 32 && experts >= 1 && experts <= 1024,
              "mxfp4 experts: %d rows, top-%d of %d", rows, top, experts);
-  TL_REQUIRE(N >= 1 && K >= 1 && K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0 && ldc == ceil_div(N, 8) * 8,
-             "mxfp4 experts: %d x %d, row strides %lld and %d", N, K, ldx, ldc);
+  TL_REQUIRE(N >= 1 && K >= 1 && ldc == ceil_div(N, 8) * 8, "mxfp4 experts: %d x %d, row stride %d", N, K, ldc);
   TL_REQUIRE(act < 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 experts: gate activation %d is none (nor an ungated one, negated)", act);
   const dim3 grid(ceil_div(N, 16), rows * top), block(mx::WARPS * 32);
-#define TL_FIRST(G_, U_)                                                                                                                      \
-  return (int)launch_chained(mx::first_kernel<G_, U_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes,                    \
+#define TL_FIRST(G_, W_, U_)                                                                                                                      \
+  return (int)launch_chained(mx::first_kernel<G_, W_, U_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes,                    \
                              (const uint8_t*)scales, (bf16*)out, ldc, N, K, ids, wts, before, rows * top, top, experts, act < 0 ? -act : act, \
                              a0, a1, status)
-  if (act > 0) TL_FIRST(true, 2);
-  TL_FIRST(false, 2);
+  if (K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0) {
+    if (act > 0) TL_FIRST(true, true, 2);
+    TL_FIRST(false, true, 2);
+  }
+  if (act > 0) TL_FIRST(true, false, 1);
+  TL_FIRST(false, false, 1);
 #undef TL_FIRST
 }
 

@@ -83,15 +83,23 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restric
   }
 }
 
-// to[i] = from[sorted[i] / top], 16 bytes a thread.
-__global__ void __launch_bounds__(256) gather_kernel(const uint4* __restrict__ from, long long ld, const int* __restrict__ sorted, int top,
-                                                     uint4* __restrict__ to, int pieces, long long total) {
+// to[i] = from[order[i] / div] (without an order from[i]), eight numbers a thread; those past `width` stay as they are.
+template <bool WHOLE>
+__global__ void __launch_bounds__(256) gather_kernel(const bf16* __restrict__ from, long long ld, const int* __restrict__ order, int div,
+                                                     bf16* __restrict__ to, int ld_to, int width, long long total) {
   chain_next();
   chain_wait();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
   if (i >= total) return;
-  const long long row = i / pieces;
-  to[i] = from[(long long)(sorted[row] / top) * ld + (i - row * pieces)];
+  const long long row = i / (ld_to / 8);
+  const int at = (int)(i - row * (ld_to / 8)) * 8;
+  const bf16* src = from + (order ? order[row] / div : row) * ld + at;
+  bf16* dst = to + row * ld_to + at;
+  if (WHOLE) {
+    *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(src);
+  } else {
+    for (int j = 0; j < 8 && at + j < width; ++j) dst[j] = src[j];
+  }
 }
 
 // out[r] = sum over r's slots, one after the other, of wts * y[place]; without weights the rows as they are. Four outputs a thread.
@@ -150,15 +158,21 @@ extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_ro
                              place, tile_group, tile_row0, tile_rows, n_tiles, status);
 }
 
-// x [*, width] bfloat16 (row stride ldx), to [pairs, width]; width and ldx multiples of 8, pointers of 16 bytes.
-extern "C" int tl_mxfp4_gather(const void* x, long long ldx, const int* sorted, int top, void* to, int pairs, int width, cudaStream_t stream) {
-  if (pairs == 0 || width == 0) return 0;
-  TL_REQUIRE(pairs > 0 && top >= 1 && width % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0 && ((uintptr_t)to % 16) == 0,
-             "mxfp4 experts: rows of %d numbers, %lld apart", width, ldx);
-  const long long total = (long long)pairs * (width / 8), blocks = ceil_div64(total, 256);
-  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4 experts: %d pairs of %d numbers are too many", pairs, width);
-  return (int)launch_chained(mx::gather_kernel, dim3((unsigned)blocks), dim3(256), 0, stream, (const uint4*)x, ldx / 8, sorted, top, (uint4*)to,
-                             width / 8, total);
+// to [rows, width] bfloat16 (row stride ld_to, a multiple of 8, 16-byte aligned) from x (row stride ldx): row i is x[order[i] / div], or x[i].
+extern "C" int tl_mxfp4_gather(const void* x, long long ldx, const int* order, int div, void* to, long long ld_to, int rows, int width,
+                               cudaStream_t stream) {
+  if (rows == 0 || width == 0) return 0;
+  TL_REQUIRE(rows > 0 && div >= 1 && width > 0 && ld_to % 8 == 0 && ld_to >= width && ld_to <= 0x7FFFFFF8 && ((uintptr_t)to % 16) == 0,
+             "mxfp4 product: rows of %d numbers to rows %lld apart", width, ld_to);
+  const long long total = (long long)rows * (ld_to / 8), blocks = ceil_div64(total, 256);
+  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4 product: %d rows of %d numbers are too many", rows, width);
+  const bool whole = width % 8 == 0 && width == ld_to && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
+#define TL_GATHER(W_)                                                                                                                       \
+  return (int)launch_chained(mx::gather_kernel<W_>, dim3((unsigned)blocks), dim3(256), 0, stream, (const bf16*)x, ldx, order, div, (bf16*)to, \
+                             (int)ld_to, width, total)
+  if (whole) TL_GATHER(true);
+  TL_GATHER(false);
+#undef TL_GATHER
 }
 
 // y [pairs, N] 32-bit, out [rows, N] contiguous, bfloat16 or 32-bit.

@@ -25,7 +25,7 @@ BLOCK = 32                      # values a scale
 TILE_ROWS, TILE_K = 8, 128      # the layout's tiles
 FEW_ROWS = 32                   # rows up to which a product goes to the register-only kernel
 EXPERT_ROWS, EXPERT_PAIRS, EXPERT_TOP = 8, 256, 32      # the experts' two-kernel form
-BYTES_A_VALUE = 17 / 32
+TILE_CODES, TILE_BYTES = TILE_ROWS * TILE_K // 2, TILE_ROWS * TILE_K * 17 // 32
 
 _SIGNATURES = {
     "tl_mxfp4_quantize": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -39,7 +39,7 @@ _SIGNATURES = {
     "tl_mxfp4_tc": [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_float,
                     c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
     "tl_mxfp4_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
-    "tl_mxfp4_gather": [c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_int, c_int, c_void_p],
+    "tl_mxfp4_gather": [c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_void_p],
     "tl_mxfp4_sum": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
 }
 _lib = None
@@ -67,38 +67,42 @@ def _check(code: int, what: str, kernels: int = 1) -> None:
     raise ops.KernelError(f"{what}: CUDA error {code}: {ops.core().tl_cuda_error_string(code).decode()}")
 
 
-def _here(device: torch.device, what: str) -> None:
-    if device.type != "cuda":
-        raise ops.KernelError(f"{what} is on {device}; the kernels run on CUDA tensors only")
-    if device.index != torch.cuda.current_device():
-        raise ops.KernelError(f"{what} is on {device}, the current device is cuda:{torch.cuda.current_device()}")
+def _here(t: torch.Tensor, what: str) -> int:
+    """The number of the current device, which `t` has to be on."""
+    index = t.get_device()
+    if index < 0:
+        raise ops.KernelError(f"{what} is on {t.device}; the kernels run on CUDA tensors only")
+    if index != torch._C._cuda_getDevice():
+        raise ops.KernelError(f"{what} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    return index
 
 
 class Mxfp4Matrix:
-    """`groups` matrices [n, k] in 4-bit blocks: codes uint8 [groups, n / 8, k / 128, 512] and scales uint8 [groups, n / 8, k / 128, 32]
-    in the kernels' layout (csrc/mxfp4.cuh), both sizes rounded up. `shape` is the shape of the tensor it was made of."""
+    """`groups` matrices [n, k] in 4-bit blocks, in the kernels' layout (csrc/mxfp4.cuh): `data` (uint8) holds the codes of all tiles of 8 rows by
+    128 k, both sizes rounded up, and behind them their scales. `shape` is the shape of the tensor it was made of."""
 
-    def __init__(self, codes: torch.Tensor, scales: torch.Tensor, shape: tuple[int, ...]):
-        self.codes, self.scales, self.shape = codes, scales, tuple(int(d) for d in shape)
-        self.groups, self.n, self.k = (1 if len(shape) == 2 else self.shape[0]), self.shape[-2], self.shape[-1]
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+    def __init__(self, data: torch.Tensor, shape: tuple[int, ...]):
+        self.data, self.shape, self.device = data, tuple(shape), data.device
+        self.groups, self.n, self.k = (1 if len(shape) == 2 else shape[0]), shape[-2], shape[-1]
+        tiles = self.groups * -(-self.n // TILE_ROWS) * -(-self.k // TILE_K)
+        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != tiles * TILE_BYTES:
+            raise ops.KernelError(f"mxfp4: {data.numel()} bytes ({data.dtype}) for a matrix of shape {self.shape}")
+        self.index, self.codes, self.scales = data.get_device(), data.data_ptr(), data.data_ptr() + tiles * TILE_CODES
 
     @property
     def nbytes(self) -> int:
-        return self.codes.numel() + self.scales.numel()
+        return self.data.numel()
 
     def numel(self) -> int:
         return self.groups * self.n * self.k
 
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values as a plain tensor of `shape`, exact in either dtype."""
-        _here(self.device, "the matrix")
+        code = ops.dtype_code(dtype)
+        _here(self.data, "the matrix")
         out = torch.empty(self.shape, dtype=dtype, device=self.device)
-        _check(lib().tl_mxfp4_values(self.codes.data_ptr(), self.scales.data_ptr(), out.data_ptr(), ops.dtype_code(dtype), self.groups, self.n,
-                                     self.k, ops.stream()), "mxfp4_values", kernels=int(out.numel() > 0))
+        _check(lib().tl_mxfp4_values(self.codes, self.scales, out.data_ptr(), code, self.groups, self.n, self.k, ops.stream()), "mxfp4_values",
+               kernels=int(out.numel() > 0))
         return out
 
 
@@ -109,47 +113,59 @@ def quantize(w: torch.Tensor) -> Mxfp4Matrix:
     if w.dim() not in (2, 3):
         raise ops.KernelError(f"mxfp4: a tensor of shape {tuple(w.shape)}; [n, k] or [groups, n, k] is wanted")
     code = ops.dtype_code(w.dtype)
-    _here(w.device, "the matrix")
-    if w.stride(-1) != 1 and w.shape[-1] > 1:
+    _here(w, "the matrix")
+    shape, stride = w.shape, w.stride()
+    if stride[-1] != 1 and shape[-1] > 1:
         w = w.contiguous()
-    groups, (n, k) = (1 if w.dim() == 2 else w.shape[0]), w.shape[-2:]
-    tiles = (groups, -(-n // TILE_ROWS), -(-k // TILE_K))
-    codes = torch.empty(*tiles, TILE_ROWS * TILE_K // 2, dtype=torch.uint8, device=w.device)
-    scales = torch.empty(*tiles, TILE_ROWS * TILE_K // BLOCK, dtype=torch.uint8, device=w.device)
-    _check(lib().tl_mxfp4_quantize(w.data_ptr(), w.stride(-2), w.stride(0) if w.dim() == 3 else 0, code, codes.data_ptr(), scales.data_ptr(),
-                                   groups, n, k, ops.stream()), "mxfp4_quantize", kernels=int(w.numel() > 0))
-    return Mxfp4Matrix(codes, scales, tuple(w.shape))
+        stride = w.stride()
+    groups, n, k = (1, *shape) if len(shape) == 2 else shape
+    data = torch.empty(groups * -(-n // TILE_ROWS) * -(-k // TILE_K) * TILE_BYTES, dtype=torch.uint8, device=w.device)
+    m = Mxfp4Matrix(data, shape)
+    _check(lib().tl_mxfp4_quantize(w.data_ptr(), stride[-2], stride[0] if len(shape) == 3 else 0, code, m.codes, m.scales, groups, n, k,
+                                   ops.stream()), "mxfp4_quantize", kernels=int(data.numel() > 0))
+    return m
 
 
-def _rows(x: torch.Tensor, w: Mxfp4Matrix) -> torch.Tensor:
-    """x as the kernels read it: rows of bfloat16 numbers that begin at multiples of 16 bytes, a multiple of 8 of them."""
+def _rows(x: torch.Tensor, w: Mxfp4Matrix) -> tuple[int, int]:
+    """(rows, elements from one to the next) of x, which has to be what the products take."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ops.KernelError(f"mxfp4 product: rows of shape {tuple(x.shape)} with a matrix of shape {w.shape}")
-    if x.dtype != torch.bfloat16:
+    if x.dtype is not torch.bfloat16:
         raise ops.KernelError(f"mxfp4 product: rows of {x.dtype}; bfloat16 is implemented")
-    _here(x.device, "x")
-    if w.device != x.device:
+    if _here(x, "x") != w.index:
         raise ops.KernelError(f"mxfp4 product: rows on {x.device}, the matrix on {w.device}")
-    if w.k % 8 or x.stride(-1) != 1 or x.stride(0) % 8 or x.data_ptr() % 16:
-        x = torch.nn.functional.pad(x, (0, -w.k % 8)).contiguous()
-        if x.data_ptr() % 16:
-            x = x.clone()
-    return x
+    ld, inner = x.stride()
+    if inner != 1 and w.k > 1:
+        raise ops.KernelError(f"mxfp4 product: rows of {w.k} elements that lie {inner} apart; unit inner stride is implemented")
+    return x.shape[0], ld
 
 
-def _vector(v: torch.Tensor | None, size: int, name: str, device) -> None:
+def _boxed(x: torch.Tensor, rows: int, k: int, ld: int, order: int | None = None, div: int = 1) -> tuple[torch.Tensor, int]:
+    """(x, its row stride) for the tensor-core product: as it is where its rows begin at multiples of 16 bytes, else a copy that does. With
+    `order` (`rows` row numbers on the device, to be divided by `div`) a copy of these rows."""
+    if order is None and ld % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x, ld
+    wide = -(-k // 8) * 8
+    copy = torch.empty(rows, wide, dtype=torch.bfloat16, device=x.device)
+    _check(lib().tl_mxfp4_gather(x.data_ptr(), ld, order, div, copy.data_ptr(), wide, rows, k, ops.stream()), "mxfp4_gather")
+    return copy, wide
+
+
+def _vector(v: torch.Tensor | None, size: int, name: str, index: int) -> int | None:
     if v is None:
-        return
-    if v.dtype != torch.float32 or not v.is_contiguous() or v.numel() != size or v.device != device:
-        raise ops.KernelError(f"mxfp4 product: {name} is {v.dtype} {tuple(v.shape)} on {v.device}; {size} contiguous float32 numbers on {device}")
+        return None
+    if v.dtype is not torch.float32 or v.numel() != size or v.get_device() != index or not v.is_contiguous():
+        raise ops.KernelError(f"mxfp4 product: {name} is {v.dtype} {tuple(v.shape)} on {v.device}; {size} contiguous float32 numbers on "
+                              f"cuda:{index} are wanted")
+    return v.data_ptr()
 
 
-def _output(out, rows: int, n: int, dtype: torch.dtype, device) -> torch.Tensor:
+def _output(out, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return torch.empty(rows, n, dtype=dtype, device=device)
-    if tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != device or out.stride(-1) != 1:
+        return x.new_empty(rows, n, dtype=dtype)
+    if tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != x.device or (out.stride(1) != 1 and n > 1):
         raise ops.KernelError(f"mxfp4 product: an output of {out.dtype} {tuple(out.shape)} on {out.device}; {dtype} ({rows}, {n}) with unit inner "
-                              f"stride on {device}")
+                              f"stride on {x.device}")
     return out
 
 
@@ -163,20 +179,21 @@ def splits_of(ctas: int, k: int, sms: int) -> int:
     return max(1, min(2 * sms // ctas, -(-k // TILE_K) // 2, 8))
 
 
-def _product(runtime, x, w: Mxfp4Matrix, bias, out, act: int, constants) -> None:
+def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, out: torch.Tensor, act: int, constants) -> None:
     """out = the product of x's rows with w: act 0 plain, a gate's code gated, negated an activation on a plain product."""
-    M = x.shape[0]
-    if M == 0:
+    if rows == 0:
         return
-    if M <= FEW_ROWS:
-        _check(lib().tl_mxfp4_few(x.data_ptr(), x.stride(0), w.codes.data_ptr(), w.scales.data_ptr(), ops.ptr(bias), out.data_ptr(), out.stride(0),
-                                  M, w.n, x.shape[1], act, *constants, ops.dtype_code(out.dtype), ops.stream()), "mxfp4_few")
+    code = ops.dtype_code(out.dtype)
+    if rows <= FEW_ROWS:
+        _check(lib().tl_mxfp4_few(x.data_ptr(), ld, w.codes, w.scales, bias, out.data_ptr(), out.stride(0), rows, w.n, w.k, act, *constants, code,
+                                  ops.stream()), "mxfp4_few")
         return
-    bn = token_tile(M)
-    ctas = -(-w.n // (64 if act > 0 else 128)) * -(-M // bn)
-    _check(lib().tl_mxfp4_tc(x.data_ptr(), x.stride(0), M, w.codes.data_ptr(), w.scales.data_ptr(), ops.ptr(bias), out.data_ptr(), out.stride(0),
-                             M, w.n, x.shape[1], act, *constants, ops.dtype_code(out.dtype), bn, splits_of(ctas, x.shape[1], ops.sm_count()),
-                             None, None, None, None, 0, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
+    x, ld = _boxed(x, rows, w.k, ld)
+    bn = token_tile(rows)
+    ctas = -(-w.n // (64 if act > 0 else 128)) * -(-rows // bn)
+    _check(lib().tl_mxfp4_tc(x.data_ptr(), ld, rows, w.codes, w.scales, bias, out.data_ptr(), out.stride(0), rows, w.n, w.k, act, *constants, code,
+                             bn, splits_of(ctas, w.k, ops.sm_count()), None, None, None, None, 0, None, None, runtime.status.data_ptr(),
+                             ops.stream()), "mxfp4_tc")
 
 
 def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
@@ -184,11 +201,18 @@ def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None =
     """x [rows, k] times the one matrix w [n, k], plus `bias` (32-bit, [n]), in `out_dtype` (default: x's)."""
     if w.groups != 1:
         raise ops.KernelError(f"mxfp4 product: a stack of {w.groups} matrices where one is wanted")
-    x = _rows(x, w)
-    _vector(bias, w.n, "the bias", x.device)
-    out = _output(out, x.shape[0], w.n, out_dtype or (out.dtype if out is not None else x.dtype), x.device)
-    _product(runtime, x, w, bias, out, 0, (0.0, 0.0))
+    rows, ld = _rows(x, w)
+    b = _vector(bias, w.n, "the bias", w.index)
+    out = _output(out, rows, w.n, out_dtype or (out.dtype if out is not None else x.dtype), x)
+    _product(runtime, x, rows, ld, w, b, out, 0, (0.0, 0.0))
     return out
+
+
+def _gate(act: str | int) -> int:
+    code = ops.activation_code(act) if isinstance(act, str) else int(act)
+    if code <= 0:
+        raise ops.KernelError(f"mxfp4 product: activation {act!r} is none of {', '.join(ops.ACTIVATIONS)}")
+    return code
 
 
 def gated(runtime, x: torch.Tensor, w: Mxfp4Matrix, act: str | int = "silu", bias: torch.Tensor | None = None,
@@ -197,13 +221,10 @@ def gated(runtime, x: torch.Tensor, w: Mxfp4Matrix, act: str | int = "silu", bia
     [2 n]). `act`: a gate of `ops.ACTIVATIONS`, by name or code; `constants`: those of one that has some."""
     if w.groups != 2:
         raise ops.KernelError(f"mxfp4 gated product: {w.groups} matrices where a gate and an up matrix are wanted")
-    x = _rows(x, w)
-    _vector(bias, 2 * w.n, "the bias", x.device)
-    code = ops.activation_code(act) if isinstance(act, str) else int(act)
-    out = torch.empty(x.shape[0], w.n, dtype=torch.bfloat16, device=x.device)
-    if code <= 0:
-        raise ops.KernelError(f"mxfp4 gated product: activation {act!r} is no gate")
-    _product(runtime, x, w, bias, out, code, constants)
+    rows, ld = _rows(x, w)
+    b = _vector(bias, 2 * w.n, "the bias", w.index)
+    out = x.new_empty(rows, w.n)
+    _product(runtime, x, rows, ld, w, b, out, _gate(act), constants)
     return out
 
 
@@ -215,64 +236,57 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
     down( act(gate x) * (up x) ); or [E, inter, hidden] without gates: down( act(up x) ). `weigh` "input": the weight multiplies what the
     first product makes of x, in front of the activation, and the experts' rows are added as they are. An id outside 0 .. E - 1 adds
     nothing and is recorded in the runtime's status word."""
-    E, gates = w_down.groups, w_first.groups // max(w_down.groups, 1)
-    if gates not in (1, 2) or w_first.groups != gates * E or (w_first.n, w_first.k) != (w_down.k, w_down.n):
-        raise ops.KernelError(f"mxfp4 experts: matrices of shapes {w_first.shape} and {w_down.shape}")
+    E = w_down.groups
+    gates = w_first.groups // max(E, 1)
+    if gates not in (1, 2) or w_first.groups != gates * E or w_first.n != w_down.k or w_first.k != w_down.n or w_first.index != w_down.index:
+        raise ops.KernelError(f"mxfp4 experts: matrices of shapes {w_first.shape} on {w_first.device} and {w_down.shape} on {w_down.device}")
     if weigh not in ("input", "output"):
         raise ops.KernelError(f"experts weighed at their {weigh!r}: input or output")
-    code = ops.activation_code(act) if isinstance(act, str) else int(act)
-    x = _rows(x, w_first)
-    rows, top = ids.shape
-    ops._need(ids, torch.int32, "expert ids"); ops._need(wts, torch.float32, "expert weights")
-    if tuple(wts.shape) != (rows, top) or rows != x.shape[0] or ids.device != x.device or wts.device != x.device:
-        raise ops.KernelError(f"mxfp4 experts: {tuple(x.shape)} rows with ids {tuple(ids.shape)} and weights {tuple(wts.shape)}")
+    rows, ld = _rows(x, w_first)
+    if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != rows or ids.get_device() != w_down.index or not ids.is_contiguous():
+        raise ops.KernelError(f"mxfp4 experts: ids {ids.dtype} {tuple(ids.shape)} on {ids.device}; contiguous int32 [{rows}, top] on {x.device} is wanted")
+    top = ids.shape[1]
+    w = _vector(wts, rows * top, "the experts' weights", w_down.index)
     if not 1 <= top <= EXPERT_TOP or not 1 <= E <= 1024:
         raise ops.KernelError(f"mxfp4 experts: top-{top} of {E}; up to top-{EXPERT_TOP} of 1024 are implemented")
-    out = torch.empty(rows, w_down.n, dtype=out_dtype or x.dtype, device=x.device)
-    if rows == 0:
-        return out
-    form = _two_kernels if rows <= EXPERT_ROWS and rows * top <= EXPERT_PAIRS else _sorted
-    form(runtime, x, ids, wts, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants, out)
+    code = _gate(act)
+    out = x.new_empty(rows, w_down.n, dtype=out_dtype)
+    if rows:
+        form = _two_kernels if rows <= EXPERT_ROWS and rows * top <= EXPERT_PAIRS else _sorted
+        form(runtime, x, rows, ld, ids.data_ptr(), top, w, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants, out)
     return out
 
 
-def _two_kernels(runtime, x, ids, wts, w_first, w_down, act: int, before: bool, constants, out) -> None:
-    rows, top = ids.shape
-    E, inter = w_down.groups, w_down.k
-    ld = -(-inter // 8) * 8
-    a = torch.empty(rows * top, ld, dtype=torch.bfloat16, device=x.device)
-    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), x.stride(0), w_first.codes.data_ptr(), w_first.scales.data_ptr(), a.data_ptr(), ld, rows,
-                                        inter, x.shape[1], ids.data_ptr(), wts.data_ptr(), int(before), top, E, act, *constants,
-                                        runtime.status.data_ptr(), ops.stream()), "mxfp4_experts_first")
-    _check(lib().tl_mxfp4_experts_second(a.data_ptr(), ld, w_down.codes.data_ptr(), w_down.scales.data_ptr(), out.data_ptr(), out.stride(0), rows,
-                                         w_down.n, inter, ids.data_ptr(), top, E, ops.dtype_code(out.dtype), runtime.status.data_ptr(),
-                                         ops.stream()), "mxfp4_experts_second")
+def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
+    E, inter, status, stream = w_down.groups, w_down.k, runtime.status.data_ptr(), ops.stream()
+    wide = -(-inter // 8) * 8
+    a = x.new_empty(rows * top, wide)
+    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, a.data_ptr(), wide, rows, inter, w_first.k, ids, wts,
+                                        int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
+    _check(lib().tl_mxfp4_experts_second(a.data_ptr(), wide, w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter, ids, top,
+                                         E, ops.dtype_code(out.dtype), status, stream), "mxfp4_experts_second")
 
 
-def _sorted(runtime, x, ids, wts, w_first, w_down, act: int, before: bool, constants, out) -> None:
+def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
-    rows, top = ids.shape
-    E, inter, hidden, pairs, k = w_down.groups, w_down.k, w_down.n, rows * top, x.shape[1]
+    E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
     tile = token_tile(1.4 * pairs / E)
     tiles = min(pairs // tile + E, pairs)
-    ints = torch.empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32, device=x.device)
+    ints = x.new_empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32)
     counts = ints.data_ptr()
     order = counts + 4 * E
     place = order + 4 * pairs
     group, row0, n_rows = (place + 4 * (pairs + i * tiles) for i in range(3))
     n_tiles = n_rows + 4 * tiles
-    _check(lib().tl_mxfp4_plan(ids.data_ptr(), pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, runtime.status.data_ptr(),
-                               ops.stream()), "mxfp4_plan")
-    xs = torch.empty(pairs, k, dtype=torch.bfloat16, device=x.device)
-    _check(lib().tl_mxfp4_gather(x.data_ptr(), x.stride(0), order, top, xs.data_ptr(), pairs, k, ops.stream()), "mxfp4_gather")
-    ld = -(-inter // 8) * 8
-    a = torch.empty(pairs, ld, dtype=torch.bfloat16, device=x.device)
-    y = torch.empty(pairs, hidden, dtype=torch.float32, device=x.device)
+    _check(lib().tl_mxfp4_plan(ids, pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, status, stream), "mxfp4_plan")
+    xs, ld = _boxed(x, pairs, w_first.k, ld, order, top)
+    wide = -(-inter // 8) * 8
+    a = x.new_empty(pairs, wide)
+    y = x.new_empty(pairs, hidden, dtype=torch.float32)
     tail = (tile, 1, group, row0, n_rows, n_tiles, tiles)
-    _check(lib().tl_mxfp4_tc(xs.data_ptr(), k, pairs, w_first.codes.data_ptr(), w_first.scales.data_ptr(), None, a.data_ptr(), ld, pairs, inter, k,
-                             act, *constants, ops.BF16, *tail, wts.data_ptr() if before else None, order if before else None,
-                             runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
-    _check(lib().tl_mxfp4_tc(a.data_ptr(), ld, pairs, w_down.codes.data_ptr(), w_down.scales.data_ptr(), None, y.data_ptr(), hidden, pairs, hidden,
-                             inter, 0, 0.0, 0.0, ops.FP32, *tail, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
-    _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids.data_ptr(), None if before else wts.data_ptr(), out.data_ptr(), ops.dtype_code(out.dtype),
-                              rows, hidden, top, E, ops.stream()), "mxfp4_sum")
+    _check(lib().tl_mxfp4_tc(xs.data_ptr(), ld, pairs, w_first.codes, w_first.scales, None, a.data_ptr(), wide, pairs, inter, w_first.k, act,
+                             *constants, ops.BF16, *tail, wts if before else None, order if before else None, status, stream), "mxfp4_tc")
+    _check(lib().tl_mxfp4_tc(a.data_ptr(), wide, pairs, w_down.codes, w_down.scales, None, y.data_ptr(), hidden, pairs, hidden, inter, 0, 0.0, 0.0,
+                             ops.FP32, *tail, None, None, status, stream), "mxfp4_tc")
+    _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids, None if before else wts, out.data_ptr(), ops.dtype_code(out.dtype), rows, hidden, top, E,
+                              stream), "mxfp4_sum")

@@ -243,7 +243,7 @@ def test_refusals(runtime):
                 lambda: mxfp4.quantize(torch.ones(4, 64, dtype=torch.float16, device=DEV)), lambda: mxfp4.quantize(torch.ones(4, 64)),
                 lambda: m.values(torch.float16),
                 lambda: mxfp4.linear(runtime, x.float(), m), lambda: mxfp4.linear(runtime, x[:, :32], m), lambda: mxfp4.linear(runtime, x[0], m),
-                lambda: mxfp4.linear(runtime, x.cpu(), m), lambda: mxfp4.linear(runtime, x, pair),
+                lambda: mxfp4.linear(runtime, x.cpu(), m), lambda: mxfp4.linear(runtime, x.repeat(1, 2)[:, ::2], m), lambda: mxfp4.linear(runtime, x, pair),
                 lambda: mxfp4.linear(runtime, x, m, torch.zeros(16, dtype=torch.bfloat16, device=DEV)),
                 lambda: mxfp4.linear(runtime, x, m, torch.zeros(15, device=DEV)), lambda: mxfp4.linear(runtime, x, m, out=x),
                 lambda: mxfp4.gated(runtime, x, m), lambda: mxfp4.gated(runtime, x, pair, "tanh"), lambda: mxfp4.gated(runtime, x, pair, "swish"),
