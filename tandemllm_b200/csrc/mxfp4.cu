@@ -23,95 +23,118 @@ __device__ __forceinline__ uint32_t encode4(float a0, float b0, float a1, float 
   return d;
 }
 
-template <typename T> struct Piece;                                 // 16 bytes of a row
-template <> struct Piece<float> { static constexpr int COUNT = 4; };
-template <> struct Piece<bf16> { static constexpr int COUNT = 8; };
+// Eight consecutive numbers of a row as they lie.
+template <typename T> struct Eight;
+template <> struct Eight<bf16> {
+  uint4 v;
+  __device__ __forceinline__ void load(const bf16* p) { v = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void get(float (&f)[8]) const { unpack8(v, f); }
+};
+template <> struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  }
+};
 
-// One warp a tile of 8 rows by 128 k: lane (g, t) takes block t of row g.
+// A block of 8 warps 8 rows, a warp every eighth of their tiles of 128 k, two rows at a time: 16 lanes a row, four lanes a block of values,
+// eight values and one word of codes a lane. Both sides of memory are then read and written in whole sectors.
+constexpr int CODER_WARPS = 8;
+struct Place {
+  unsigned row_tile, group;   // among all matrices' row tiles; the matrix
+  int row, k, at, scale_at;   // the lane's first row and, in a tile, its first value, the word of codes that holds it, its block's scale
+  __device__ __forceinline__ explicit Place(int row_tiles) {
+    row_tile = blockIdx.x;
+    group = row_tile / (unsigned)row_tiles;
+    const int lane = threadIdx.x & 31, piece = lane & 15;
+    row = (int)(row_tile - group * (unsigned)row_tiles) * TILE_ROWS + (lane >> 4);
+    k = piece * 8;
+    at = ((piece >> 2) * TILE_ROWS + (lane >> 4)) * 4 + (piece & 3);
+    scale_at = (lane >> 4) * (TILE_K / BLOCK) + (piece >> 2);
+  }
+};
+
 template <typename T, bool WHOLE>
-__global__ void __launch_bounds__(256) quantize_kernel(const T* __restrict__ w, long long ld, long long ld_group, uint8_t* __restrict__ codes,
-                                                       uint8_t* __restrict__ scales, int N, int K, int row_tiles, int k_tiles,
-                                                       long long tiles) {
-  const long long tile = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (tile >= tiles) return;
-  const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
-  const long long rows_at = tile / k_tiles;
-  const int k0 = (int)(tile - rows_at * k_tiles) * TILE_K + t * BLOCK;
-  const long long group = rows_at / row_tiles;
-  const int row = (int)(rows_at - group * row_tiles) * TILE_ROWS + g;
-  const T* from = w + group * ld_group + (long long)row * ld + k0;
-  float v[BLOCK];
-  if (WHOLE && row < N && k0 + BLOCK <= K) {
+__global__ void __launch_bounds__(CODER_WARPS * 32, 4) quantize_kernel(const T* __restrict__ w, long long ld, long long ld_group,
+                                                                    uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int N, int K,
+                                                                    int row_tiles, int k_tiles) {
+  const Place to(row_tiles);
+  const T* from = w + to.group * ld_group + (long long)to.row * ld + to.k;
+  for (int c = threadIdx.x >> 5; c < k_tiles; c += CODER_WARPS) {
+    const long long tile = (long long)to.row_tile * k_tiles + c;
+    const int left = K - c * TILE_K - to.k;
+    float v[4][8];
+    if (WHOLE && left >= 8 && to.row + 6 < N) {
+      Eight<T> e[4];                            // (all four loads on their way before the first is looked at)
 #pragma unroll
-    for (int i = 0; i < BLOCK; i += Piece<T>::COUNT) {
-      const uint4 u = *reinterpret_cast<const uint4*>(from + i);
-      if constexpr (sizeof(T) == 2) {
-        float f[8];
-        unpack8(u, f);
+      for (int i = 0; i < 4; ++i) e[i].load(from + 2 * i * ld + c * TILE_K);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[i + j] = f[j];
-      } else {
-        v[i] = __uint_as_float(u.x), v[i + 1] = __uint_as_float(u.y), v[i + 2] = __uint_as_float(u.z), v[i + 3] = __uint_as_float(u.w);
-      }
+      for (int i = 0; i < 4; ++i) e[i].get(v[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = to.row + 2 * i < N && j < left ? to_f32(from[2 * i * ld + c * TILE_K + j]) : 0.f;
     }
-  } else {
 #pragma unroll
-    for (int i = 0; i < BLOCK; ++i) v[i] = row < N && k0 + i < K ? to_f32(from[i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[i][j]) & 0x7FFFFFFFu);      // (a NaN's bits are above an infinity's)
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = top >> 23;
+      const bool finite = e < 255u;
+      const uint32_t s = finite ? max(e, 2u) - 2u : 255u;
+      const float inverse = __uint_as_float((254u - min(s, 253u)) << 23);                       // 2^(127 - s), a normal number
+      float y[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inverse;
+      const uint32_t word = placed(encode4(y[2], y[0], y[6], y[4], y[3], y[1], y[7], y[5]));   // (of a block without a number: any codes)
+      reinterpret_cast<uint32_t*>(codes + tile * TILE_CODES)[to.at + 8 * i] = word;
+      if ((threadIdx.x & 3) == 0) scales[tile * TILE_SCALES + to.scale_at + 2 * i * (TILE_K / BLOCK)] = (uint8_t)s;
+    }
   }
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < BLOCK; ++i) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);       // (a NaN's bits are above an infinity's)
-  const uint32_t e = top >> 23;
-  const bool finite = e < 255u;
-  const uint32_t s = finite ? max(e, 2u) - 2u : 255u;
-  const float inverse = finite ? __uint_as_float((254u - s) << 23) : 0.f;                     // 2^(127 - s), a normal number: s <= 252
-  uint32_t out[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float y[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) y[j] = finite ? v[8 * i + j] * inverse : 0.f;
-    out[i] = placed(encode4(y[2], y[0], y[6], y[4], y[3], y[1], y[7], y[5]));
-  }
-  reinterpret_cast<uint4*>(codes + tile * TILE_CODES)[t * TILE_ROWS + g] = make_uint4(out[0], out[1], out[2], out[3]);
-  scales[tile * TILE_SCALES + g * (TILE_K / BLOCK) + t] = (uint8_t)s;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256) values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                     int N, int K, int row_tiles, int k_tiles, long long tiles, int whole) {
-  const long long tile = (long long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-  if (tile >= tiles) return;
-  const int lane = threadIdx.x & 31, g = lane & 7, t = lane >> 3;
-  const long long rows_at = tile / k_tiles;
-  const int k0 = (int)(tile - rows_at * k_tiles) * TILE_K + t * BLOCK;
-  const long long group = rows_at / row_tiles;
-  const int row = (int)(rows_at - group * row_tiles) * TILE_ROWS + g;
-  if (row >= N || k0 >= K) return;
-  const uint4 c = reinterpret_cast<const uint4*>(codes + tile * TILE_CODES)[t * TILE_ROWS + g];
-  const uint32_t s = scales[tile * TILE_SCALES + g * (TILE_K / BLOCK) + t];
-  const uint32_t f = factor(s), left = factor_left(s), word[4] = {c.x, c.y, c.z, c.w};
-  T* to = out + (group * N + row) * (long long)K + k0;
+__global__ void __launch_bounds__(CODER_WARPS * 32) values_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales,
+                                                                  T* __restrict__ out, int N, int K, int row_tiles, int k_tiles, int whole) {
+  const Place at(row_tiles);
+  T* to = out + ((long long)at.group * N + at.row) * K + at.k;
+  for (int c = threadIdx.x >> 5; c < k_tiles; c += CODER_WARPS) {
+    const long long tile = (long long)at.row_tile * k_tiles + c;
+    const int left = K - c * TILE_K - at.k;
+    uint32_t word[4], s[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t v[4];
-    values(word[i], f, v);
+    for (int i = 0; i < 4; ++i) {
+      word[i] = reinterpret_cast<const uint32_t*>(codes + tile * TILE_CODES)[at.at + 8 * i];
+      s[i] = scales[tile * TILE_SCALES + at.scale_at + 2 * i * (TILE_K / BLOCK)];
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], left);
-    if (whole && k0 + BLOCK <= K) {
-      if constexpr (sizeof(T) == 2) {
-        reinterpret_cast<uint4*>(to)[i] = make_uint4(v[0], v[1], v[2], v[3]);
+    for (int i = 0; i < 4; ++i) {
+      if (at.row + 2 * i >= N) continue;
+      const uint32_t more = factor_left(s[i]);
+      uint32_t v[4];
+      values(word[i], factor(s[i]), v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = mul2(v[j], more);
+      T* p = to + 2 * i * (long long)K + c * TILE_K;
+      if (whole && left >= 8) {
+        if constexpr (sizeof(T) == 2) {
+          *reinterpret_cast<uint4*>(p) = make_uint4(v[0], v[1], v[2], v[3]);
+        } else {
+          reinterpret_cast<uint4*>(p)[0] = make_uint4(v[0] << 16, v[0] & 0xFFFF0000u, v[1] << 16, v[1] & 0xFFFF0000u);
+          reinterpret_cast<uint4*>(p)[1] = make_uint4(v[2] << 16, v[2] & 0xFFFF0000u, v[3] << 16, v[3] & 0xFFFF0000u);
+        }
       } else {
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-          reinterpret_cast<uint4*>(to)[2 * i + j] =
-              make_uint4(v[2 * j] << 16, v[2 * j] & 0xFFFF0000u, v[2 * j + 1] << 16, v[2 * j + 1] & 0xFFFF0000u);
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const uint32_t bits = j & 1 ? v[j >> 1] & 0xFFFF0000u : v[j >> 1] << 16;
-        if (k0 + 8 * i + j < K) to[8 * i + j] = from_f32<T>(__uint_as_float(bits));
+        for (int j = 0; j < 8; ++j)
+          if (j < left) p[j] = from_f32<T>(__uint_as_float(j & 1 ? v[j >> 1] & 0xFFFF0000u : v[j >> 1] << 16));
       }
     }
   }
@@ -131,13 +154,13 @@ extern "C" int tl_mxfp4_quantize(const void* w, long long ld, long long ld_group
   TL_REQUIRE(groups > 0 && N > 0 && K > 0 && K <= 0x7FFFFF00, "mxfp4: %d matrices of %d x %d", groups, N, K);
   TL_REQUIRE(dtype == TL_FP32 || dtype == TL_BF16, "mxfp4: elements of type %d", dtype);
   const int row_tiles = ceil_div(N, mx::TILE_ROWS), k_tiles = ceil_div(K, mx::TILE_K);
-  const long long tiles = (long long)groups * row_tiles * k_tiles, blocks = ceil_div64(tiles, 8);
-  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4: %lld tiles are too many", tiles);
+  const long long blocks = (long long)groups * row_tiles;
+  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4: %lld tiles of rows are too many", blocks);
   const int size = dtype == TL_FP32 ? 4 : 2;
   const bool whole = ((uintptr_t)w % 16) == 0 && ld * size % 16 == 0 && ld_group * size % 16 == 0;
 #define TL_QUANTIZE(T_, W_)                                                                                                        \
   mx::quantize_kernel<T_, W_><<<(unsigned)blocks, 256, 0, stream>>>((const T_*)w, ld, ld_group, (uint8_t*)codes, (uint8_t*)scales, N, K, \
-                                                                    row_tiles, k_tiles, tiles)
+                                                                    row_tiles, k_tiles)
   if (dtype == TL_FP32) {
     if (whole) TL_QUANTIZE(float, true);
     else TL_QUANTIZE(float, false);
@@ -156,15 +179,15 @@ extern "C" int tl_mxfp4_values(const void* codes, const void* scales, void* out,
   TL_REQUIRE(groups > 0 && N > 0 && K > 0 && K <= 0x7FFFFF00, "mxfp4: %d matrices of %d x %d", groups, N, K);
   TL_REQUIRE(dtype == TL_FP32 || dtype == TL_BF16, "mxfp4: elements of type %d", dtype);
   const int row_tiles = ceil_div(N, mx::TILE_ROWS), k_tiles = ceil_div(K, mx::TILE_K);
-  const long long tiles = (long long)groups * row_tiles * k_tiles, blocks = ceil_div64(tiles, 8);
-  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4: %lld tiles are too many", tiles);
+  const long long blocks = (long long)groups * row_tiles;
+  TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4: %lld tiles of rows are too many", blocks);
   const int whole = ((uintptr_t)out % 16) == 0 && (long long)K * (dtype == TL_FP32 ? 4 : 2) % 16 == 0;
   if (dtype == TL_FP32)
     mx::values_kernel<float><<<(unsigned)blocks, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, (float*)out, N, K,
-                                                                   row_tiles, k_tiles, tiles, whole);
+                                                                   row_tiles, k_tiles, whole);
   else
     mx::values_kernel<bf16><<<(unsigned)blocks, 256, 0, stream>>>((const uint8_t*)codes, (const uint8_t*)scales, (bf16*)out, N, K,
-                                                                  row_tiles, k_tiles, tiles, whole);
+                                                                  row_tiles, k_tiles, whole);
   TL_LAUNCH_CHECK();
   return 0;
 }
