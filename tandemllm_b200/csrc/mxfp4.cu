@@ -53,7 +53,7 @@ struct Place {
     const int lane = threadIdx.x & 31, piece = lane & 15;
     row = (int)(row_tile - group * (unsigned)row_tiles) * TILE_ROWS + (lane >> 4);
     k = piece * 8;
-    at = ((piece >> 2) * TILE_ROWS + (lane >> 4)) * 4 + (piece & 3);
+    at = (lane >> 4) * 16 + (piece & 3) * 4 + (piece >> 2);
     scale_at = (lane >> 4) * (TILE_K / BLOCK) + (piece >> 2);
   }
 };
@@ -61,7 +61,7 @@ struct Place {
 template <typename T, bool WHOLE>
 __global__ void __launch_bounds__(CODER_WARPS * 32, 4) quantize_kernel(const T* __restrict__ w, long long ld, long long ld_group,
                                                                     uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int N, int K,
-                                                                    int row_tiles, int k_tiles) {
+                                                                       int row_tiles, int k_tiles) {
   const Place to(row_tiles);
   const T* from = w + to.group * ld_group + (long long)to.row * ld + to.k;
   for (int c = threadIdx.x >> 5; c < k_tiles; c += CODER_WARPS) {
@@ -94,8 +94,8 @@ __global__ void __launch_bounds__(CODER_WARPS * 32, 4) quantize_kernel(const T* 
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inverse;
-      const uint32_t word = placed(encode4(y[2], y[0], y[6], y[4], y[3], y[1], y[7], y[5]));   // (of a block without a number: any codes)
-      reinterpret_cast<uint32_t*>(codes + tile * TILE_CODES)[to.at + 8 * i] = word;
+      const uint32_t word = finite ? encode4(y[2], y[0], y[6], y[4], y[3], y[1], y[7], y[5]) : 0u;
+      reinterpret_cast<uint32_t*>(codes + tile * TILE_CODES)[to.at + 32 * i] = word;
       if ((threadIdx.x & 3) == 0) scales[tile * TILE_SCALES + to.scale_at + 2 * i * (TILE_K / BLOCK)] = (uint8_t)s;
     }
   }
@@ -112,7 +112,7 @@ __global__ void __launch_bounds__(CODER_WARPS * 32) values_kernel(const uint8_t*
     uint32_t word[4], s[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      word[i] = reinterpret_cast<const uint32_t*>(codes + tile * TILE_CODES)[at.at + 8 * i];
+      word[i] = reinterpret_cast<const uint32_t*>(codes + tile * TILE_CODES)[at.at + 32 * i];
       s[i] = scales[tile * TILE_SCALES + at.scale_at + 2 * i * (TILE_K / BLOCK)];
     }
 #pragma unroll

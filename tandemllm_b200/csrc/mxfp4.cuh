@@ -2,14 +2,10 @@
 // power of two 2^(s - 127), held in a byte s (E8M0, 255: not a number), and each value is a 4-bit number (E2M1: sign, 0 1/2 1 3/2 2 3 4 6).
 //
 // Layout, made for the products: tiles of 8 rows by 128 k, [matrix][N / 8][K / 128], both rounded up (rows and values past the matrix
-// are zeros). A tile's codes are 512 bytes, [k-block of 32][row][16 bytes], so that 32 lanes that take a row's 32 values each read them
-// in one go, whether as 8 rows by 4 blocks (the MMA fragments of a warp) or as 32 rows of one block (the lanes of tensor memory); its
-// scales are 32 bytes, [row][k-block].
-//
-// A 32-bit word holds eight consecutive values; of the pair j (values 2 j and 2 j + 1) the first lies in the lower and the second in the
-// upper half of the word, at the bits where a bfloat16 has its sign, its two lowest exponent bits and its highest mantissa bit, moved
-// down by 3 j (j < 3): a shift and a mask make a pair of bfloat16 numbers that are value * 2^-126 (E2M1's subnormal falls on bfloat16's), and one
-// multiplication by 2^(s - 1) makes them the values, exactly. What is left for pair 3 is bit 14 (sign) and 13, 11, 10.
+// are zeros). A word of codes holds eight consecutive values of a row, those of even places in its lower half, those of odd places in its
+// upper one. A tile's codes are 512 bytes, [row r][quarter t of 4][block b of 4]: the word of row r's values 32 b + 8 t .. + 7. So 16 bytes at (r, t)
+// are what lane (r, t) of a warp multiplies in an MMA of each of the tile's four blocks, and 64 bytes what a lane of tensor memory needs. Behind the
+// codes of all tiles come their scales, 32 bytes a tile, [row][block].
 #pragma once
 #include "common.cuh"
 
@@ -22,33 +18,39 @@ constexpr int TILE_K = 128;
 constexpr int TILE_CODES = TILE_ROWS * TILE_K / 2;             // bytes
 constexpr int TILE_SCALES = TILE_ROWS * TILE_K / BLOCK;
 
-// The factors of a block with scale code s: 2^(min(s, 128) - 1) twice in a word; and what is left where s > 128 (not a number for 255).
-__device__ __forceinline__ uint32_t factor(uint32_t s) { return (min(s, 128u) + 126u) * 0x00800080u; }
-__device__ __forceinline__ uint32_t factor_left(uint32_t s) {
-  return s <= 128u ? 0x3F803F80u : s == 255u ? 0x7FFF7FFFu : (s - 1u) * 0x00800080u;
-}
-
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 
-// The four pairs of a word, times `f`.
+// As bfloat16 numbers, exactly. With a code's lower three bits at the lowest exponent bits and the highest mantissa bit a bfloat16 number is
+// value * 2^-126 (E2M1's subnormal falls on bfloat16's), and one multiplication by 2^(s - 1) makes it the value. `factor` is 2^(min(s, 128) - 1)
+// twice in a word, `factor_left` what is missing where s > 128 (not a number for 255).
+__device__ __forceinline__ uint32_t factor(uint32_t s) { return (min(s, 128u) + 126u) * 0x00800080u; }
+__device__ __forceinline__ uint32_t factor_left(uint32_t s) {
+  return s <= 128u ? 0x3F803F80u : s == 255u ? 0x7FFF7FFFu : (s - 1u) * 0x00800080u;
+}
+// The four pairs of a word, times `f`: pair j is values 2 j (lower half) and 2 j + 1.
 __device__ __forceinline__ void values(uint32_t w, uint32_t f, uint32_t (&v)[4]) {
-  constexpr uint32_t MASK = 0x81C081C0u;
-  v[0] = mul2(w & MASK, f);
-  v[1] = mul2((w << 3) & MASK, f);
-  v[2] = mul2((w << 6) & MASK, f);
-  v[3] = mul2(((w << 1) & 0x80008000u) | ((w >> 4) & 0x00C000C0u) | ((w >> 5) & 0x01000100u), f);
+  constexpr uint32_t SIGN = 0x80008000u, REST = 0x01C001C0u;
+  v[0] = mul2(((w << 12) & SIGN) | ((w << 6) & REST), f);
+  v[1] = mul2(((w << 8) & SIGN) | ((w << 2) & REST), f);
+  v[2] = mul2(((w << 4) & SIGN) | ((w >> 2) & REST), f);
+  v[3] = mul2((w & SIGN) | ((w >> 6) & REST), f);
 }
 
-// The word of eight E2M1 codes that lie as four in each half, pair j at bits 4 j .. 4 j + 3.
-__device__ __forceinline__ uint32_t placed(uint32_t n) {
-  return ((n & 0x00080008u) << 12) | ((n & 0x00070007u) << 6) |            // pair 0
-         ((n & 0x00800080u) << 5) | ((n & 0x00700070u) >> 1) |             // pair 1
-         ((n & 0x08000800u) >> 2) | ((n & 0x07000700u) >> 8) |             // pair 2
-         ((n & 0xC000C000u) >> 1) | ((n & 0x30003000u) >> 2);              // pair 3
+// As float16 numbers without their scale, pairs as the conversion finds them in the word's bytes: values (0, 2), (4, 6), (1, 3), (5, 7).
+__device__ __forceinline__ void values16(uint32_t w, uint32_t (&v)[4]) {
+  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(w));
+}
+// The scale of block b from a row's four in a word, in 32 bits: 2^(s - 127); 0 for s = 0 (2^-127 times a sum of float16 products is below 32-bit's
+// normal numbers), infinite for 255, which the zeros that such a block has for codes make a NaN.
+__device__ __forceinline__ float scale32(uint32_t four, int b) {
+  return __uint_as_float((b < 3 ? four << (23 - 8 * b) : four >> 1) & 0x7F800000u);
 }
 
 }  // namespace mx

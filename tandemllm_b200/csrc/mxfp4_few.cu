@@ -1,182 +1,100 @@
 // Products of a few bfloat16 rows with MXFP4 weights (mxfp4.cuh), for decode steps:
 //
-//   few_kernel      C = X W^T (+ bias), or gated C = act(X G^T + b_g) * (X U^T + b_u)
-//   first_kernel    the experts' first half for up to 8 rows: a[p] = act(G_e x) * (U_e x) of every (row, slot) pair p, times the pair's weight
-//   second_kernel   their second half: out[r] = sum over r's pairs of D_e a[p], all experts in one sum
+//   DENSE   C = X W^T (+ bias), or gated C = act(X G^T + b_g) * (X U^T + b_u)
+//   FIRST   the experts' first half for up to 8 rows: a[p] = act(G_e x) * (U_e x) of every (row, slot) pair p, times the pair's weight
+//   SECOND  their second half: out[r] = sum over r's pairs of D_e a[p], all experts in one sum
 //
-// Such a product reads every weight once and does little with it, so its time is the weights' bytes or, for a few MB, the length of its
-// chain of dependent steps. As in the bfloat16 form (gemm_skinny_mma.cu) there is no staging: a lane loads 32 values of a row and their scale
-// (16 bytes and 1), makes them bfloat16 numbers in its registers (15 instructions for eight) and multiplies them with mma.sync m16n8k16 by the
-// same 32 numbers of a token row, which it loads as they lie; k's order within an MMA is any, as long as both operands have the same.
-// The warps of a CTA split k in tiles of 128, and their 32-bit sums are added in warp order through shared memory, so results do not
-// depend on timing.
+// Such a product reads every weight once and does little with it: its bounds are the weights' stream and their conversion. Codes become float16
+// numbers two at a time by a conversion of the GPU's, and a block's 32 products are two mma.sync m16n8k16 whose sum joins the others times the block's
+// scale, in 32 bits. (As bfloat16 numbers made of bits and times their scale, a word of eight codes takes 32 cycles of a scheduler with its MMA;
+// converted and times a float16 scale 19; so about 12.) The token rows become float16 numbers relative to their largest, which keeps all bits of a bfloat16
+// number down to 2^-31 of it; the power of two comes back with the sum.
+//
+// A persistent CTA an SM has four groups of four warps. A group's producer (one thread of a warp of its own) keeps a ring of stages full
+// with bulk copies, which the layout's tiles make long: a stage is 16 weight rows by up to `slice` tiles of 128 k. The group's four warps take
+// every fourth tile of a stage, and a sixth warp makes results of their sums while they are at the next ones. The token rows lie in shared
+// memory for good.
+//
+// The unit of work is 16 weight rows (gated: 8 gate rows and the 8 up rows of the same outputs) of one matrix. It belongs to a team of one, two or
+// four groups, the larger the fewer units there are. The warps' 32-bit sums are added in the order of the warps, so results do not depend on
+// timing.
+//
+// Every wait on an mbarrier is bounded: when a bound is hit the CTA records status 11, its warps stop, wait (bounded again) for the copies
+// in flight, and return.
+#include <cuda_fp16.h>
+
 #include "mxfp4.cuh"
+#include "tma.cuh"
 
 namespace tl {
 namespace mx {
 
-constexpr int WARPS = 8;
-constexpr int MAX_PAIRS = 256;      // of the experts' form
+constexpr int GROUPS = 4;
+constexpr int GROUP_WARPS = 4;
+constexpr int WARPS = GROUPS * GROUP_WARPS;           // that multiply; a group has one more that copies and one that finishes
+constexpr int THREADS = (WARPS + 2 * GROUPS) * 32;
+constexpr int MAX_TOKENS = 16;
+constexpr int MAX_PAIRS = 256;                        // of the experts' form
 constexpr int MAX_ROWS = 8;
 
+// Token rows in shared memory: a row's length is 64 modulo 128 bytes, so that the 16 bytes of eight lanes (two rows, four quarters of a
+// block) fall on all banks. Eight numbers lie as the codes' conversion leaves theirs: 0 2, 4 6, 1 3, 5 7.
+__host__ __device__ __forceinline__ int row_bytes(int k_tiles) { return k_tiles * TILE_K * 2 + 64; }
+
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// 16 bytes where valid, else zeros. Volatile: a round's loads stay in front of its MMAs, all in flight together.
-__device__ __forceinline__ uint4 load16(const void* p, bool valid) {
-  uint4 v;
-  asm volatile(
-      "{\n\t.reg .pred ok;\n\t"
-      "setp.ne.b32 ok, %5, 0;\n\t"
-      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-      "@ok ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p), "r"((int)valid));
-  return v;
-}
-// Eight numbers of a token row from its element k on, zeros past K and where not valid. WHOLE: rows begin at multiples of 16 bytes and K is a
-// multiple of 8, so the eight are in or out; else they are fetched one by one.
-template <bool WHOLE>
-__device__ __forceinline__ uint4 load_row(const bf16* row, int k, int K, bool valid) {
-  if constexpr (WHOLE) return load16(row + k, valid && k < K);
-  uint32_t v[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool lo = valid && k + 2 * i < K, hi = valid && k + 2 * i + 1 < K;
-    const uint32_t a = lo ? __bfloat16_as_ushort(row[k + 2 * i]) : 0u, b = hi ? __bfloat16_as_ushort(row[k + 2 * i + 1]) : 0u;
-    v[i] = a | b << 16;
-  }
-  return make_uint4(v[0], v[1], v[2], v[3]);
-}
-// 16 bytes of weights, which no kernel writes and no other CTA reads.
-__device__ __forceinline__ uint4 load_codes(const uint8_t* p, bool valid) {
-  uint4 v;
-  asm volatile(
-      "{\n\t.reg .pred ok;\n\t"
-      "setp.ne.b32 ok, %5, 0;\n\t"
-      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-      "@ok ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-      : "l"(p), "r"((int)valid));
-  return v;
-}
-__device__ __forceinline__ uint32_t load_scale(const uint8_t* p, bool valid) {
-  uint32_t v;
-  asm volatile(
-      "{\n\t.reg .pred ok;\n\t"
-      "setp.ne.b32 ok, %2, 0;\n\t"
-      "mov.b32 %0, 0;\n\t"
-      "@ok ld.global.nc.u8 %0, [%1];\n\t}"
-      : "=r"(v) : "l"(p), "r"((int)valid));
-  return v;
+__device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+               ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
 }
 
-// A lane's share of 16 rows by 128 k: 32 values of row g and of row g + 8.
-struct Fragment {
-  uint4 lo, hi;
-  uint32_t s_lo, s_hi;
-};
+// 2^e for e in -126 .. 127
+__device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// The exponent of a row whose largest number has the bits `top` (without the sign): its numbers times 2^(14 - exponent) are float16 numbers.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -112); }
 
-// Lane (g = lane / 4, t = lane % 4) of the tiles at row tile `at` (a tile's place counted in all matrices) and the one below it.
-__device__ __forceinline__ void load_fragment(Fragment& f, const uint8_t* codes, const uint8_t* scales, long long tile_lo, long long tile_hi,
-                                              int g, int t, bool ok_lo, bool ok_hi) {
-  f.lo = load_codes(codes + tile_lo * TILE_CODES + (t * TILE_ROWS + g) * 16, ok_lo);
-  f.hi = load_codes(codes + tile_hi * TILE_CODES + (t * TILE_ROWS + g) * 16, ok_hi);
-  f.s_lo = load_scale(scales + tile_lo * TILE_SCALES + g * 4 + t, ok_lo);
-  f.s_hi = load_scale(scales + tile_hi * TILE_SCALES + g * 4 + t, ok_hi);
-}
-
-// acc[j] += the fragment times the 32 numbers a lane holds of its token row in every tile j of eight rows.
+// acc[j] += 16 weight rows by 128 k times the token rows of every tile j of eight. `lo` and `hi`: a lane's words of the four blocks in row g and
+// in row g + 8; `s_lo` and `s_hi` these rows' scales.
 template <int NT>
-__device__ __forceinline__ void multiply(float (&acc)[NT][4], const Fragment& f, const uint4 (&x)[NT][4]) {
-  const uint32_t f_lo = factor(f.s_lo), f_hi = factor(f.s_hi);
-  const bool far = __any_sync(0xffffffffu, max(f.s_lo, f.s_hi) > 128u);       // blocks of 8 and more: one multiplication more
-  const uint32_t lo[4] = {f.lo.x, f.lo.y, f.lo.z, f.lo.w}, hi[4] = {f.hi.x, f.hi.y, f.hi.z, f.hi.w};
+__device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4& lo4, const uint4& hi4, uint32_t s_lo, uint32_t s_hi,
+                                         const uint8_t* const (&rows)[NT], int at) {
+  const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
+  uint4 x[4][NT];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    uint32_t a[4], b[4];
-    values(lo[i], f_lo, a);
-    values(hi[i], f_hi, b);
-    if (far) {
-      const uint32_t l_lo = factor_left(f.s_lo), l_hi = factor_left(f.s_hi);
+  for (int b = 0; b < 4; ++b)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) a[j] = mul2(a[j], l_lo), b[j] = mul2(b[j], l_hi);
+    for (int j = 0; j < NT; ++j) x[b][j] = *reinterpret_cast<const uint4*>(rows[j] + at + 64 * b);
+  // two blocks side by side: an MMA's sum is there 30 cycles later
+#pragma unroll
+  for (int b0 = 0; b0 < 4; b0 += 2) {
+    uint32_t u[2][4], v[2][4];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      values16(lo[b0 + b], u[b]);
+      values16(hi[b0 + b], v[b]);
     }
+    float c[2][NT][4] = {};
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      mma_16816(acc[j], a[0], b[0], a[1], b[1], x[j][i].x, x[j][i].y);
-      mma_16816(acc[j], a[2], b[2], a[3], b[3], x[j][i].z, x[j][i].w);
-    }
-  }
-}
-
-template <int RT, int NT>
-__device__ __forceinline__ void keep(float (&part)[RT][16][8 * NT + 1], const float (&acc)[RT][NT][4], int g, int t) {
+    for (int h = 0; h < 4; h += 2)
 #pragma unroll
-  for (int r = 0; r < RT; ++r)
+      for (int b = 0; b < 2; ++b)
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      part[r][g][8 * j + 2 * t] = acc[r][j][0];
-      part[r][g][8 * j + 2 * t + 1] = acc[r][j][1];
-      part[r][g + 8][8 * j + 2 * t] = acc[r][j][2];
-      part[r][g + 8][8 * j + 2 * t + 1] = acc[r][j][3];
-    }
-}
-
-// 16 outputs a CTA for up to 8 NT rows. `gate` != 0: the second matrix holds the up rows, and `bias` its numbers behind the gate's.
-template <int NT, bool GATED, bool WHOLE, int UNROLL, typename TOut>
-__global__ void __launch_bounds__(WARPS * 32) few_kernel(const bf16* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
-                                                         const uint8_t* __restrict__ scales, const float* __restrict__ bias, TOut* __restrict__ out,
-                                                         long long ldc, int M, int N, int K, int act, float ga0, float ga1) {
-  constexpr int RT = GATED ? 2 : 1;
-  __shared__ float part[WARPS][RT][16][8 * NT + 1];
-  chain_next();
-  chain_wait();
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int k_tiles = ceil_div(K, TILE_K), row_tiles = ceil_div(N, TILE_ROWS), row_tile = blockIdx.x * 2;
-  const bool ok_hi = row_tile + 1 < row_tiles;
-  float acc[RT][NT][4] = {};
-  for (int c0 = warp; c0 < k_tiles; c0 += WARPS * UNROLL) {
-    Fragment f[UNROLL][RT];
-    uint4 b[UNROLL][NT][4];
+        for (int j = 0; j < NT; ++j)
+          mma_16816(c[b][j], u[b][h], v[b][h], u[b][h + 1], v[b][h + 1], h ? x[b0 + b][j].z : x[b0 + b][j].x, h ? x[b0 + b][j].w : x[b0 + b][j].y);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int c = c0 + u * WARPS;
-      const bool in = c < k_tiles;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const long long at = ((long long)r * row_tiles + row_tile) * k_tiles + (in ? c : 0);
-        load_fragment(f[u][r], codes, scales, at, ok_hi ? at + k_tiles : at, g, t, in, in && ok_hi);
-      }
+    for (int b = 0; b < 2; ++b) {
+      const float f_lo = scale32(s_lo, b0 + b), f_hi = scale32(s_hi, b0 + b);
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int m = j * 8 + g, k = c * TILE_K + t * BLOCK;
-        const bf16* row = x + (long long)(m < M ? m : 0) * ldx;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) b[u][j][i] = load_row<WHOLE>(row, k + 8 * i, K, m < M);
+        acc[j][0] = fmaf(c[b][j][0], f_lo, acc[j][0]);
+        acc[j][1] = fmaf(c[b][j][1], f_lo, acc[j][1]);
+        acc[j][2] = fmaf(c[b][j][2], f_hi, acc[j][2]);
+        acc[j][3] = fmaf(c[b][j][3], f_hi, acc[j][3]);
       }
     }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) multiply<NT>(acc[r], f[u][r], b[u]);
-  }
-  keep<RT, NT>(part[warp], acc, g, t);
-  __syncthreads();
-  for (int i = threadIdx.x; i < 16 * 8 * NT; i += WARPS * 32) {
-    const int row = i & 15, m = i >> 4, n = blockIdx.x * 16 + row;
-    if (m >= M || n >= N) continue;
-    float v[RT];
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      v[r] = 0.f;
-#pragma unroll
-      for (int s = 0; s < WARPS; ++s) v[r] += part[s][r][row][m];
-      if (bias) v[r] += bias[r * N + n];
-    }
-    out[(long long)m * ldc + n] = from_f32<TOut>(GATED ? gated(v[0], v[RT - 1], act, ga0, ga1) : (act < 0 ? gate_activation(v[0], -act) : v[0]));
   }
 }
 
@@ -188,16 +106,17 @@ struct Items {
   short expert[MAX_PAIRS];
   short pair[MAX_PAIRS][MAX_ROWS];        // -1: the row did not choose it
   int key[MAX_PAIRS];
+  short leader[MAX_PAIRS];
   uint32_t firsts[MAX_PAIRS / 32];
+  float weight[MAX_PAIRS];
 };
 
-// All of the CTA's threads (at least MAX_PAIRS where the pairs are more than a warp's); ends with a barrier. An id that names no expert is
-// recorded in `status` and its pair counts for nothing.
-__device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids, int pairs, int top, int experts, int* status) {
-  const int p = threadIdx.x, lane = p & 31, warp = p >> 5;
+// All of the CTA's threads; ends with a barrier. `mine`: with up to 32 pairs, the id of pair `lane` in the first copying warp. An id that names no expert is recorded in `status` and its pair counts for nothing.
+__device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids, int mine, int pairs, int top, int experts, int* status) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (pairs <= 32) {
-    if (warp == 0) {
-      const int id = lane < pairs ? ids[lane] : -1, row = lane / top;
+    if (warp == WARPS) {                    // (the others may be at the token rows meanwhile)
+      const int id = mine, row = lane / top;
       const bool ok = id >= 0 && id < experts;
       if (lane < pairs && !ok) atomicExch(status, 6);
       for (int i = lane; i < pairs * MAX_ROWS; i += 32) (&s.pair[0][0])[i] = -1;
@@ -217,34 +136,42 @@ __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids
     __syncthreads();
     return;
   }
-  int id = -1, key = -1;
-  if (p < pairs) {
-    id = ids[p];
-    if (id >= 0 && id < experts) {
-      int again = 0;
-      for (int q = p - p % top; q < p; ++q) again += ids[q] == id;
-      key = id * 32 + again;
-    } else {
-      atomicExch(status, 6);
+  for (int p = threadIdx.x; p < MAX_PAIRS; p += THREADS) {
+    int key = -1;
+    if (p < pairs) {
+      const int id = ids[p];
+      if (id >= 0 && id < experts) {
+        int again = 0;
+        for (int q = p - p % top; q < p; ++q) again += ids[q] == id;
+        key = id * 32 + again;
+      } else {
+        atomicExch(status, 6);
+      }
+#pragma unroll
+      for (int r = 0; r < MAX_ROWS; ++r) s.pair[p][r] = -1;
     }
     s.key[p] = key;
-#pragma unroll
-    for (int r = 0; r < MAX_ROWS; ++r) s.pair[p][r] = -1;
   }
   __syncthreads();
-  int leader = p;
-  if (key >= 0)
-    for (leader = 0; s.key[leader] != key;) ++leader;
-  const uint32_t firsts = __ballot_sync(0xffffffffu, key >= 0 && leader == p);
-  if (lane == 0 && warp < MAX_PAIRS / 32) s.firsts[warp] = firsts;
+  for (int p = threadIdx.x; p < MAX_PAIRS; p += THREADS) {
+    const int key = s.key[p];
+    int leader = 0;
+    if (key >= 0)
+      while (s.key[leader] != key) ++leader;
+    s.leader[p] = (short)leader;
+    const uint32_t firsts = __ballot_sync(0xffffffffu, key >= 0 && leader == p);
+    if (lane == 0) s.firsts[p >> 5] = firsts;
+  }
   __syncthreads();
-  if (key >= 0) {
+  for (int p = threadIdx.x; p < pairs; p += THREADS) {
+    const int key = s.key[p], leader = s.leader[p];
+    if (key < 0) continue;
     int at = __popc(s.firsts[leader >> 5] & ((1u << (leader & 31)) - 1u));
     for (int i = 0; i < leader >> 5; ++i) at += __popc(s.firsts[i]);
     s.pair[at][p / top] = (short)p;
-    if (leader == p) s.expert[at] = (short)id;
+    if (leader == p) s.expert[at] = (short)(key >> 5);
   }
-  if (p == 0) {
+  if (threadIdx.x == 0) {
     int n = 0;
     for (int i = 0; i < MAX_PAIRS / 32; ++i) n += __popc(s.firsts[i]);
     s.count = n;
@@ -252,113 +179,337 @@ __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids
   __syncthreads();
 }
 
-// grid (16 outputs, items at most): a CTA takes an item's expert and the rows that chose it. `out` [pairs, ldc], outputs up to ldc (those
-// past N come from rows of zeros). `before`: the pair's weight multiplies the sums, in front of the activation, else what comes of them.
-template <bool GATED, bool WHOLE, int UNROLL>
-__global__ void __launch_bounds__(WARPS * 32) first_kernel(const bf16* __restrict__ x, long long ldx, const uint8_t* __restrict__ codes,
-                                                           const uint8_t* __restrict__ scales, bf16* __restrict__ out, int ldc, int N, int K,
-                                                           const int* __restrict__ ids, const float* __restrict__ wts, int before, int pairs,
-                                                           int top, int experts, int act, float ga0, float ga1, int* status) {
-  constexpr int RT = GATED ? 2 : 1;
-  __shared__ float part[WARPS][RT][16][8 + 1];
-  __shared__ Items items;
-  chain_next();
-  chain_wait();
-  find_items(items, ids, pairs, top, experts, status);
-  const int item = blockIdx.y;
-  if (item >= items.count) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int k_tiles = ceil_div(K, TILE_K), row_tiles = ceil_div(N, TILE_ROWS), row_tile = blockIdx.x * 2;
-  const bool ok_hi = row_tile + 1 < row_tiles;
-  const long long matrix = (long long)items.expert[item] * RT;
-  const int pair = items.pair[item][g];
-  const bf16* row = x + (long long)(pair >= 0 ? pair / top : 0) * ldx;
-  float acc[RT][1][4] = {};
-  for (int c0 = warp; c0 < k_tiles; c0 += WARPS * UNROLL) {
-    Fragment f[UNROLL][RT];
-    uint4 b[UNROLL][1][4];
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int c = c0 + u * WARPS, k = c * TILE_K + t * BLOCK;
-      const bool in = c < k_tiles;
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        const long long at = ((matrix + r) * row_tiles + row_tile) * k_tiles + (in ? c : 0);
-        load_fragment(f[u][r], codes, scales, at, ok_hi ? at + k_tiles : at, g, t, in, in && ok_hi);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[u][0][i] = load_row<WHOLE>(row, k + 8 * i, K, pair >= 0);
-    }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u)
-#pragma unroll
-      for (int r = 0; r < RT; ++r) multiply<1>(acc[r], f[u][r], b[u]);
-  }
-  keep<RT, 1>(part[warp], acc, g, t);
-  __syncthreads();
-  if (threadIdx.x < 16 * MAX_ROWS) {
-    const int i = threadIdx.x & 15, m = threadIdx.x >> 4, n = blockIdx.x * 16 + i, p = items.pair[item][m];
-    if (p >= 0 && n < ldc) {
-      const float weight = wts[p];
-      float v[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        v[r] = 0.f;
-#pragma unroll
-        for (int s = 0; s < WARPS; ++s) v[r] += part[s][r][i][m];
-        if (before) v[r] *= weight;
-      }
-      const float a = GATED ? gated(v[0], v[RT - 1], act, ga0, ga1) : gate_activation(v[0], act);
-      out[(long long)p * ldc + n] = __float2bfloat16_rn(before ? a : a * weight);
-    }
-  }
+struct FewParams {
+  const void* x;              // DENSE, FIRST: token rows; SECOND: a row a pair
+  long long ldx;
+  const uint8_t* codes;
+  const uint8_t* scales;
+  const float* bias;          // DENSE (or null)
+  void* out;                  // FIRST: what SECOND reads, K rounded up to 128
+  long long ldc;
+  float* largest;             // FIRST, SECOND: [pairs][parts], the largest numbers of each part of a row between the two
+  int parts;
+  int M, N, K;                // SECOND: M the pairs
+  int act;                    // the gate's activation; a plain product: negated an activation on its results, or 0
+  float ga0, ga1;
+  const int* ids;             // FIRST, SECOND
+  const float* wts;           // FIRST
+  int before;                 // FIRST: the weight multiplies the sums, in front of the activation, else what comes of them
+  int rows, top, experts;     // FIRST, SECOND
+  int team, slice, stages;    // groups a unit, tiles a stage, stages a ring
+  int* status;
+};
+
+enum Kind { DENSE, FIRST, SECOND };
+
+template <Kind KIND> struct Place { typedef Items Type; };
+template <> struct Place<DENSE> { typedef int Type; };              // (never looked into)
+
+__host__ __device__ __forceinline__ int stage_bytes(int slice) { return 2 * slice * (TILE_CODES + TILE_SCALES); }
+// Dynamic shared memory: token rows (SECOND: and one of zeros), rings, two sets of the warps' sums, barriers (full and empty ones of the rings,
+// of the sums two each a group), the rows' largest numbers.
+__host__ __device__ __forceinline__ int rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
+__host__ __device__ __forceinline__ int few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
+  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + GROUPS * (2 * stages + 4) * 8 + m * 4;
 }
 
-// 16 outputs a CTA: all experts' products of all rows are one sum, whose terms are the items' tiles of 128 k one item after the other; a
-// row that did not choose an item's expert has zeros there.
-template <int UNROLL, typename TOut>
-__global__ void __launch_bounds__(WARPS * 32) second_kernel(const bf16* __restrict__ a, int lda, const uint8_t* __restrict__ codes,
-                                                            const uint8_t* __restrict__ scales, TOut* __restrict__ out, long long ldc, int rows,
-                                                            int N, int K, const int* __restrict__ ids, int pairs, int top, int experts,
-                                                            int* status) {
-  __shared__ float part[WARPS][1][16][8 + 1];
-  __shared__ Items items;
-  chain_next();
-  chain_wait();
-  find_items(items, ids, pairs, top, experts, status);
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const int k_tiles = ceil_div(K, TILE_K), row_tiles = ceil_div(N, TILE_ROWS), row_tile = blockIdx.x * 2;
-  const bool ok_hi = row_tile + 1 < row_tiles;
-  const int total = items.count * k_tiles;
-  float acc[1][1][4] = {};
-  for (int u0 = warp; u0 < total; u0 += WARPS * UNROLL) {
-    Fragment f[UNROLL];
-    uint4 b[UNROLL][1][4];
+// Eight numbers of a token row from element k on, zeros past K and where there is no row. ALIGNED: rows begin at multiples of 16 bytes and K is a
+// multiple of 8, so the eight are in or out; the load then stands alone (a branch around it would wait for it), else one by one.
+template <bool ALIGNED>
+__device__ __forceinline__ uint4 load_piece(const bf16* row, int k, int K, bool there) {
+  uint4 v;
+  if constexpr (ALIGNED) {
+    asm volatile(
+        "{\n\t.reg .pred ok;\n\t"
+        "setp.ne.b32 ok, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@ok ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(row + k), "r"((int)(there && k < K)) : "memory");
+  } else {
+    uint32_t u[4];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int unit = u0 + u * WARPS;
-      const bool in = unit < total;
-      const int item = in ? unit / k_tiles : 0, c = in ? unit - item * k_tiles : 0, k = c * TILE_K + t * BLOCK;
-      const long long at = ((long long)(in ? items.expert[item] : 0) * row_tiles + row_tile) * k_tiles + c;
-      load_fragment(f[u], codes, scales, at, ok_hi ? at + k_tiles : at, g, t, in, in && ok_hi);
-      const int pair = in ? items.pair[item][g] : -1;
-      const bf16* row = a + (long long)(pair >= 0 ? pair : 0) * lda + k;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) b[u][0][i] = load16(row + 8 * i, pair >= 0 && k + 8 * i < lda);
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t lo = there && k + 2 * j < K ? __bfloat16_as_ushort(row[k + 2 * j]) : 0u;
+      const uint32_t hi = there && k + 2 * j + 1 < K ? __bfloat16_as_ushort(row[k + 2 * j + 1]) : 0u;
+      u[j] = lo | hi << 16;
     }
-#pragma unroll
-    for (int u = 0; u < UNROLL; ++u) multiply<1>(acc[0], f[u], b[u]);
+    v = make_uint4(u[0], u[1], u[2], u[3]);
   }
-  keep<1, 1>(part[warp], acc, g, t);
-  __syncthreads();
-  if (threadIdx.x < 16 * MAX_ROWS) {
-    const int i = threadIdx.x & 15, m = threadIdx.x >> 4, n = blockIdx.x * 16 + i;
-    if (m < rows && n < N) {
-      float v = 0.f;
+  return v;
+}
+
+template <int NT, bool GATED, Kind KIND, bool ALIGNED, typename TOut>
+__global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
+  constexpr int OUTS = GATED ? 8 : 16, COLS = 8 * NT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ typename Place<KIND>::Type place;
+  __shared__ int aborted_;
+  volatile int* aborted = &aborted_;
+  // SECOND starts behind FIRST's end on its SM, not behind all of it (programmatic dependent launch): it sets itself up, finds its items and has its
+  // first weights on their way before it waits for the rows that FIRST makes.
+  chain_next();
+  if (KIND != SECOND) chain_wait();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = warp < WARPS ? warp / GROUP_WARPS : (warp - WARPS) % GROUPS;
+  int my_id = -1;
+  if (KIND != DENSE && warp == WARPS && lane < p.rows * p.top) my_id = p.ids[lane];
+  const int k_tiles = ceil_div(p.K, TILE_K), row_tiles = ceil_div(p.N, TILE_ROWS);
+  const int x_bytes = row_bytes(k_tiles), one_stage = stage_bytes(p.slice);
+  // The token rows: a warp takes 256 numbers of a row at a time, ROUND such pieces on their way. Their largest numbers come first; what fits one
+  // round stays in registers until these are known, the rest is read again.
+  constexpr int ROUND = 4;
+  const int a_row = ceil_div(k_tiles, 2), all_pieces = p.M * a_row;
+  uint4 raw[ROUND];
+  int m_of[ROUND], k_of[ROUND];
+  int next_m = 0, next_c = warp;
+  auto load_round = [&]() {
 #pragma unroll
-      for (int s = 0; s < WARPS; ++s) v += part[s][0][i][m];
-      out[(long long)m * ldc + n] = from_f32<TOut>(v);
+    for (int j = 0; j < ROUND; ++j) {
+      while (next_c >= a_row) next_c -= a_row, ++next_m;
+      m_of[j] = next_m, k_of[j] = next_c * 256 + lane * 8;
+      raw[j] = load_piece<ALIGNED>(static_cast<const bf16*>(p.x) + next_m * p.ldx, k_of[j], p.K, next_m < p.M);
+      next_c += WARPS;
     }
+  };
+  if (KIND != SECOND && warp < WARPS) load_round();
+  uint8_t* xs = smem;
+  uint8_t* rings = smem + rows_bytes(KIND, p.M, k_tiles);
+  uint8_t* ring = rings + group * p.stages * one_stage;
+  float (*part)[WARPS][16][COLS + 1] = reinterpret_cast<float (*)[WARPS][16][COLS + 1]>(rings + GROUPS * p.stages * one_stage);
+  uint64_t* full = reinterpret_cast<uint64_t*>(part + 2);       // [stages][GROUPS], and so on
+  uint64_t* empty = full + p.stages * GROUPS;
+  uint64_t* summed = empty + p.stages * GROUPS;                 // [2][GROUPS]: a team's sums are there
+  uint64_t* taken = summed + 2 * GROUPS;                        // and read
+  uint32_t* tops = reinterpret_cast<uint32_t*>(taken + 2 * GROUPS);       // the bits of a token row's largest number
+  if (threadIdx.x < (2 * p.stages + 4) * GROUPS) {
+    const int i = threadIdx.x / GROUPS - p.stages;
+    mbar_init(&full[threadIdx.x], i < 0 ? 1 : i < p.stages ? GROUP_WARPS : i < p.stages + 2 ? p.team * GROUP_WARPS : p.team);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x == 0) aborted_ = 0;
+  for (int m = threadIdx.x; m < p.M; m += THREADS) tops[m] = 0u;
+  __syncthreads();
+  if constexpr (KIND == FIRST)
+    for (int i = threadIdx.x - (WARPS + GROUPS) * 32; i >= 0 && i < p.rows * p.top; i += GROUPS * 32) reinterpret_cast<Items*>(&place)->weight[i] = p.wts[i];
+  if (KIND != SECOND && warp < WARPS) {
+    for (int done = 0; done < all_pieces; done += ROUND * WARPS) {
+      if (done) load_round();
+#pragma unroll
+      for (int j = 0; j < ROUND; ++j) {
+        if (m_of[j] >= p.M) break;
+        const uint32_t a = __vmaxu2(raw[j].x & 0x7FFF7FFFu, raw[j].y & 0x7FFF7FFFu), b = __vmaxu2(raw[j].z & 0x7FFF7FFFu, raw[j].w & 0x7FFF7FFFu);
+        const uint32_t c = __vmaxu2(a, b), top = __reduce_max_sync(0xffffffffu, max(c << 16, c & 0xFFFF0000u));
+        if (lane == 0) atomicMax(&tops[m_of[j]], top);
+      }
+    }
+  }
+  Items* items = reinterpret_cast<Items*>(&place);
+  int count = 1;
+  if constexpr (KIND != DENSE) {
+    find_items(*items, p.ids, my_id, p.rows * p.top, p.top, p.experts, p.status);
+    count = items->count;
+  }
+  // What all roles go through, in the same order: this team's units, and of a unit the slices that are this group's.
+  const int blocks = ceil_div(p.N, OUTS), units = KIND == FIRST ? blocks * count : blocks;
+  const int teams = gridDim.x * (GROUPS / p.team), member = group % p.team, team0 = group - member;
+  const int parts = ceil_div(k_tiles, p.slice), slices = KIND == SECOND ? parts * count : parts;
+  const int first_unit = blockIdx.x * (GROUPS / p.team) + group / p.team;
+  auto give_up = [&]() {
+    *aborted = 1;
+    atomicExch(p.status, 11);
+  };
+
+  if (warp >= WARPS && warp < WARPS + GROUPS) {
+    // ---- copies ----
+    if (lane == 0) {
+      int it = 0;
+      for (int unit = first_unit; unit < units && !*aborted; unit += teams) {
+        const int item0 = KIND == FIRST ? unit / blocks : 0, block = unit - item0 * blocks;
+        const int row_lo = GATED ? block : 2 * block, row_hi = GATED ? block : min(row_lo + 1, row_tiles - 1);
+        for (int sl = member; sl < slices; sl += p.team, ++it) {
+          const int item = KIND == SECOND ? sl / parts : item0, tile0 = (sl - (KIND == SECOND ? item * parts : 0)) * p.slice;
+          const int n = min(p.slice, k_tiles - tile0), s = it % p.stages;
+          uint64_t* bar = &full[s * GROUPS + group];
+          if (it >= p.stages && !mbar_wait(&empty[s * GROUPS + group], ((it / p.stages) - 1) & 1)) give_up();
+          if (*aborted) break;
+          uint8_t* to = ring + s * one_stage;
+          uint8_t* to_scales = to + p.slice * 2 * TILE_CODES;
+          const long long matrix = KIND == DENSE ? 0 : (long long)items->expert[item] * (GATED ? 2 : 1);
+          const long long lo = (matrix * row_tiles + row_lo) * k_tiles + tile0;
+          const long long hi = ((matrix + (GATED ? 1 : 0)) * row_tiles + row_hi) * k_tiles + tile0;
+          mbar_expect_tx(bar, 2 * n * (TILE_CODES + TILE_SCALES));
+          copy_bulk(to, p.codes + lo * TILE_CODES, n * TILE_CODES, bar);
+          copy_bulk(to + p.slice * TILE_CODES, p.codes + hi * TILE_CODES, n * TILE_CODES, bar);
+          copy_bulk(to_scales, p.scales + lo * TILE_SCALES, n * TILE_SCALES, bar);
+          copy_bulk(to_scales + p.slice * TILE_SCALES, p.scales + hi * TILE_SCALES, n * TILE_SCALES, bar);
+        }
+      }
+      // no CTA leaves with copies under way, whether it gave up or not
+      for (int i = max(0, it - p.stages); i < it; ++i) mbar_wait(&full[(i % p.stages) * GROUPS + group], (i / p.stages) & 1);
+    }
+    return;
+  }
+
+  if (warp >= WARPS + GROUPS) {
+    // ---- results ----
+    if (KIND == SECOND) chain_wait();
+    int nth = 0;
+    for (int unit = first_unit; unit < units; unit += teams, ++nth) {
+      const int item = KIND == FIRST ? unit / blocks : 0, block = unit - item * blocks, buffer = nth & 1;
+      const bool ok = __all_sync(0xffffffffu, !*aborted && mbar_wait(&summed[buffer * GROUPS + team0], (nth >> 1) & 1));
+      if (!ok) {
+        if (lane == 0) give_up();
+        break;
+      }
+#pragma unroll 2
+      for (int i = member * 32 + lane; i < OUTS * COLS; i += p.team * 32) {
+        const int o = i & (OUTS - 1), m = i / OUTS, n = block * OUTS + o;
+        int row = m;
+        bool mine = m < (KIND == SECOND ? p.rows : p.M) && n < p.N;
+        float weight = 1.f;
+        if (KIND == FIRST) {
+          row = items->pair[item][m];
+          mine = row >= 0;
+          if (mine) weight = items->weight[row];
+        }
+        float v = 0.f, u = 0.f;
+        for (int s = team0 * GROUP_WARPS; s < (team0 + p.team) * GROUP_WARPS; ++s) {
+          v += part[buffer][s][o][m];
+          if (GATED) u += part[buffer][s][o + 8][m];
+        }
+        if (KIND != SECOND && mine) {
+          const float f = power(row_exponent(tops[m]) - 14);
+          v *= f;
+          if (GATED) u *= f;
+        }
+        if (KIND == FIRST && n >= p.N) v = u = 0.f;             // (what lies behind the last output meets codes of zeros)
+        if (KIND == FIRST && p.before) v *= weight, u *= weight;
+        if (KIND == DENSE && p.bias && mine) {
+          v += p.bias[n];
+          if (GATED) u += p.bias[p.N + n];
+        }
+        float out = GATED ? gated(v, u, p.act, p.ga0, p.ga1) : p.act < 0 ? gate_activation(v, -p.act) : v;
+        if (KIND == FIRST && !p.before) out *= weight;
+        const TOut rounded = from_f32<TOut>(out);
+        if (mine) static_cast<TOut*>(p.out)[row * p.ldc + n] = rounded;
+        if (KIND == FIRST) {                                      // (bits: a NaN's are above all others)
+          uint32_t top = mine ? __float_as_uint(to_f32(rounded)) & 0x7FFFFFFFu : 0u;
+#pragma unroll
+          for (int d = 1; d < OUTS; d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+          if (mine && o == 0) p.largest[(long long)row * p.parts + block] = __uint_as_float(top);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&taken[buffer * GROUPS + team0]);
+    }
+    return;
+  }
+
+  // ---- token rows into shared memory ----
+  if (KIND == SECOND) {
+    chain_wait();
+    load_round();
+    for (int m = warp; m < p.M; m += WARPS) {
+      uint32_t top = 0u;
+#pragma unroll 4
+      for (int i = lane; i < p.parts; i += 32) top = max(top, __float_as_uint(p.largest[(long long)m * p.parts + i]));
+      top = __reduce_max_sync(0xffffffffu, top);
+      if (lane == 0) tops[m] = top;
+    }
+  }
+  asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+  if (KIND != SECOND && all_pieces > ROUND * WARPS) {
+    next_m = 0, next_c = warp;
+    load_round();
+  }
+  for (int done = 0; done < all_pieces; done += ROUND * WARPS) {
+    if (done) load_round();
+#pragma unroll
+    for (int j = 0; j < ROUND; ++j) {
+      if (m_of[j] >= p.M || k_of[j] >= k_tiles * TILE_K) continue;
+      const float f = power(14 - row_exponent(tops[m_of[j]]));
+      float v[8];
+      unpack8(raw[j], v);
+      __half2 h[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = (e & 1) * 4 + (e >> 1);
+        h[e] = __floats2half2_rn(v[at] * f, v[at + 2] * f);
+      }
+      *reinterpret_cast<uint4*>(xs + m_of[j] * x_bytes + k_of[j] * 2) = *reinterpret_cast<const uint4*>(h);
+    }
+  }
+  if (KIND == SECOND)
+    for (int i = threadIdx.x; i < x_bytes / 16; i += WARPS * 32) reinterpret_cast<uint4*>(xs + p.M * x_bytes)[i] = make_uint4(0u, 0u, 0u, 0u);
+  asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+
+  // ---- products ----
+  const int g = lane >> 2, t = lane & 3, w = warp % GROUP_WARPS;
+  const unsigned lane_codes = lane * 16;
+  int it = 0, nth = 0;
+  for (int unit = first_unit; unit < units; unit += teams, ++nth) {
+    float acc[NT][4] = {};
+    bool ok = true;
+    for (int sl = member; sl < slices; sl += p.team, ++it) {
+      const int item = KIND == SECOND ? sl / parts : 0, tile0 = (sl - (KIND == SECOND ? item * parts : 0)) * p.slice;
+      const int n = min(p.slice, k_tiles - tile0), s = it % p.stages;
+      const uint8_t* from = ring + s * one_stage;
+      const uint8_t* rows[NT];
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        int m = min(j * 8 + g, p.M - 1);
+        if (KIND == SECOND) {
+          const int pair = items->pair[item][g];
+          m = pair >= 0 ? pair : p.M;
+        }
+        rows[j] = xs + m * x_bytes + tile0 * (TILE_K * 2) + t * 16;
+      }
+      ok = __all_sync(0xffffffffu, !*aborted && mbar_wait(&full[s * GROUPS + group], (it / p.stages) & 1));
+      if (!ok) break;
+      float sum[NT][4] = {};
+      for (int c = (w + it) & (GROUP_WARPS - 1); c < n; c += GROUP_WARPS) {
+        const uint8_t* codes = from + c * TILE_CODES + lane_codes;
+        const uint8_t* scales = from + p.slice * 2 * TILE_CODES + c * TILE_SCALES + g * 4;
+        multiply<NT>(KIND == SECOND ? sum : acc, *reinterpret_cast<const uint4*>(codes), *reinterpret_cast<const uint4*>(codes + p.slice * TILE_CODES),
+                     *reinterpret_cast<const uint32_t*>(scales), *reinterpret_cast<const uint32_t*>(scales + p.slice * TILE_SCALES), rows,
+                     c * (TILE_K * 2));
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[s * GROUPS + group]);
+      if (KIND == SECOND) {       // every pair has an exponent of its own; the rows that did not choose the expert have nothing to add
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int pair = items->pair[item][2 * t + c];
+          if (pair >= 0) {
+            const float f = power(row_exponent(tops[pair]) - 14);
+            acc[0][c] = fmaf(sum[0][c], f, acc[0][c]);
+            acc[0][c + 2] = fmaf(sum[0][c + 2], f, acc[0][c + 2]);
+          }
+        }
+      }
+    }
+    // ---- the unit's end ----
+    const int buffer = nth & 1;
+    if (ok && nth >= 2) ok = __all_sync(0xffffffffu, !*aborted && mbar_wait(&taken[buffer * GROUPS + team0], ((nth >> 1) - 1) & 1));
+    if (!ok) {
+      if (lane == 0) give_up();
+      break;
+    }
+    float (&mine)[16][COLS + 1] = part[buffer][warp];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      mine[g][8 * j + 2 * t] = acc[j][0];
+      mine[g][8 * j + 2 * t + 1] = acc[j][1];
+      mine[g + 8][8 * j + 2 * t] = acc[j][2];
+      mine[g + 8][8 * j + 2 * t + 1] = acc[j][3];
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&summed[buffer * GROUPS + team0]);
+  }
+  if (KIND == FIRST) {        // and the rest of the last tile of 128, in every pair's row
+    const int from = blocks * OUTS, rest = (int)p.ldc - from;
+    for (int i = blockIdx.x * WARPS * 32 + threadIdx.x; i < p.rows * p.top * rest; i += gridDim.x * WARPS * 32)
+      static_cast<TOut*>(p.out)[(i / rest) * p.ldc + from + i % rest] = from_f32<TOut>(0.f);
   }
 }
 
@@ -367,74 +518,160 @@ __global__ void __launch_bounds__(WARPS * 32) second_kernel(const bf16* __restri
 
 using namespace tl;
 
-// x [M, K] bfloat16 (row stride ldx), M <= 32; the matrix N x K (gated: two, gate and up); bias [N] (gated: [2 N]) 32-bit or null; out [M, N]
+namespace {
+
+constexpr int FEW_SMEM = 226 * 1024;
+constexpr int few_dynamic(mx::Kind kind) { return FEW_SMEM - (kind == mx::DENSE ? 0 : (int)sizeof(mx::Items)) - 64; }
+
+// Tiles a stage and stages a ring that fit beside the token rows, or false. Stages of 16 tiles where a slice is as long, so that a wait and an
+// arrival serve four tiles a warp, else of 8 or 4.
+bool few_fits(mx::Kind kind, int nt, int m, int k_tiles, mx::FewParams& p) {
+  const int share = kind == mx::SECOND ? k_tiles : ceil_div(k_tiles, p.team);
+  for (int slice = 16; slice >= 4; slice /= 2) {
+    if (slice > 4 && slice / 2 >= share) continue;
+    for (int stages = 6; stages >= 2; --stages)
+      if (mx::few_bytes(kind, nt, m, k_tiles, slice, stages) <= few_dynamic(kind) && (stages <= 3 || stages * slice <= 32)) {
+        p.slice = slice, p.stages = stages;
+        return true;
+      }
+  }
+  return false;
+}
+
+template <auto kernel>
+int launch_few(const mx::FewParams& p, mx::Kind kind, int nt, long long units, cudaStream_t stream) {
+  static thread_local int set_on = -1;              // the device whose function has its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (set_on != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, few_dynamic(kind));
+    if (e != cudaSuccess) return (int)e;
+    set_on = dev;
+  }
+  const long long ctas = ceil_div64(units, mx::GROUPS / p.team);
+  const int bytes = mx::few_bytes(kind, nt, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)(ctas < sm_count() ? ctas : sm_count()));
+  cfg.blockDim = dim3(mx::THREADS);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = kind == mx::SECOND || chained_launches() ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// Groups a unit: one where the groups of the GPU have units enough each, else two or four.
+int team_of(long long units) {
+  const long long groups = (long long)mx::GROUPS * sm_count();
+  return units >= groups ? 1 : 2 * units >= groups ? 2 : 4;
+}
+
+bool a_few(int rows, int top, int experts) {
+  return rows >= 1 && rows <= mx::MAX_ROWS && top >= 1 && rows * top <= mx::MAX_PAIRS && top <= 32 && experts >= 1 && experts <= 1024;
+}
+
+}  // namespace
+
+// Whether `M` rows of K elements go through the form below.
+extern "C" int tl_mxfp4_few_fits(int M, int N, int K, int act) {
+  if (M < 1 || M > mx::MAX_TOKENS || N < 1 || K < 1) return 0;
+  mx::FewParams p = {};
+  p.team = team_of(ceil_div(N, act > 0 ? 8 : 16));
+  return few_fits(mx::DENSE, M <= 8 ? 1 : 2, M, ceil_div(K, mx::TILE_K), p);
+}
+
+// x [M, K] bfloat16 (row stride ldx), M <= 16; the matrix N x K (gated: two, gate and up); bias [N] (gated: [2 N]) 32-bit or null; out [M, N]
 // (row stride ldc) bfloat16 or 32-bit. `act`: the gate's activation TL_ACT_*, 0 for a plain product, negated an activation on its results.
 extern "C" int tl_mxfp4_few(const void* x, long long ldx, const void* codes, const void* scales, const float* bias, void* out, long long ldc,
-                            int M, int N, int K, int act, float a0, float a1, int out_dtype, cudaStream_t stream) {
+                            int M, int N, int K, int act, float a0, float a1, int out_dtype, int* status, cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
-  TL_REQUIRE(M >= 1 && M <= 32 && N >= 1 && K >= 1, "mxfp4 product of few rows: %d rows x (%d x %d)", M, N, K);
+  TL_REQUIRE(M >= 1 && M <= mx::MAX_TOKENS && N >= 1 && K >= 1, "mxfp4 product of few rows: %d rows x (%d x %d)", M, N, K);
   TL_REQUIRE(act <= 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 product: gate activation %d is none (nor an ungated one, negated)", act);
   TL_REQUIRE(act <= 0 || out_dtype == TL_BF16, "mxfp4 product: gated outputs of type %d", out_dtype);
-  const dim3 grid(ceil_div(N, 16)), block(mx::WARPS * 32);
-  const int nt = ceil_div(M, 8);
-  const bool whole = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
-#define TL_FEW(NT_, G_, W_, U_, T_)                                                                                               \
-  return (int)launch_chained(mx::few_kernel<NT_, G_, W_, U_, T_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes, \
-                             (const uint8_t*)scales, bias, (T_*)out, ldc, M, N, K, act, a0, a1)
-#define TL_FEW_(NT_, W_, U_)                                     \
-  do {                                                           \
-    if (act > 0) TL_FEW(NT_, true, W_, U_, bf16);                \
-    if (out_dtype == TL_FP32) TL_FEW(NT_, false, W_, U_, float); \
-    TL_FEW(NT_, false, W_, U_, bf16);                            \
+  mx::FewParams p = {};
+  p.x = x, p.ldx = ldx, p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.bias = bias, p.out = out, p.ldc = ldc;
+  p.M = M, p.N = N, p.K = K, p.act = act, p.ga0 = a0, p.ga1 = a1, p.status = status;
+  const bool aligned = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
+  const int nt = M <= 8 ? 1 : 2, units = ceil_div(N, act > 0 ? 8 : 16);
+  p.team = team_of(units);
+  TL_REQUIRE(few_fits(mx::DENSE, nt, M, ceil_div(K, mx::TILE_K), p), "mxfp4 product of few rows: %d rows of %d elements are too many", M, K);
+#define TL_FEW(NT_, G_, T_)                                                                                            \
+  do {                                                                                                                 \
+    if (aligned) return launch_few<mx::few_kernel<NT_, G_, mx::DENSE, true, T_>>(p, mx::DENSE, NT_, units, stream);    \
+    return launch_few<mx::few_kernel<NT_, G_, mx::DENSE, false, T_>>(p, mx::DENSE, NT_, units, stream);                \
   } while (0)
-  if (whole) {
-    if (nt == 1) TL_FEW_(1, true, 2);
-    if (nt == 2) TL_FEW_(2, true, 1);
-    TL_FEW_(4, true, 1);
-  }
-  if (nt == 1) TL_FEW_(1, false, 1);
-  if (nt == 2) TL_FEW_(2, false, 1);
-  TL_FEW_(4, false, 1);
+#define TL_FEW_(NT_)                                     \
+  do {                                                   \
+    if (act > 0) TL_FEW(NT_, true, bf16);                \
+    if (out_dtype == TL_FP32) TL_FEW(NT_, false, float); \
+    TL_FEW(NT_, false, bf16);                            \
+  } while (0)
+  if (nt == 1) TL_FEW_(1);
+  TL_FEW_(2);
 #undef TL_FEW_
 #undef TL_FEW
 }
 
+// Whether `rows` rows of K elements and what top experts of `inter` outputs each make of them go through the two kernels below; and the bytes
+// of what lies between the two.
+extern "C" int tl_mxfp4_experts_fit(int rows, int top, int K, int inter) {
+  if (!a_few(rows, top, 1) || K < 1 || inter < 1) return 0;
+  mx::FewParams p = {};
+  p.team = 4;
+  return few_fits(mx::FIRST, 1, rows, ceil_div(K, mx::TILE_K), p) && few_fits(mx::SECOND, 1, rows * top, ceil_div(inter, mx::TILE_K), p);
+}
+static int between_row(int inter) { return ceil_div(inter, mx::TILE_K) * mx::TILE_K; }
+extern "C" long long tl_mxfp4_experts_between(int pairs, int inter) {
+  return (long long)pairs * (between_row(inter) * 2 + ceil_div(inter, 8) * 4);
+}
+
 // Routed experts of up to 8 rows and 256 pairs, first half: x [rows, K]; matrices [experts] (or gated [2 experts], gate and up in turn) of N x K;
-// out [rows * top, ldc] bfloat16 with ldc = N rounded up to 8.
-extern "C" int tl_mxfp4_experts_first(const void* x, long long ldx, const void* codes, const void* scales, void* out, int ldc, int rows, int N,
-                                      int K, const int* ids, const float* wts, int before, int top, int experts, int act, float a0, float a1,
-                                      int* status, cudaStream_t stream) {
+// `between` (16-byte aligned) receives a bfloat16 row of N numbers, rounded up to 128, for every pair, and behind them the rows' largest numbers.
+extern "C" int tl_mxfp4_experts_first(const void* x, long long ldx, const void* codes, const void* scales, void* between, int rows, int N, int K,
+                                      const int* ids, const float* wts, int before, int top, int experts, int act, float a0, float a1, int* status,
+                                      cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
-  TL_REQUIRE(rows >= 1 && rows <= mx::MAX_ROWS && top >= 1 && rows * top <= mx::MAX_PAIRS && top <= 32 && experts >= 1 && experts <= 1024,
-             "mxfp4 experts: %d rows, top-%d of %d", rows, top, experts);
-  TL_REQUIRE(N >= 1 && K >= 1 && ldc == ceil_div(N, 8) * 8, "mxfp4 experts: %d x %d, row stride %d", N, K, ldc);
+  TL_REQUIRE(a_few(rows, top, experts), "mxfp4 experts: %d rows, top-%d of %d", rows, top, experts);
+  TL_REQUIRE(N >= 1 && K >= 1 && ((uintptr_t)between % 16) == 0, "mxfp4 experts: %d x %d", N, K);
   TL_REQUIRE(act < 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 experts: gate activation %d is none (nor an ungated one, negated)", act);
-  const dim3 grid(ceil_div(N, 16), rows * top), block(mx::WARPS * 32);
-#define TL_FIRST(G_, W_, U_)                                                                                                                      \
-  return (int)launch_chained(mx::first_kernel<G_, W_, U_>, grid, block, 0, stream, (const bf16*)x, ldx, (const uint8_t*)codes,                    \
-                             (const uint8_t*)scales, (bf16*)out, ldc, N, K, ids, wts, before, rows * top, top, experts, act < 0 ? -act : act, \
-                             a0, a1, status)
-  if (K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0) {
-    if (act > 0) TL_FIRST(true, true, 2);
-    TL_FIRST(false, true, 2);
-  }
-  if (act > 0) TL_FIRST(true, false, 1);
-  TL_FIRST(false, false, 1);
+  mx::FewParams p = {};
+  p.x = x, p.ldx = ldx, p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.out = between;
+  p.ldc = between_row(N), p.M = rows, p.N = N, p.K = K, p.act = act, p.ga0 = a0, p.ga1 = a1;
+  p.parts = ceil_div(N, act > 0 ? 8 : 16), p.largest = (float*)((uint8_t*)between + rows * top * p.ldc * 2);
+  p.ids = ids, p.wts = wts, p.before = before, p.rows = rows, p.top = top, p.experts = experts, p.status = status;
+  const bool aligned = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
+  const long long units = (long long)p.parts * (top < experts ? top : experts);       // (at least so many)
+  p.team = team_of(units);
+  TL_REQUIRE(few_fits(mx::FIRST, 1, rows, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d rows of %d elements are too many", rows, K);
+#define TL_FIRST(G_)                                                                                                     \
+  do {                                                                                                                   \
+    if (aligned) return launch_few<mx::few_kernel<1, G_, mx::FIRST, true, bf16>>(p, mx::FIRST, 1, units * rows, stream); \
+    return launch_few<mx::few_kernel<1, G_, mx::FIRST, false, bf16>>(p, mx::FIRST, 1, units * rows, stream);             \
+  } while (0)
+  if (act > 0) TL_FIRST(true);
+  TL_FIRST(false);
 #undef TL_FIRST
 }
 
-// Second half: a [rows * top, lda] (what the first half left, K rounded up to 8); matrices [experts] of N x K; out [rows, N] (row stride ldc).
-extern "C" int tl_mxfp4_experts_second(const void* a, int lda, const void* codes, const void* scales, void* out, long long ldc, int rows, int N,
-                                       int K, const int* ids, int top, int experts, int out_dtype, int* status, cudaStream_t stream) {
+// Second half: `between` as the first half (of the same `act`) left it for pairs of K numbers; matrices [experts] of N x K; out [rows, N] (row
+// stride ldc).
+extern "C" int tl_mxfp4_experts_second(void* between, const void* codes, const void* scales, void* out, long long ldc, int rows, int N, int K,
+                                       const int* ids, int top, int experts, int act, int out_dtype, int* status, cudaStream_t stream) {
   if (rows == 0 || N == 0) return 0;
-  TL_REQUIRE(rows >= 1 && rows <= mx::MAX_ROWS && top >= 1 && rows * top <= mx::MAX_PAIRS && top <= 32 && experts >= 1 && experts <= 1024,
-             "mxfp4 experts: %d rows, top-%d of %d", rows, top, experts);
-  TL_REQUIRE(N >= 1 && K >= 1 && lda == ceil_div(K, 8) * 8 && ((uintptr_t)a % 16) == 0, "mxfp4 experts: %d x %d, row stride %d", N, K, lda);
-  const dim3 grid(ceil_div(N, 16)), block(mx::WARPS * 32);
-#define TL_SECOND(T_)                                                                                                        \
-  return (int)launch_chained(mx::second_kernel<4, T_>, grid, block, 0, stream, (const bf16*)a, lda, (const uint8_t*)codes,   \
-                             (const uint8_t*)scales, (T_*)out, ldc, rows, N, K, ids, rows * top, top, experts, status)
-  if (out_dtype == TL_FP32) TL_SECOND(float);
-  TL_SECOND(bf16);
-#undef TL_SECOND
+  TL_REQUIRE(a_few(rows, top, experts), "mxfp4 experts: %d rows, top-%d of %d", rows, top, experts);
+  TL_REQUIRE(N >= 1 && K >= 1 && ((uintptr_t)between % 16) == 0, "mxfp4 experts: %d x %d", N, K);
+  mx::FewParams p = {};
+  p.x = between, p.ldx = between_row(K), p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.out = out, p.ldc = ldc;
+  p.M = rows * top, p.N = N, p.K = (int)p.ldx;
+  p.parts = ceil_div(K, act > 0 ? 8 : 16), p.largest = (float*)((uint8_t*)between + rows * top * p.ldx * 2);
+  p.ids = ids, p.rows = rows, p.top = top, p.experts = experts, p.status = status;
+  const int units = ceil_div(N, 16);
+  p.team = team_of(units);
+  TL_REQUIRE(few_fits(mx::SECOND, 1, p.M, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d pairs of %d elements are too many", p.M, K);
+  if (out_dtype == TL_FP32) return launch_few<mx::few_kernel<1, false, mx::SECOND, true, float>>(p, mx::SECOND, 1, units, stream);
+  return launch_few<mx::few_kernel<1, false, mx::SECOND, true, bf16>>(p, mx::SECOND, 1, units, stream);
 }

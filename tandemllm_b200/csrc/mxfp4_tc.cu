@@ -10,7 +10,7 @@
 //
 //   warp 0       one thread keeps the ring of token boxes full
 //   warp 1       one thread issues the MMAs (kind::f16, A in tensor memory, B in shared memory) and releases both operands' stages
-//   warps 2..9   two groups of four that take every other k-block of weights; then the epilogue, each group every other 16 columns
+//   warps 2..9   two groups of four that take every other tile of 128 k of the weights; then the epilogue, each group every other 16 columns
 //
 // An MMA of 128 x 128 x 64 takes 256 cycles of the tensor pipe and its weights 134 issue cycles of each scheduler, so with tiles of 128
 // token rows the conversion runs under the products; two CTAs an SM run under each other's ends.
@@ -59,7 +59,7 @@ struct Tc {
   static constexpr int A_COLS = KB / 2;                         // columns of tensor memory a k-block of weights takes
   static constexpr int A_STAGES = BN >= 128 ? 4 : 6;
   static constexpr int TMEM_COLS = 256;
-  static constexpr int AHEAD = BN >= 128 ? 2 : 4;               // k-blocks of codes a thread has on their way
+  static constexpr int AHEAD = 2;                               // tiles of codes a thread has at hand or on their way
   static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
   // What a launch with clusters asks for at least. A CTA of a cluster that waits for tensor memory keeps the others waiting, who keep
   // theirs; beside another kernel of clusters that could close a circle. With this much shared memory no SM has room for more CTAs of such kernels
@@ -132,41 +132,47 @@ __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-// The codes and scales of a thread's row in one k-block.
-struct RowBlock {
-  uint4 c[2];
-  uint32_t s;                 // the two blocks' scales, the first in the low byte
+// The codes and scales of a thread's row in one tile of 128 k: the words of its four blocks in each of the tile's quarters.
+struct RowTile {
+  uint4 c[4];
+  uint32_t s;
 };
-__device__ __forceinline__ void load_row_block(RowBlock& q, const uint8_t* codes, const uint8_t* scales, int tile, bool valid) {
-  asm volatile(
-      "{\n\t.reg .pred ok;\n\t"
-      "setp.ne.b32 ok, %11, 0;\n\t"
-      "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
-      "mov.b32 %4, 0;\n\tmov.b32 %5, 0;\n\tmov.b32 %6, 0;\n\tmov.b32 %7, 0;\n\tmov.b32 %8, 0;\n\t"
-      "@ok ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%9];\n\t"
-      "@ok ld.global.nc.v4.u32 {%4, %5, %6, %7}, [%9 + 128];\n\t"
-      "@ok ld.global.nc.u16 %8, [%10];\n\t}"
-      : "=r"(q.c[0].x), "=r"(q.c[0].y), "=r"(q.c[0].z), "=r"(q.c[0].w), "=r"(q.c[1].x), "=r"(q.c[1].y), "=r"(q.c[1].z), "=r"(q.c[1].w), "=r"(q.s)
-      : "l"(codes + (long long)tile * TILE_CODES), "l"(scales + (long long)tile * TILE_SCALES), "r"((int)valid));
+__device__ __forceinline__ void load_row_tile(RowTile& q, const uint8_t* codes, const uint8_t* scales, int tile, bool valid) {
+  const uint8_t* from = codes + (long long)tile * TILE_CODES;
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+    asm volatile(
+        "{\n\t.reg .pred ok;\n\t"
+        "setp.ne.b32 ok, %5, 0;\n\t"
+        "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
+        "@ok ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
+        : "=r"(q.c[t].x), "=r"(q.c[t].y), "=r"(q.c[t].z), "=r"(q.c[t].w) : "l"(from + t * 16), "r"((int)valid));
+  asm volatile("{\n\t.reg .pred ok;\n\tsetp.ne.b32 ok, %2, 0;\n\tmov.b32 %0, 0;\n\t@ok ld.global.nc.u32 %0, [%1];\n\t}"
+               : "=r"(q.s) : "l"(scales + (long long)tile * TILE_SCALES), "r"((int)valid));
 }
 
-__device__ __forceinline__ void convert(const RowBlock& q, uint32_t (&v)[32]) {
-  const uint32_t s[2] = {q.s & 255u, q.s >> 8};
+// The values of the tile's first or second 64 k, two a register.
+template <int HALF>
+__device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
+  const uint32_t s[2] = {(q.s >> (16 * HALF)) & 255u, (q.s >> (16 * HALF + 8)) & 255u};
   const bool far = __any_sync(0xffffffffu, max(s[0], s[1]) > 128u);
 #pragma unroll
-  for (int b = 0; b < 2; ++b) {
-    const uint32_t f = factor(s[b]), w[4] = {q.c[b].x, q.c[b].y, q.c[b].z, q.c[b].w};
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t w[2] = {HALF ? q.c[t].z : q.c[t].x, HALF ? q.c[t].w : q.c[t].y};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int b = 0; b < 2; ++b) {
       uint32_t x[4];
-      values(w[i], f, x);
+      values(w[b], factor(s[b]), x);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[b * 16 + i * 4 + j] = x[j];
+      for (int j = 0; j < 4; ++j) v[b * 16 + t * 4 + j] = x[j];
     }
-    if (far) {
-      const uint32_t left = factor_left(s[b]);
+  }
+  if (far) {
+    const uint32_t left[2] = {factor_left(s[0]), factor_left(s[1])};
 #pragma unroll
-      for (int j = 0; j < 16; ++j) v[b * 16 + j] = mul2(v[b * 16 + j], left);
+    for (int j = 0; j < 32; ++j) {
+      v[j] = mul2(v[j], left[j >> 4]);
+      asm volatile("" : "+r"(v[j]));          // (a branch of its own, not 32 instructions that mostly do nothing)
     }
   }
 }
@@ -265,38 +271,46 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
       commit(acc_full);
     }
   } else {
-    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, k-blocks of this group's parity ----
+    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
     const int eight = r >> 3, row_tiles = ceil_div(p.N, TILE_ROWS);
     const int row_tile = (n0 >> 3) + (GATED ? eight >> 1 : eight);
     const bool valid = row_tile < row_tiles;
     const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (valid ? row_tile : 0)) * k_tiles + tile0;
-    const uint8_t* codes = p.codes + first * TILE_CODES + (2 * half * TILE_ROWS + (r & 7)) * 16;
-    const uint8_t* scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK) + 2 * half;
-    RowBlock q[S::AHEAD];
+    const uint8_t* codes = p.codes + first * TILE_CODES + (r & 7) * (TILE_K / 2);
+    const uint8_t* scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
+    const int tiles = ceil_div(num_kb, 2);
+    RowTile q[S::AHEAD];
 #pragma unroll
-    for (int u = 0; u < S::AHEAD; ++u) load_row_block(q[u], codes, scales, u, valid && 2 * u + half < num_kb);
+    for (int u = 0; u < S::AHEAD; ++u) load_row_tile(q[u], codes, scales, half + 2 * u, valid && half + 2 * u < tiles);
     bool ok = true;
-    for (int i0 = half; i0 < num_kb && ok; i0 += 2 * S::AHEAD) {
+    auto give = [&](int i, const uint32_t (&v)[32]) {           // the k-block's values to its stage, once the products have left that
+      const int s = i % S::A_STAGES;
+      if (i >= S::A_STAGES) ok = mbar_wait(&a_empty[s], ((i / S::A_STAGES) - 1) & 1) && *aborted == 0;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_store32(t_lane + BN + s * S::A_COLS, v);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_full[s]);
+      } else if (lane == 0) {
+        give_up();
+      }
+    };
+    for (int c0 = half; c0 < tiles && ok; c0 += 2 * S::AHEAD) {
 #pragma unroll
       for (int u = 0; u < S::AHEAD; ++u) {
-        const int i = i0 + 2 * u;
-        if (i < num_kb && ok) {
+        const int c = c0 + 2 * u;
+        if (c < tiles && ok) {
           uint32_t v[32];
-          convert(q[u], v);
-          load_row_block(q[u], codes, scales, (i >> 1) + S::AHEAD, valid && i + 2 * S::AHEAD < num_kb);
-          const int s = i % S::A_STAGES;
-          if (i >= S::A_STAGES) ok = __all_sync(0xffffffffu, mbar_wait(&a_empty[s], ((i / S::A_STAGES) - 1) & 1)) && *aborted == 0;
-          ok = __all_sync(0xffffffffu, ok);
-          if (ok) {
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            tmem_store32(t_lane + BN + s * S::A_COLS, v);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&a_full[s]);
-          } else if (lane == 0) {
-            give_up();
+          convert<0>(q[u], v);
+          give(2 * c, v);
+          if (ok && 2 * c + 1 < num_kb) {
+            convert<1>(q[u], v);
+            load_row_tile(q[u], codes, scales, c + 2 * S::AHEAD, valid && c + 2 * S::AHEAD < tiles);
+            give(2 * c + 1, v);
           }
         }
       }

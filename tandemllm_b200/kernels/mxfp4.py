@@ -23,18 +23,20 @@ from .build import Launchers, load
 
 BLOCK = 32                      # values a scale
 TILE_ROWS, TILE_K = 8, 128      # the layout's tiles
-FEW_ROWS = 32                   # rows up to which a product goes to the register-only kernel
-EXPERT_ROWS, EXPERT_PAIRS, EXPERT_TOP = 8, 256, 32      # the experts' two-kernel form
+FEW_ROWS = 16                   # rows up to which a product goes to the register-only kernel
+EXPERT_ROWS, EXPERT_TOP = 8, 32     # rows of the experts' two-kernel form, experts a row
 TILE_CODES, TILE_BYTES = TILE_ROWS * TILE_K // 2, TILE_ROWS * TILE_K * 17 // 32
 
 _SIGNATURES = {
     "tl_mxfp4_quantize": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
     "tl_mxfp4_values": [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p],
+    "tl_mxfp4_few_fits": [c_int, c_int, c_int, c_int],
     "tl_mxfp4_few": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_float, c_float,
-                     c_int, c_void_p],
-    "tl_mxfp4_experts_first": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int,
-                               c_int, c_int, c_int, c_float, c_float, c_void_p, c_void_p],
-    "tl_mxfp4_experts_second": [c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int,
+                     c_int, c_void_p, c_void_p],
+    "tl_mxfp4_experts_fit": [c_int, c_int, c_int, c_int],
+    "tl_mxfp4_experts_first": [c_void_p, c_longlong, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_int, c_int,
+                               c_int, c_float, c_float, c_void_p, c_void_p],
+    "tl_mxfp4_experts_second": [c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int,
                                 c_void_p, c_void_p],
     "tl_mxfp4_tc": [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_float,
                     c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
@@ -54,6 +56,7 @@ def lib():
             fn.argtypes = args
             fn.restype = c_int
         l.tl_mx_last_error.restype = ctypes.c_char_p
+        l.tl_mxfp4_experts_between.argtypes, l.tl_mxfp4_experts_between.restype = [c_int, c_int], c_longlong
         _lib = Launchers(l, _SIGNATURES)
     return _lib
 
@@ -84,10 +87,8 @@ class Mxfp4Matrix:
     def __init__(self, data: torch.Tensor, shape: tuple[int, ...]):
         self.data, self.shape, self.device = data, tuple(shape), data.device
         self.groups, self.n, self.k = (1 if len(shape) == 2 else shape[0]), shape[-2], shape[-1]
-        tiles = self.groups * -(-self.n // TILE_ROWS) * -(-self.k // TILE_K)
-        if data.dtype != torch.uint8 or not data.is_contiguous() or data.numel() != tiles * TILE_BYTES:
-            raise ops.KernelError(f"mxfp4: {data.numel()} bytes ({data.dtype}) for a matrix of shape {self.shape}")
-        self.index, self.codes, self.scales = data.get_device(), data.data_ptr(), data.data_ptr() + tiles * TILE_CODES
+        self.index, self.codes = data.get_device(), data.data_ptr()
+        self.scales = self.codes + data.numel() // TILE_BYTES * TILE_CODES
 
     @property
     def nbytes(self) -> int:
@@ -184,9 +185,9 @@ def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, o
     if rows == 0:
         return
     code = ops.dtype_code(out.dtype)
-    if rows <= FEW_ROWS:
+    if rows <= FEW_ROWS and lib().tl_mxfp4_few_fits(rows, w.n, w.k, act):
         _check(lib().tl_mxfp4_few(x.data_ptr(), ld, w.codes, w.scales, bias, out.data_ptr(), out.stride(0), rows, w.n, w.k, act, *constants, code,
-                                  ops.stream()), "mxfp4_few")
+                                  runtime.status.data_ptr(), ops.stream()), "mxfp4_few")
         return
     x, ld = _boxed(x, rows, w.k, ld)
     bn = token_tile(rows)
@@ -252,19 +253,18 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
     code = _gate(act)
     out = x.new_empty(rows, w_down.n, dtype=out_dtype)
     if rows:
-        form = _two_kernels if rows <= EXPERT_ROWS and rows * top <= EXPERT_PAIRS else _sorted
+        form = _two_kernels if rows <= EXPERT_ROWS and lib().tl_mxfp4_experts_fit(rows, top, w_first.k, w_down.k) else _sorted
         form(runtime, x, rows, ld, ids.data_ptr(), top, w, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants, out)
     return out
 
 
 def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
     E, inter, status, stream = w_down.groups, w_down.k, runtime.status.data_ptr(), ops.stream()
-    wide = -(-inter // 8) * 8
-    a = x.new_empty(rows * top, wide)
-    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, a.data_ptr(), wide, rows, inter, w_first.k, ids, wts,
+    between = x.new_empty(lib().tl_mxfp4_experts_between(rows * top, inter), dtype=torch.uint8)
+    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, between.data_ptr(), rows, inter, w_first.k, ids, wts,
                                         int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
-    _check(lib().tl_mxfp4_experts_second(a.data_ptr(), wide, w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter, ids, top,
-                                         E, ops.dtype_code(out.dtype), status, stream), "mxfp4_experts_second")
+    _check(lib().tl_mxfp4_experts_second(between.data_ptr(), w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter, ids, top,
+                                         E, act, ops.dtype_code(out.dtype), status, stream), "mxfp4_experts_second")
 
 
 def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
