@@ -69,27 +69,41 @@ struct Tc {
   static_assert(B_STAGES * B_BYTES >= BN * ROWS * 4, "an accumulator fits the ring of token boxes");
 };
 
-__device__ __forceinline__ uint64_t desc(uint32_t smem_addr) {  // K-major, 128-byte rows and swizzle: 8-row groups 1024 bytes apart
-  uint64_t d = 0;
-  d |= (uint64_t)((smem_addr >> 4) & 0x3FFF);
-  d |= (uint64_t)1 << 16;
-  d |= (uint64_t)(1024 >> 4) << 32;
-  d |= (uint64_t)1 << 46;
-  d |= (uint64_t)2 << 61;
-  return d;
+// A shared-memory operand, K-major with 128-byte rows and swizzle (8-row groups 1024 bytes apart), from 16 bytes' number `at16` on.
+__device__ __forceinline__ uint64_t desc(uint32_t at16) {
+  constexpr uint64_t FIXED = (uint64_t)1 << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+  return FIXED | at16;
 }
 
-__device__ __forceinline__ void mma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The whole warp goes through the products' loop and its lane `leader` issues: in a branch of one lane every operand would have to be moved to a
+// uniform register first (a k-block's four MMAs and two waits took 1100 cycles so, more than the products themselves).
+__device__ __forceinline__ void mma_a_tmem(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, l;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 l, %5, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
       : "memory");
 }
 
-__device__ __forceinline__ void commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "setp.ne.b32 l, %1, 0;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+      ::"r"(smem_u32(bar)), "r"(leader) : "memory");
+}
+
+// mbar_wait behind one look, which mostly suffices
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done || mbar_wait(bar, parity);
 }
 
 __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&v)[32]) {
@@ -254,22 +268,21 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
         for (int i = max(0, issued - S::B_STAGES); i < issued; ++i) mbar_wait(&b_full[i % S::B_STAGES], (i / S::B_STAGES) & 1);
     }
   } else if (warp == 1) {
-    if (lane == 0) {
-      // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
-      constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-      for (int i = 0; i < num_kb; ++i) {
-        const int sa = i % S::A_STAGES, sb = i % S::B_STAGES;
-        if (!mbar_wait(&b_full[sb], (i / S::B_STAGES) & 1) || !mbar_wait(&a_full[sa], (i / S::A_STAGES) & 1)) give_up();
-        if (*aborted) break;
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const uint32_t b = smem_u32(boxes + sb * S::B_BYTES), a = tmem_base + BN + sa * S::A_COLS;
+    // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
+    constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+    const uint32_t leader = lane == 0, boxes16 = smem_u32(boxes) >> 4;
+    for (int i = 0; i < num_kb; ++i) {
+      const int sa = i % S::A_STAGES, sb = i % S::B_STAGES;
+      if (!wait_for(&b_full[sb], (i / S::B_STAGES) & 1) || !wait_for(&a_full[sa], (i / S::A_STAGES) & 1)) give_up();
+      if (*aborted) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t b = boxes16 + sb * (S::B_BYTES >> 4), a = tmem_base + BN + sa * S::A_COLS;
 #pragma unroll
-        for (int k = 0; k < KB / 16; ++k) mma_a_tmem(tmem_base, a + k * 8, desc(b + k * 32), idesc, (i > 0 || k > 0) ? 1u : 0u);
-        commit(&b_empty[sb]);
-        commit(&a_empty[sa]);
-      }
-      commit(acc_full);
+      for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, tmem_base, a + k * 8, desc(b + k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
+      commit(leader, &b_empty[sb]);
+      commit(leader, &a_empty[sa]);
     }
+    commit(leader, acc_full);
   } else {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
@@ -287,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     bool ok = true;
     auto give = [&](int i, const uint32_t (&v)[32]) {           // the k-block's values to its stage, once the products have left that
       const int s = i % S::A_STAGES;
-      if (i >= S::A_STAGES) ok = mbar_wait(&a_empty[s], ((i / S::A_STAGES) - 1) & 1) && *aborted == 0;
+      if (i >= S::A_STAGES) ok = wait_for(&a_empty[s], ((i / S::A_STAGES) - 1) & 1) && *aborted == 0;
       ok = __all_sync(0xffffffffu, ok);
       if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -410,6 +423,318 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// The same for prompts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240 cycles)
+// hides under its products (2 cycles a token row). Tensor memory holds four stages of weights and two accumulators of 192 columns, or one of 256
+// where that saves a round; four warps of their own finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up to
+// 16, and they come in boxes of half a tile.
+template <int MAXN>
+struct Many {
+  static constexpr int BOX_ROWS = MAXN / 2;                      // token rows a TMA box
+  static constexpr int BOX_BYTES = BOX_ROWS * KB * 2;
+  static constexpr int B_BYTES = 2 * MAXN * KB * 2;              // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
+  static constexpr int B_STAGES = MAXN > 192 ? 3 : 4;
+  static constexpr int A_COLS = KB / 2;                          // a stage of weights: a k-block
+  static constexpr int A_STAGES = 4;
+  static constexpr int ACCS = MAXN > 192 ? 1 : 2;
+  static constexpr int A_AT = 512 - A_STAGES * A_COLS;           // the accumulators come first
+  static constexpr int CONVERT_WARPS = 8;
+  static constexpr int THREADS = (2 + CONVERT_WARPS + 4) * 32;
+  static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+  static_assert(ACCS * MAXN <= A_AT, "accumulators and weights share tensor memory");
+  static_assert(BOX_BYTES % 1024 == 0, "a box begins where the swizzle does");
+};
+
+__device__ __forceinline__ void gate_all(float (&g)[8], const float (&u)[8], const TcParams& p) {
+  if (p.act == TL_ACT_SILU) {          // (the fast exponential and division: the result is rounded to bfloat16, far coarser than their error)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = __fdividef(g[j], 1.f + __expf(-g[j])) * u[j];
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) g[j] = gated(g[j], u[j], p.act, p.ga0, p.ga1);
+  }
+}
+
+template <int MAXN, bool GATED, typename TOut>
+__global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const __grid_constant__ CUtensorMap tmX, TcParams p, int tile_at_most) {
+  using S = Many<MAXN>;
+  constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
+  chain_next();
+  chain_wait();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+  uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
+  uint64_t* b_empty = b_full + S::B_STAGES;
+  uint64_t* a_full = b_empty + S::B_STAGES;
+  uint64_t* a_empty = a_full + S::A_STAGES;
+  uint64_t* acc_full = a_empty + S::A_STAGES;
+  uint64_t* acc_empty = acc_full + 2;
+  uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
+  volatile uint32_t* aborted = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < S::B_STAGES; ++s) {
+      mbar_init(&b_full[s], 1);
+      mbar_init(&b_empty[s], 1);
+    }
+    for (int s = 0; s < S::A_STAGES; ++s) {
+      mbar_init(&a_full[s], 4);                                 // one arrival a warp of the group whose k-block it is
+      mbar_init(&a_empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);                              // one arrival a finishing warp
+    }
+    *aborted = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem_base = *tmem_slot;
+  auto give_up = [&]() {
+    *aborted = 1;
+    atomicExch(p.status, 11);
+  };
+
+  const int k_tiles = ceil_div(p.K, TILE_K), num_kb = ceil_div(p.K, KB), row_tiles = ceil_div(p.N, TILE_ROWS);
+  const int tiles_n = ceil_div(p.N, OUTS), tiles_m = p.tile_group ? *p.n_tiles : ceil_div(p.M, tile_at_most);
+  const int work = tiles_n * tiles_m;
+  // work item w: token tile w / tiles_n, weight tile w % tiles_n (neighbouring CTAs share token rows)
+  auto tokens_of = [&](int w, int& tok0, int& tok_rows) {
+    const int tm = w / tiles_n;
+    tok0 = p.tile_group ? p.tile_row0[tm] : tm * tile_at_most;
+    tok_rows = p.tile_group ? min(p.tile_rows[tm], MAXN) : min(tile_at_most, p.M - tok0);
+  };
+
+  if (warp == 0) {
+    // ---- token rows ----
+    int it = 0;
+    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x) {
+      int tok0, tok_rows;
+      tokens_of(w, tok0, tok_rows);
+      const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
+      for (int c = 0; c < k_tiles; ++c, ++it) {
+        const int s = it % S::B_STAGES, blocks = min(2, num_kb - 2 * c);
+        if (it >= S::B_STAGES && !wait_for(&b_empty[s], ((it / S::B_STAGES) - 1) & 1)) give_up();
+        if (*aborted) break;
+        if (lane == 0) {
+          mbar_expect_tx(&b_full[s], blocks * boxes_here * S::BOX_BYTES);
+          for (int i = 0; i < blocks; ++i)
+            for (int b = 0; b < boxes_here; ++b)
+              tma_load_2d(boxes + s * S::B_BYTES + i * (S::B_BYTES / 2) + b * S::BOX_BYTES, &tmX, &b_full[s], (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
+        }
+        __syncwarp();
+      }
+    }
+    if (*aborted)              // copies already started must land before the CTA's shared memory goes away
+      for (int i = max(0, it - S::B_STAGES); i < it; ++i) mbar_wait(&b_full[i % S::B_STAGES], (i / S::B_STAGES) & 1);
+  } else if (warp == 1) {
+    // ---- products ----
+    const uint32_t leader = lane == 0, boxes16 = smem_u32(boxes) >> 4;
+    int it = 0, itb = 0, nth = 0;
+    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x, ++nth) {
+      int tok0, tok_rows;
+      tokens_of(w, tok0, tok_rows);
+      const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ceil_div(tok_rows, 16) * 2) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+      const int acc = nth % S::ACCS;
+      const uint32_t d = tmem_base + acc * MAXN;
+      if (nth >= S::ACCS && !wait_for(&acc_empty[acc], ((nth / S::ACCS) - 1) & 1)) give_up();
+      if (*aborted) break;
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      for (int c = 0; c < k_tiles; ++c, ++itb) {
+        const int sb = itb % S::B_STAGES;
+        if (!wait_for(&b_full[sb], (itb / S::B_STAGES) & 1)) give_up();
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          if (2 * c + i >= num_kb) break;
+          const int sa = it % S::A_STAGES;
+          if (!wait_for(&a_full[sa], (it / S::A_STAGES) & 1)) give_up();
+          if (*aborted) break;
+          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+          const uint32_t b = boxes16 + sb * (S::B_BYTES >> 4) + i * (S::B_BYTES >> 5), a = tmem_base + S::A_AT + sa * S::A_COLS;
+#pragma unroll
+          for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + k * 8, desc(b + k * 2), idesc, (c > 0 || i > 0 || k > 0) ? 1u : 0u);
+          commit(leader, &a_empty[sa]);
+          ++it;
+        }
+        if (*aborted) break;
+        commit(leader, &b_empty[sb]);
+      }
+      commit(leader, &acc_full[acc]);          // (also where it gave up: whoever waits learns of it)
+    }
+    // the last products have left tensor memory and shared memory before anybody frees them
+    if (nth > 0) mbar_wait(&acc_full[(nth - 1) % S::ACCS], ((nth - 1) / S::ACCS) & 1);
+  } else if (warp < 2 + S::CONVERT_WARPS) {
+    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
+    const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, eight = r >> 3;
+    const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + S::A_AT;
+    // where a thread is: the work item, the tile of 128 k, and its row's first tile
+    struct Cursor {
+      int w, c;
+      const uint8_t* codes;
+      const uint8_t* scales;
+      bool valid;
+    };
+    auto enter = [&](Cursor& q, int w) {
+      q.w = w;
+      q.c = half;
+      q.valid = false;
+      q.codes = p.codes, q.scales = p.scales;
+      if (w >= work || half >= k_tiles) return;
+      const int tm = w / tiles_n, n0 = (w - tm * tiles_n) * OUTS, group = p.tile_group ? p.tile_group[tm] : 0;
+      const int row_tile = (n0 >> 3) + (GATED ? eight >> 1 : eight);
+      q.valid = row_tile < row_tiles;
+      const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (q.valid ? row_tile : 0)) * k_tiles;
+      q.codes = p.codes + first * TILE_CODES + (r & 7) * (TILE_K / 2);
+      q.scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
+    };
+    auto advance = [&](Cursor& q) {
+      q.c += 2;
+      if (q.c >= k_tiles) enter(q, q.w + gridDim.x);
+    };
+    constexpr int AHEAD = 2;
+    RowTile q[AHEAD];
+    Cursor next, now;
+    enter(next, blockIdx.x);
+    now = next;
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
+      advance(next);
+    }
+    int base = 0;                                               // k-blocks of the work items before this one
+    bool ok = half < k_tiles;
+    auto give = [&](int it, const uint32_t (&v)[32]) {          // the k-block's values to its stage, once the products have left that
+      const int s = it % S::A_STAGES;
+      if (it >= S::A_STAGES) ok = wait_for(&a_empty[s], ((it / S::A_STAGES) - 1) & 1) && *aborted == 0;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        tmem_store32(t_lane + s * S::A_COLS, v);
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&a_full[s]);
+      } else if (lane == 0) {
+        give_up();
+      }
+    };
+    while (ok && now.w < work) {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        if (!ok || now.w >= work) break;
+        uint32_t v[32];
+        convert<0>(q[u], v);
+        give(base + 2 * now.c, v);
+        if (ok && 2 * now.c + 1 < num_kb) {
+          convert<1>(q[u], v);
+          load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
+          give(base + 2 * now.c + 1, v);
+        } else {
+          load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
+        }
+        advance(next);
+        const int w = now.w;
+        now.c += 2;
+        if (now.c >= k_tiles) now.c = half, now.w = w + gridDim.x, base += num_kb;
+      }
+    }
+  } else {
+    // ---- results: accumulator rows 32 (warp % 4) .. + 31 ----
+    const int r = (warp & 3) * 32 + lane, eight = r >> 3;
+    const bool up = GATED && (eight & 1);
+    int nth = 0;
+    for (int w = blockIdx.x; w < work; w += gridDim.x, ++nth) {
+      int tok0, tok_rows;
+      tokens_of(w, tok0, tok_rows);
+      const int acc = nth % S::ACCS, n = (w % tiles_n) * OUTS + (GATED ? (r >> 4) * 8 + (r & 7) : r);
+      const bool mine = n < p.N;
+      const float bias = p.bias && mine ? p.bias[up ? p.N + n : n] : 0.f;
+      if (!__all_sync(0xffffffffu, mbar_wait(&acc_full[acc], (nth / S::ACCS) & 1) && *aborted == 0)) {
+        if (lane == 0) give_up();
+        break;
+      }
+      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * MAXN;
+      TOut* C = (TOut*)p.C;
+#pragma unroll 1
+      for (int c0 = 0; c0 < tok_rows; c0 += 16) {
+        float v[16];
+        tmem_load16(from + c0, v);
+        const int left = tok_rows - c0;
+        if (p.row_weight) {
+          const float weight = (lane & 15) < left ? pair_weight(p.row_weight, p.weight_index, (long long)tok0 + c0 + (lane & 15)) : 1.f;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] *= __shfl_sync(0xffffffffu, weight, j);
+        }
+        if (p.bias) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) v[j] += bias;
+        }
+        if constexpr (GATED) {
+          // of two tokens the lane with the gate row finishes the first and the one with the up row the second
+          float g[8], u[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[2 * j] : v[2 * j + 1], 8);
+            g[j] = up ? other : v[2 * j];
+            u[j] = up ? v[2 * j + 1] : other;
+          }
+          gate_all(g, u, p);
+          if (mine) {
+            TOut* to = C + (long long)(tok0 + c0 + (up ? 1 : 0)) * p.ldc + n;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              if (2 * j + (up ? 1 : 0) < left) store_one(to + (long long)(2 * j) * p.ldc, g[j]);
+          }
+        } else {
+          if (p.act < 0) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) v[j] = gate_activation(v[j], -p.act);
+          }
+          if (mine) {
+            TOut* to = C + (long long)(tok0 + c0) * p.ldc + n;
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              if (j < left) store_one(to + (long long)j * p.ldc, v[j]);
+          }
+        }
+      }
+      asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+    }
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u));
+  }
+}
+
+template <int MAXN, bool GATED, typename TOut>
+int launch_many(const CUtensorMap& tmX, const TcParams& p, int tile_at_most, long long work, cudaStream_t stream) {
+  using S = Many<MAXN>;
+  auto kernel = tc_many_kernel<MAXN, GATED, TOut>;
+  static thread_local int set_on = -1;              // the device whose function has its shared memory
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return (int)e;
+  if (set_on != dev) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL);
+    if (e != cudaSuccess) return (int)e;
+    set_on = dev;
+  }
+  kernel<<<(unsigned)(work < sm_count() ? work : sm_count()), S::THREADS, S::TOTAL, stream>>>(tmX, p, tile_at_most);
+  return (int)cudaGetLastError();
+}
+
 template <int BN, bool GATED, bool SPLIT, typename TOut>
 int launch_tc(const CUtensorMap& tmX, const TcParams& p, dim3 grid, cudaStream_t stream) {
   constexpr int BYTES = SPLIT ? Tc<BN>::SPLIT_TOTAL : Tc<BN>::TOTAL;
@@ -446,7 +771,8 @@ using namespace tl;
 
 // x [x_rows, K] bfloat16 (row stride ldx); the matrix N x K, or with `matrices` 2 a gate and an up matrix; grouped (tile_group ...): as many for
 // every group, x in the plan's order, tiles of at most `bn` rows. bias [N] (gated: [2 N]) 32-bit or null. out [M, N] (row stride ldc). `act`
-// as in tl_mxfp4_few. `bn`: token rows a tile, 16, 32, 64 or 128. `splits`: CTAs that share a tile's k, 1 to 8, none of them without any.
+// as in tl_mxfp4_few. `bn`: token rows a tile, 16, 32, 64, 128, or more than
+// that, a multiple of 16 up to 256, for the persistent form. `splits`: CTAs that share a tile's k, 1 to 8, none of them without any.
 extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const void* codes, const void* scales, const float* bias, void* out,
                            long long ldc, int M, int N, int K, int act, float a0, float a1, int out_dtype, int bn, int splits,
                            const int* tile_group, const int* tile_row0, const int* tile_rows, const int* n_tiles, int max_tiles,
@@ -466,6 +792,23 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
   splits = ceil_div(k_tiles, p.tiles_a_split);                  // (rounding up may leave the last ones nothing)
   p.tile_group = tile_group, p.tile_row0 = tile_row0, p.tile_rows = tile_rows, p.n_tiles = n_tiles;
   p.act = act, p.ga0 = a0, p.ga1 = a1, p.row_weight = row_weight, p.weight_index = weight_index, p.status = status;
+  if (bn > 128) {
+    TL_REQUIRE(splits == 1 && bn <= 256 && bn % 16 == 0, "mxfp4 product: token tiles of %d rows, k in %d runs", bn, splits);
+    const long long work = (long long)ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS) * (tile_group ? max_tiles : ceil_div(M, bn));
+    TL_REQUIRE(work <= 0x7FFFFFFF, "mxfp4 product: %lld tiles are too many", work);
+    CUtensorMap tmX;
+    const int r = tensor_map(x, x_rows, K, ldx, (bn <= 192 ? 192 : 256) / 2, &tmX);
+    if (r) return r;
+#define TL_MX_MANY(N_)                                                                                \
+  do {                                                                                                \
+    if (act > 0) return mx::launch_many<N_, true, bf16>(tmX, p, bn, work, stream);                    \
+    if (out_dtype == TL_FP32) return mx::launch_many<N_, false, float>(tmX, p, bn, work, stream);     \
+    return mx::launch_many<N_, false, bf16>(tmX, p, bn, work, stream);                                \
+  } while (0)
+    if (bn <= 192) TL_MX_MANY(192);
+    TL_MX_MANY(256);
+#undef TL_MX_MANY
+  }
   const dim3 grid(ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS), tile_group ? max_tiles : ceil_div(M, bn), splits);
   TL_REQUIRE(grid.y <= 65535, "mxfp4 product: %d token tiles exceed the grid limit", (int)grid.y);
   CUtensorMap tmX;

@@ -180,6 +180,23 @@ def splits_of(ctas: int, k: int, sms: int) -> int:
     return max(1, min(2 * sms // ctas, -(-k // TILE_K) // 2, 8))
 
 
+def shape_of(rows: int, row_tiles: int, k: int, sms: int) -> tuple[int, int]:
+    """(token rows a tile, CTAs that share a tile's k) of the tensor-core product of `rows` rows with `row_tiles` tiles of weight rows."""
+    blocks = -(-k // 64)
+    best = None
+    for n in range(-(-rows // 256), max(1, rows // 129) + 1):           # the persistent form: tiles of 144 to 256 rows, all about as high
+        h = max(144, -(-rows // (16 * n)) * 16)
+        cost = -(-row_tiles * n // sms) * blocks * max(2 * h, 260) + 12 * h + 4000
+        if best is None or cost < best[0]:
+            best = cost, h, 1
+    bn = token_tile(rows)
+    ctas = row_tiles * -(-rows // bn)
+    splits = splits_of(ctas, k, sms)
+    rounds = -(-ctas * splits // (2 * sms))
+    cost = rounds * -(-blocks // splits) * max(4 * bn, 480) * (0.6 if ctas * splits <= sms else 1.0) + 3000 + (2000 if splits > 1 else 0)
+    return best[1:] if best is not None and rows > 128 and best[0] < cost else (bn, splits)
+
+
 def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, out: torch.Tensor, act: int, constants) -> None:
     """out = the product of x's rows with w: act 0 plain, a gate's code gated, negated an activation on a plain product."""
     if rows == 0:
@@ -190,11 +207,9 @@ def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, o
                                   runtime.status.data_ptr(), ops.stream()), "mxfp4_few")
         return
     x, ld = _boxed(x, rows, w.k, ld)
-    bn = token_tile(rows)
-    ctas = -(-w.n // (64 if act > 0 else 128)) * -(-rows // bn)
+    bn, splits = shape_of(rows, -(-w.n // (64 if act > 0 else 128)), w.k, ops.sm_count())
     _check(lib().tl_mxfp4_tc(x.data_ptr(), ld, rows, w.codes, w.scales, bias, out.data_ptr(), out.stride(0), rows, w.n, w.k, act, *constants, code,
-                             bn, splits_of(ctas, w.k, ops.sm_count()), None, None, None, None, 0, None, None, runtime.status.data_ptr(),
-                             ops.stream()), "mxfp4_tc")
+                             bn, splits, None, None, None, None, 0, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
 
 
 def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
@@ -270,7 +285,7 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w
 def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
-    tile = token_tile(1.4 * pairs / E)
+    tile = token_tile(1.4 * pairs / E) if pairs <= 64 * E else 192
     tiles = min(pairs // tile + E, pairs)
     ints = x.new_empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32)
     counts = ints.data_ptr()
