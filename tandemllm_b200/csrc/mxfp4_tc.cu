@@ -54,12 +54,12 @@ struct TcParams {
 
 template <int BN>
 struct Tc {
-  static constexpr int B_BYTES = BN * KB * 2;
-  static constexpr int B_STAGES = BN >= 128 ? 6 : 8;
-  static constexpr int A_COLS = KB / 2;                         // columns of tensor memory a k-block of weights takes
-  static constexpr int A_STAGES = BN >= 128 ? 4 : 6;
+  static constexpr int HALF_BYTES = BN * KB * 2;
+  static constexpr int B_BYTES = 2 * HALF_BYTES;                // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
+  static constexpr int B_STAGES = BN >= 128 ? 3 : 4;
+  static constexpr int A_COLS = TILE_K / 2;                     // columns of tensor memory a stage of weights takes: a tile of 128 k
+  static constexpr int A_STAGES = 2;
   static constexpr int TMEM_COLS = 256;
-  static constexpr int AHEAD = 2;                               // tiles of codes a thread has at hand or on their way
   static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
   // What a launch with clusters asks for at least. A CTA of a cluster that waits for tensor memory keeps the others waiting, who keep
   // theirs; beside another kernel of clusters that could close a circle. With this much shared memory no SM has room for more CTAs of such kernels
@@ -67,6 +67,16 @@ struct Tc {
   static constexpr int SPLIT_TOTAL = TOTAL > 72 * 1024 ? TOTAL : 72 * 1024;
   static_assert(BN + A_STAGES * A_COLS <= TMEM_COLS, "accumulator and weights share half of tensor memory");
   static_assert(B_STAGES * B_BYTES >= BN * ROWS * 4, "an accumulator fits the ring of token boxes");
+};
+
+// A ring's place: its stage and how often it went round, for consumers (the parity to wait for) and producers (nothing to wait for on the first).
+template <int STAGES>
+struct Ring {
+  int stage = 0;
+  uint32_t round = 0;
+  __device__ __forceinline__ void next() {
+    if (++stage == STAGES) stage = 0, ++round;
+  }
 };
 
 // A shared-memory operand, K-major with 128-byte rows and swizzle (8-row groups 1024 bytes apart), from 16 bytes' number `at16` on.
@@ -191,6 +201,36 @@ __device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
   }
 }
 
+// A tile's values to a stage of tensor memory that is this warp's group's alone, for the `nth` time, once the products have left it; `then` runs
+// when the tile's codes are used up. False where the wait ran out or somebody gave up.
+template <typename Then>
+__device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* empty, int nth, volatile uint32_t* aborted, Then then) {
+  uint32_t v[32];
+  convert<0>(q, v);
+  if (!__all_sync(0xffffffffu, (nth == 0 || wait_for(empty, (nth - 1) & 1)) && *aborted == 0)) return false;
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  tmem_store32(taddr, v);
+  convert<1>(q, v);
+  then();
+  tmem_store32(taddr + KB / 2, v);
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(full);
+  return true;
+}
+
+// The products of a tile of 128 k (of its first 64 where there is no `second`): weights at `a` in tensor memory, token rows at 16 bytes' number `b` in
+// shared memory, the second 64 k `half16` behind the first.
+__device__ __forceinline__ void multiply_tile(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t half16, uint32_t idesc, bool add, bool second) {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+  for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + k * 8, desc(b + k * 2), idesc, (add || k > 0) ? 1u : 0u);
+  if (second) {
+#pragma unroll
+    for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + KB / 2 + k * 8, desc(b + half16 + k * 2), idesc, 1u);
+  }
+}
+
 template <typename TOut> __device__ __forceinline__ void store_one(TOut* p, float v) { *p = from_f32<TOut>(v); }
 
 template <int BN, bool GATED, bool SPLIT, typename TOut>
@@ -252,37 +292,39 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     atomicExch(p.status, 11);
   };
 
+  const int tiles = ceil_div(num_kb, 2);
   if (warp == 0) {
-    if (lane == 0) {
-      // ---- token rows ----
-      int issued = 0;
-      for (int i = 0; i < num_kb; ++i) {
-        const int s = i % S::B_STAGES;
-        if (i >= S::B_STAGES && !mbar_wait(&b_empty[s], ((i / S::B_STAGES) - 1) & 1)) give_up();
-        if (*aborted) break;
-        mbar_expect_tx(&b_full[s], S::B_BYTES);
-        tma_load_2d(boxes + s * S::B_BYTES, &tmX, &b_full[s], (kb0 + i) * KB, tok0);
-        issued = i + 1;
+    // ---- token rows ----
+    Ring<S::B_STAGES> ring;
+    int issued = 0;
+    for (int c = 0; c < tiles; ++c, ring.next()) {
+      if (ring.round && !wait_for(&b_empty[ring.stage], (ring.round - 1) & 1)) give_up();
+      if (*aborted) break;
+      const int blocks = min(2, num_kb - 2 * c);
+      if (lane == 0) {
+        mbar_expect_tx(&b_full[ring.stage], blocks * S::HALF_BYTES);
+        for (int i = 0; i < blocks; ++i)
+          tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES, &tmX, &b_full[ring.stage], (kb0 + 2 * c + i) * KB, tok0);
       }
-      if (*aborted)            // copies already started must land before the CTA's shared memory goes away
-        for (int i = max(0, issued - S::B_STAGES); i < issued; ++i) mbar_wait(&b_full[i % S::B_STAGES], (i / S::B_STAGES) & 1);
+      __syncwarp();
+      issued = c + 1;
     }
+    if (*aborted)              // copies already started must land before the CTA's shared memory goes away
+      for (int c = max(0, issued - S::B_STAGES); c < issued; ++c) mbar_wait(&b_full[c % S::B_STAGES], (c / S::B_STAGES) & 1);
   } else if (warp == 1) {
     // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-    const uint32_t leader = lane == 0, boxes16 = smem_u32(boxes) >> 4;
-    for (int i = 0; i < num_kb; ++i) {
-      const int sa = i % S::A_STAGES, sb = i % S::B_STAGES;
-      if (!wait_for(&b_full[sb], (i / S::B_STAGES) & 1) || !wait_for(&a_full[sa], (i / S::A_STAGES) & 1)) give_up();
+    Ring<S::A_STAGES> ra;
+    Ring<S::B_STAGES> rb;
+    for (int c = 0; c < tiles; ++c, ra.next(), rb.next()) {
+      if (!wait_for(&b_full[rb.stage], rb.round & 1) || !wait_for(&a_full[ra.stage], ra.round & 1)) give_up();
       if (*aborted) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      const uint32_t b = boxes16 + sb * (S::B_BYTES >> 4), a = tmem_base + BN + sa * S::A_COLS;
-#pragma unroll
-      for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, tmem_base, a + k * 8, desc(b + k * 2), idesc, (i > 0 || k > 0) ? 1u : 0u);
-      commit(leader, &b_empty[sb]);
-      commit(leader, &a_empty[sa]);
+      multiply_tile(lane == 0, tmem_base, tmem_base + BN + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
+                    c > 0, 2 * c + 1 < num_kb);
+      commit(lane == 0, &b_empty[rb.stage]);
+      commit(lane == 0, &a_empty[ra.stage]);
     }
-    commit(leader, acc_full);
+    commit(lane == 0, acc_full);
   } else {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
@@ -293,38 +335,21 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (valid ? row_tile : 0)) * k_tiles + tile0;
     const uint8_t* codes = p.codes + first * TILE_CODES + (r & 7) * (TILE_K / 2);
     const uint8_t* scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
-    const int tiles = ceil_div(num_kb, 2);
-    RowTile q[S::AHEAD];
+    constexpr int AHEAD = 2;                                    // tiles of codes a thread has at hand or on their way
+    RowTile q[AHEAD];
 #pragma unroll
-    for (int u = 0; u < S::AHEAD; ++u) load_row_tile(q[u], codes, scales, half + 2 * u, valid && half + 2 * u < tiles);
+    for (int u = 0; u < AHEAD; ++u) load_row_tile(q[u], codes, scales, half + 2 * u, valid && half + 2 * u < tiles);
     bool ok = true;
-    auto give = [&](int i, const uint32_t (&v)[32]) {           // the k-block's values to its stage, once the products have left that
-      const int s = i % S::A_STAGES;
-      if (i >= S::A_STAGES) ok = wait_for(&a_empty[s], ((i / S::A_STAGES) - 1) & 1) && *aborted == 0;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_store32(t_lane + BN + s * S::A_COLS, v);
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[s]);
-      } else if (lane == 0) {
-        give_up();
-      }
-    };
-    for (int c0 = half; c0 < tiles && ok; c0 += 2 * S::AHEAD) {
+    for (int c0 = half; c0 < tiles && ok; c0 += 2 * AHEAD) {
 #pragma unroll
-      for (int u = 0; u < S::AHEAD; ++u) {
+      for (int u = 0; u < AHEAD; ++u) {
         const int c = c0 + 2 * u;
         if (c < tiles && ok) {
-          uint32_t v[32];
-          convert<0>(q[u], v);
-          give(2 * c, v);
-          if (ok && 2 * c + 1 < num_kb) {
-            convert<1>(q[u], v);
-            load_row_tile(q[u], codes, scales, c + 2 * S::AHEAD, valid && c + 2 * S::AHEAD < tiles);
-            give(2 * c + 1, v);
-          }
+          // (stage `half` is this group's: its nth tile there is c / 2)
+          ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &a_full[half], &a_empty[half], c >> 1, aborted, [&]() {
+            load_row_tile(q[u], codes, scales, c + 2 * AHEAD, valid && c + 2 * AHEAD < tiles);
+          });
+          if (!ok && lane == 0) give_up();
         }
       }
     }
@@ -424,22 +449,24 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The same for prompts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240 cycles)
-// hides under its products (2 cycles a token row). Tensor memory holds four stages of weights and two accumulators of 192 columns, or one of 256
-// where that saves a round; four warps of their own finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up to
-// 16, and they come in boxes of half a tile.
+// The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240
+// cycles) hides under its products (2 cycles a token row). Tensor memory holds two stages of weights and two accumulators of 192 columns, or four
+// and one of 256 where that saves a round, or (few rows an expert) four and two of 64. Eight warps of their own finish a tile while the next one's
+// products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of half a tile or of 16.
 template <int MAXN>
 struct Many {
-  static constexpr int BOX_ROWS = MAXN / 2;                      // token rows a TMA box
+  static constexpr int BOX_ROWS = MAXN > 64 ? MAXN / 2 : 16;     // token rows a TMA box
   static constexpr int BOX_BYTES = BOX_ROWS * KB * 2;
-  static constexpr int B_BYTES = 2 * MAXN * KB * 2;              // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
+  static constexpr int HALF_BYTES = MAXN * KB * 2;
+  static constexpr int B_BYTES = 2 * HALF_BYTES;                 // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
   static constexpr int B_STAGES = MAXN > 192 ? 3 : 4;
-  static constexpr int A_COLS = KB / 2;                          // a stage of weights: a k-block
-  static constexpr int A_STAGES = 4;
+  static constexpr int A_COLS = TILE_K / 2;                      // a stage of weights: a tile of 128 k
+  static constexpr int A_STAGES = MAXN == 192 ? 2 : 4;
   static constexpr int ACCS = MAXN > 192 ? 1 : 2;
   static constexpr int A_AT = 512 - A_STAGES * A_COLS;           // the accumulators come first
   static constexpr int CONVERT_WARPS = 8;
-  static constexpr int THREADS = (2 + CONVERT_WARPS + 4) * 32;
+  static constexpr int FINISH_WARPS = 8;
+  static constexpr int THREADS = (2 + CONVERT_WARPS + FINISH_WARPS) * 32;
   static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
   static_assert(ACCS * MAXN <= A_AT, "accumulators and weights share tensor memory");
   static_assert(BOX_BYTES % 1024 == 0, "a box begins where the swizzle does");
@@ -484,7 +511,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 4);                              // one arrival a finishing warp
+      mbar_init(&acc_empty[b], S::FINISH_WARPS);                // one arrival each
     }
     *aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -514,62 +541,55 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
 
   if (warp == 0) {
     // ---- token rows ----
-    int it = 0;
+    Ring<S::B_STAGES> ring;
+    int issued = 0;
     for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x) {
       int tok0, tok_rows;
       tokens_of(w, tok0, tok_rows);
       const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
-      for (int c = 0; c < k_tiles; ++c, ++it) {
-        const int s = it % S::B_STAGES, blocks = min(2, num_kb - 2 * c);
-        if (it >= S::B_STAGES && !wait_for(&b_empty[s], ((it / S::B_STAGES) - 1) & 1)) give_up();
+      for (int c = 0; c < k_tiles; ++c, ring.next()) {
+        if (ring.round && !wait_for(&b_empty[ring.stage], (ring.round - 1) & 1)) give_up();
         if (*aborted) break;
+        const int blocks = min(2, num_kb - 2 * c);
         if (lane == 0) {
-          mbar_expect_tx(&b_full[s], blocks * boxes_here * S::BOX_BYTES);
+          mbar_expect_tx(&b_full[ring.stage], blocks * boxes_here * S::BOX_BYTES);
           for (int i = 0; i < blocks; ++i)
             for (int b = 0; b < boxes_here; ++b)
-              tma_load_2d(boxes + s * S::B_BYTES + i * (S::B_BYTES / 2) + b * S::BOX_BYTES, &tmX, &b_full[s], (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
+              tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, &b_full[ring.stage], (2 * c + i) * KB,
+                          tok0 + b * S::BOX_ROWS);
         }
         __syncwarp();
+        ++issued;
       }
     }
     if (*aborted)              // copies already started must land before the CTA's shared memory goes away
-      for (int i = max(0, it - S::B_STAGES); i < it; ++i) mbar_wait(&b_full[i % S::B_STAGES], (i / S::B_STAGES) & 1);
+      for (int c = max(0, issued - S::B_STAGES); c < issued; ++c) mbar_wait(&b_full[c % S::B_STAGES], (c / S::B_STAGES) & 1);
   } else if (warp == 1) {
     // ---- products ----
-    const uint32_t leader = lane == 0, boxes16 = smem_u32(boxes) >> 4;
-    int it = 0, itb = 0, nth = 0;
-    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x, ++nth) {
+    Ring<S::A_STAGES> ra;
+    Ring<S::B_STAGES> rb;
+    Ring<S::ACCS> rd;
+    int done = 0;
+    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x, rd.next()) {
       int tok0, tok_rows;
       tokens_of(w, tok0, tok_rows);
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ceil_div(tok_rows, 16) * 2) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-      const int acc = nth % S::ACCS;
-      const uint32_t d = tmem_base + acc * MAXN;
-      if (nth >= S::ACCS && !wait_for(&acc_empty[acc], ((nth / S::ACCS) - 1) & 1)) give_up();
+      if (rd.round && !wait_for(&acc_empty[rd.stage], (rd.round - 1) & 1)) give_up();
       if (*aborted) break;
-      asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-      for (int c = 0; c < k_tiles; ++c, ++itb) {
-        const int sb = itb % S::B_STAGES;
-        if (!wait_for(&b_full[sb], (itb / S::B_STAGES) & 1)) give_up();
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (2 * c + i >= num_kb) break;
-          const int sa = it % S::A_STAGES;
-          if (!wait_for(&a_full[sa], (it / S::A_STAGES) & 1)) give_up();
-          if (*aborted) break;
-          asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-          const uint32_t b = boxes16 + sb * (S::B_BYTES >> 4) + i * (S::B_BYTES >> 5), a = tmem_base + S::A_AT + sa * S::A_COLS;
-#pragma unroll
-          for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + k * 8, desc(b + k * 2), idesc, (c > 0 || i > 0 || k > 0) ? 1u : 0u);
-          commit(leader, &a_empty[sa]);
-          ++it;
-        }
+      const uint32_t d = tmem_base + rd.stage * MAXN;
+      for (int c = 0; c < k_tiles; ++c, ra.next(), rb.next()) {
+        if (!wait_for(&b_full[rb.stage], rb.round & 1) || !wait_for(&a_full[ra.stage], ra.round & 1)) give_up();
         if (*aborted) break;
-        commit(leader, &b_empty[sb]);
+        multiply_tile(lane == 0, d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
+                      c > 0, 2 * c + 1 < num_kb);
+        commit(lane == 0, &a_empty[ra.stage]);
+        commit(lane == 0, &b_empty[rb.stage]);
       }
-      commit(leader, &acc_full[acc]);          // (also where it gave up: whoever waits learns of it)
+      commit(lane == 0, &acc_full[rd.stage]);          // (also where it gave up: whoever waits learns of it)
+      ++done;
     }
     // the last products have left tensor memory and shared memory before anybody frees them
-    if (nth > 0) mbar_wait(&acc_full[(nth - 1) % S::ACCS], ((nth - 1) / S::ACCS) & 1);
+    if (done > 0) mbar_wait(&acc_full[(done - 1) % S::ACCS], ((done - 1) / S::ACCS) & 1);
   } else if (warp < 2 + S::CONVERT_WARPS) {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, eight = r >> 3;
@@ -608,46 +628,35 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
       advance(next);
     }
-    int base = 0;                                               // k-blocks of the work items before this one
-    bool ok = half < k_tiles;
-    auto give = [&](int it, const uint32_t (&v)[32]) {          // the k-block's values to its stage, once the products have left that
-      const int s = it % S::A_STAGES;
-      if (it >= S::A_STAGES) ok = wait_for(&a_empty[s], ((it / S::A_STAGES) - 1) & 1) && *aborted == 0;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_store32(t_lane + s * S::A_COLS, v);
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&a_full[s]);
-      } else if (lane == 0) {
-        give_up();
-      }
-    };
-    while (ok && now.w < work) {
+    // The tiles of all of the CTA's work items are one sequence; this group's are those of its parity in an item, so the stage of one is its place
+    // in the sequence, and how often the stage was used before it that place's round.
+    int at = half;                                              // the place of the tile at hand
+    bool ok = true;
+    while (ok && now.w < work && half < k_tiles) {
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         if (!ok || now.w >= work) break;
-        uint32_t v[32];
-        convert<0>(q[u], v);
-        give(base + 2 * now.c, v);
-        if (ok && 2 * now.c + 1 < num_kb) {
-          convert<1>(q[u], v);
+        const int stage = at % S::A_STAGES;
+        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &a_full[stage], &a_empty[stage], at / S::A_STAGES, aborted, [&]() {
           load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
-          give(base + 2 * now.c + 1, v);
-        } else {
-          load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
-        }
+        });
+        if (!ok && lane == 0) give_up();
         advance(next);
-        const int w = now.w;
+        const int before = now.c;
         now.c += 2;
-        if (now.c >= k_tiles) now.c = half, now.w = w + gridDim.x, base += num_kb;
+        if (now.c >= k_tiles) {
+          now.c = half, now.w += gridDim.x;
+          at += k_tiles - before + half;
+        } else {
+          at += 2;
+        }
       }
     }
   } else {
     // ---- results: accumulator rows 32 (warp % 4) .. + 31 ----
     const int r = (warp & 3) * 32 + lane, eight = r >> 3;
     const bool up = GATED && (eight & 1);
+    const int other = (warp - 2 - S::CONVERT_WARPS) >> 2;       // two warps a quarter of the rows, every other 16 columns each
     int nth = 0;
     for (int w = blockIdx.x; w < work; w += gridDim.x, ++nth) {
       int tok0, tok_rows;
@@ -663,7 +672,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * MAXN;
       TOut* C = (TOut*)p.C;
 #pragma unroll 1
-      for (int c0 = 0; c0 < tok_rows; c0 += 16) {
+      for (int c0 = other * 16; c0 < tok_rows; c0 += 32) {
         float v[16];
         tmem_load16(from + c0, v);
         const int left = tok_rows - c0;
@@ -681,9 +690,9 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
           float g[8], u[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float other = __shfl_xor_sync(0xffffffffu, up ? v[2 * j] : v[2 * j + 1], 8);
-            g[j] = up ? other : v[2 * j];
-            u[j] = up ? v[2 * j + 1] : other;
+            const float theirs = __shfl_xor_sync(0xffffffffu, up ? v[2 * j] : v[2 * j + 1], 8);
+            g[j] = up ? theirs : v[2 * j];
+            u[j] = up ? v[2 * j + 1] : theirs;
           }
           gate_all(g, u, p);
           if (mine) {
@@ -771,8 +780,8 @@ using namespace tl;
 
 // x [x_rows, K] bfloat16 (row stride ldx); the matrix N x K, or with `matrices` 2 a gate and an up matrix; grouped (tile_group ...): as many for
 // every group, x in the plan's order, tiles of at most `bn` rows. bias [N] (gated: [2 N]) 32-bit or null. out [M, N] (row stride ldc). `act`
-// as in tl_mxfp4_few. `bn`: token rows a tile, 16, 32, 64, 128, or more than
-// that, a multiple of 16 up to 256, for the persistent form. `splits`: CTAs that share a tile's k, 1 to 8, none of them without any.
+// as in tl_mxfp4_few. `splits` 0: the persistent form, in
+// tiles of up to `bn` <= 256 token rows; else token tiles of `bn` rows, 16, 32, 64 or 128, and the CTAs, 1 to 8, that share a tile's k.
 extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const void* codes, const void* scales, const float* bias, void* out,
                            long long ldc, int M, int N, int K, int act, float a0, float a1, int out_dtype, int bn, int splits,
                            const int* tile_group, const int* tile_row0, const int* tile_rows, const int* n_tiles, int max_tiles,
@@ -783,21 +792,23 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
   TL_REQUIRE(act <= 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 product: gate activation %d is none (nor an ungated one, negated)", act);
   TL_REQUIRE(act <= 0 || out_dtype == TL_BF16, "mxfp4 product: gated outputs of type %d", out_dtype);
   const int k_tiles = ceil_div(K, mx::TILE_K);
-  TL_REQUIRE(splits >= 1 && splits <= mx::MAX_SPLITS && splits <= k_tiles, "mxfp4 product: k %d in %d runs", K, splits);
+  TL_REQUIRE(splits >= 0 && splits <= mx::MAX_SPLITS && splits <= k_tiles, "mxfp4 product: k %d in %d runs", K, splits);
   TL_REQUIRE(!tile_group || (tile_row0 && tile_rows && n_tiles), "mxfp4 product: an incomplete plan (%d tiles)", max_tiles);
   mx::TcParams p = {};
   p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.bias = bias, p.C = out, p.ldc = ldc, p.M = M, p.N = N, p.K = K;
   p.matrices = act > 0 ? 2 : 1;
-  p.tiles_a_split = ceil_div(k_tiles, splits);
-  splits = ceil_div(k_tiles, p.tiles_a_split);                  // (rounding up may leave the last ones nothing)
+  if (splits) {
+    p.tiles_a_split = ceil_div(k_tiles, splits);
+    splits = ceil_div(k_tiles, p.tiles_a_split);                // (rounding up may leave the last ones nothing)
+  }
   p.tile_group = tile_group, p.tile_row0 = tile_row0, p.tile_rows = tile_rows, p.n_tiles = n_tiles;
   p.act = act, p.ga0 = a0, p.ga1 = a1, p.row_weight = row_weight, p.weight_index = weight_index, p.status = status;
-  if (bn > 128) {
-    TL_REQUIRE(splits == 1 && bn <= 256 && bn % 16 == 0, "mxfp4 product: token tiles of %d rows, k in %d runs", bn, splits);
+  if (splits == 0) {
+    TL_REQUIRE(bn >= 1 && bn <= 256, "mxfp4 product: token tiles of %d rows", bn);
     const long long work = (long long)ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS) * (tile_group ? max_tiles : ceil_div(M, bn));
     TL_REQUIRE(work <= 0x7FFFFFFF, "mxfp4 product: %lld tiles are too many", work);
     CUtensorMap tmX;
-    const int r = tensor_map(x, x_rows, K, ldx, (bn <= 192 ? 192 : 256) / 2, &tmX);
+    const int r = tensor_map(x, x_rows, K, ldx, bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 192 ? mx::Many<192>::BOX_ROWS : mx::Many<256>::BOX_ROWS, &tmX);
     if (r) return r;
 #define TL_MX_MANY(N_)                                                                                \
   do {                                                                                                \
@@ -805,6 +816,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     if (out_dtype == TL_FP32) return mx::launch_many<N_, false, float>(tmX, p, bn, work, stream);     \
     return mx::launch_many<N_, false, bf16>(tmX, p, bn, work, stream);                                \
   } while (0)
+    if (bn <= 64) TL_MX_MANY(64);
     if (bn <= 192) TL_MX_MANY(192);
     TL_MX_MANY(256);
 #undef TL_MX_MANY

@@ -181,14 +181,14 @@ def splits_of(ctas: int, k: int, sms: int) -> int:
 
 
 def shape_of(rows: int, row_tiles: int, k: int, sms: int) -> tuple[int, int]:
-    """(token rows a tile, CTAs that share a tile's k) of the tensor-core product of `rows` rows with `row_tiles` tiles of weight rows."""
+    """(token rows a tile, CTAs that share a tile's k, or 0 for the persistent form) of the tensor-core product of `rows` rows with `row_tiles` tiles of weight rows."""
     blocks = -(-k // 64)
     best = None
     for n in range(-(-rows // 256), max(1, rows // 129) + 1):           # the persistent form: tiles of 144 to 256 rows, all about as high
         h = max(144, -(-rows // (16 * n)) * 16)
         cost = -(-row_tiles * n // sms) * blocks * max(2 * h, 260) + 12 * h + 4000
         if best is None or cost < best[0]:
-            best = cost, h, 1
+            best = cost, h, 0
     bn = token_tile(rows)
     ctas = row_tiles * -(-rows // bn)
     splits = splits_of(ctas, k, sms)
@@ -285,7 +285,7 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w
 def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
-    tile = token_tile(1.4 * pairs / E) if pairs <= 64 * E else 192
+    tile = 64 if pairs <= 48 * E else 192
     tiles = min(pairs // tile + E, pairs)
     ints = x.new_empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32)
     counts = ints.data_ptr()
@@ -298,7 +298,7 @@ def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_firs
     wide = -(-inter // 8) * 8
     a = x.new_empty(pairs, wide)
     y = x.new_empty(pairs, hidden, dtype=torch.float32)
-    tail = (tile, 1, group, row0, n_rows, n_tiles, tiles)
+    tail = (tile, 0, group, row0, n_rows, n_tiles, tiles)
     _check(lib().tl_mxfp4_tc(xs.data_ptr(), ld, pairs, w_first.codes, w_first.scales, None, a.data_ptr(), wide, pairs, inter, w_first.k, act,
                              *constants, ops.BF16, *tail, wts if before else None, order if before else None, status, stream), "mxfp4_tc")
     _check(lib().tl_mxfp4_tc(a.data_ptr(), wide, pairs, w_down.codes, w_down.scales, None, y.data_ptr(), hidden, pairs, hidden, inter, 0, 0.0, 0.0,
