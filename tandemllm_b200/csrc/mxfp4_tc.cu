@@ -69,6 +69,12 @@ struct Tc {
   static_assert(B_STAGES * B_BYTES >= BN * ROWS * 4, "an accumulator fits the ring of token boxes");
 };
 
+// The products of the CTA's nth tile of 128 k arrive, once done, at done[nth % DONE]: its stages of weights and of token rows are then free. Whoever
+// fills a stage again waits for the tile that had it, at most DONE before its own, so no phase is missed.
+constexpr int DONE = 4;
+__device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity);
+__device__ __forceinline__ bool wait_done(uint64_t* done, int nth) { return nth < 0 || wait_for(&done[nth % DONE], (nth / DONE) & 1); }
+
 // A ring's place: its stage and how often it went round, for consumers (the parity to wait for) and producers (nothing to wait for on the first).
 template <int STAGES>
 struct Ring {
@@ -103,6 +109,34 @@ __device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
       "setp.ne.b32 l, %1, 0;\n\t"
       "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
       ::"r"(smem_u32(bar)), "r"(leader) : "memory");
+}
+
+// One box from (column x, row y), its bytes counted on `bar`; and the bytes that `bar` is to expect: by the lane `leader`, as above.
+__device__ __forceinline__ void load_box(uint32_t leader, uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "setp.ne.b32 l, %5, 0;\n\t"
+      "@l cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t leader, uint32_t bar, uint32_t bytes) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\t"
+      "setp.ne.b32 l, %2, 0;\n\t"
+      "@l mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
+      ::"r"(bar), "r"(bytes), "r"(leader) : "memory");
+}
+
+// Whether the phase with this parity is complete, without waiting.
+__device__ __forceinline__ bool look(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return done;
 }
 
 // mbar_wait behind one look, which mostly suffices
@@ -201,13 +235,13 @@ __device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
   }
 }
 
-// A tile's values to a stage of tensor memory that is this warp's group's alone, for the `nth` time, once the products have left it; `then` runs
-// when the tile's codes are used up. False where the wait ran out or somebody gave up.
+// A tile's values to a stage of tensor memory, once the products of the tile that had it (`before`; negative: none) are done; `then` runs when
+// the tile's codes are used up. False where the wait ran out or somebody gave up.
 template <typename Then>
-__device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* empty, int nth, volatile uint32_t* aborted, Then then) {
+__device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* done, int before, volatile uint32_t* aborted, Then then) {
   uint32_t v[32];
   convert<0>(q, v);
-  if (!__all_sync(0xffffffffu, (nth == 0 || wait_for(empty, (nth - 1) & 1)) && *aborted == 0)) return false;
+  if (!__all_sync(0xffffffffu, wait_done(done, before) && *aborted == 0)) return false;
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   tmem_store32(taddr, v);
   convert<1>(q, v);
@@ -258,23 +292,17 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
-  uint64_t* b_empty = b_full + S::B_STAGES;
-  uint64_t* a_full = b_empty + S::B_STAGES;
-  uint64_t* a_empty = a_full + S::A_STAGES;
-  uint64_t* acc_full = a_empty + S::A_STAGES;
+  uint64_t* a_full = b_full + S::B_STAGES;
+  uint64_t* done = a_full + S::A_STAGES;                        // [DONE]: see there
+  uint64_t* acc_full = done + DONE;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile uint32_t* aborted = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::B_STAGES; ++s) {
-      mbar_init(&b_full[s], 1);
-      mbar_init(&b_empty[s], 1);
-    }
-    for (int s = 0; s < S::A_STAGES; ++s) {
-      mbar_init(&a_full[s], 4);                                 // one arrival a warp of the group whose k-block it is
-      mbar_init(&a_empty[s], 1);
-    }
+    for (int s = 0; s < S::B_STAGES; ++s) mbar_init(&b_full[s], 1);
+    for (int s = 0; s < S::A_STAGES; ++s) mbar_init(&a_full[s], 4);       // one arrival a warp of the group whose tile it is
+    for (int s = 0; s < DONE; ++s) mbar_init(&done[s], 1);
     mbar_init(acc_full, 1);
     *aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -298,15 +326,14 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     Ring<S::B_STAGES> ring;
     int issued = 0;
     for (int c = 0; c < tiles; ++c, ring.next()) {
-      if (ring.round && !wait_for(&b_empty[ring.stage], (ring.round - 1) & 1)) give_up();
-      if (*aborted) break;
-      const int blocks = min(2, num_kb - 2 * c);
-      if (lane == 0) {
-        mbar_expect_tx(&b_full[ring.stage], blocks * S::HALF_BYTES);
-        for (int i = 0; i < blocks; ++i)
-          tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES, &tmX, &b_full[ring.stage], (kb0 + 2 * c + i) * KB, tok0);
+      if (!__all_sync(0xffffffffu, wait_done(done, c - S::B_STAGES) && *aborted == 0)) {
+        give_up();
+        break;
       }
-      __syncwarp();
+      const int blocks = min(2, num_kb - 2 * c);
+      const uint32_t bar = smem_u32(&b_full[ring.stage]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
+      expect(lane == 0, bar, blocks * S::HALF_BYTES);
+      for (int i = 0; i < blocks; ++i) load_box(lane == 0, to + i * S::HALF_BYTES, &tmX, bar, (kb0 + 2 * c + i) * KB, tok0);
       issued = c + 1;
     }
     if (*aborted)              // copies already started must land before the CTA's shared memory goes away
@@ -316,13 +343,17 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     Ring<S::A_STAGES> ra;
     Ring<S::B_STAGES> rb;
-    for (int c = 0; c < tiles; ++c, ra.next(), rb.next()) {
-      if (!wait_for(&b_full[rb.stage], rb.round & 1) || !wait_for(&a_full[ra.stage], ra.round & 1)) give_up();
-      if (*aborted) break;
-      multiply_tile(lane == 0, tmem_base, tmem_base + BN + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
-                    c > 0, 2 * c + 1 < num_kb);
-      commit(lane == 0, &b_empty[rb.stage]);
-      commit(lane == 0, &a_empty[ra.stage]);
+    bool there = false;
+    for (int c = 0; c < tiles; ++c) {
+      if (!there && !__all_sync(0xffffffffu, wait_for(&b_full[rb.stage], rb.round & 1) && wait_for(&a_full[ra.stage], ra.round & 1))) {
+        give_up();
+        break;
+      }
+      const uint32_t a = tmem_base + BN + ra.stage * S::A_COLS, b = smem_u32(boxes + rb.stage * S::B_BYTES) >> 4;
+      ra.next(), rb.next();
+      there = __all_sync(0xffffffffu, look(&b_full[rb.stage], rb.round & 1) && look(&a_full[ra.stage], ra.round & 1));
+      multiply_tile(lane == 0, tmem_base, a, b, S::HALF_BYTES >> 4, idesc, c > 0, 2 * c + 1 < num_kb);
+      commit(lane == 0, &done[c % DONE]);
     }
     commit(lane == 0, acc_full);
   } else {
@@ -345,8 +376,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
       for (int u = 0; u < AHEAD; ++u) {
         const int c = c0 + 2 * u;
         if (c < tiles && ok) {
-          // (stage `half` is this group's: its nth tile there is c / 2)
-          ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &a_full[half], &a_empty[half], c >> 1, aborted, [&]() {
+          ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &a_full[half], done, c - S::A_STAGES, aborted, [&]() {
             load_row_tile(q[u], codes, scales, c + 2 * AHEAD, valid && c + 2 * AHEAD < tiles);
           });
           if (!ok && lane == 0) give_up();
@@ -452,10 +482,10 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 // The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240
 // cycles) hides under its products (2 cycles a token row). Tensor memory holds two stages of weights and two accumulators of 192 columns, or four
 // and one of 256 where that saves a round, or (few rows an expert) four and two of 64. Eight warps of their own finish a tile while the next one's
-// products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of half a tile or of 16.
+// products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of 256, 96 or 16.
 template <int MAXN>
 struct Many {
-  static constexpr int BOX_ROWS = MAXN > 64 ? MAXN / 2 : 16;     // token rows a TMA box
+  static constexpr int BOX_ROWS = MAXN > 192 ? 256 : MAXN > 64 ? 96 : 16;      // token rows a TMA box
   static constexpr int BOX_BYTES = BOX_ROWS * KB * 2;
   static constexpr int HALF_BYTES = MAXN * KB * 2;
   static constexpr int B_BYTES = 2 * HALF_BYTES;                 // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
@@ -491,24 +521,18 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
-  uint64_t* b_empty = b_full + S::B_STAGES;
-  uint64_t* a_full = b_empty + S::B_STAGES;
-  uint64_t* a_empty = a_full + S::A_STAGES;
-  uint64_t* acc_full = a_empty + S::A_STAGES;
+  uint64_t* a_full = b_full + S::B_STAGES;
+  uint64_t* done = a_full + S::A_STAGES;                        // [DONE]: see there
+  uint64_t* acc_full = done + DONE;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile uint32_t* aborted = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::B_STAGES; ++s) {
-      mbar_init(&b_full[s], 1);
-      mbar_init(&b_empty[s], 1);
-    }
-    for (int s = 0; s < S::A_STAGES; ++s) {
-      mbar_init(&a_full[s], 4);                                 // one arrival a warp of the group whose k-block it is
-      mbar_init(&a_empty[s], 1);
-    }
+    for (int s = 0; s < S::B_STAGES; ++s) mbar_init(&b_full[s], 1);
+    for (int s = 0; s < S::A_STAGES; ++s) mbar_init(&a_full[s], 4);       // one arrival a warp of the group whose tile it is
+    for (int s = 0; s < DONE; ++s) mbar_init(&done[s], 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], S::FINISH_WARPS);                // one arrival each
@@ -543,22 +567,23 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     // ---- token rows ----
     Ring<S::B_STAGES> ring;
     int issued = 0;
-    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x) {
+    bool ok = true;
+    for (int w = blockIdx.x; w < work && ok; w += gridDim.x) {
       int tok0, tok_rows;
       tokens_of(w, tok0, tok_rows);
       const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
       for (int c = 0; c < k_tiles; ++c, ring.next()) {
-        if (ring.round && !wait_for(&b_empty[ring.stage], (ring.round - 1) & 1)) give_up();
-        if (*aborted) break;
-        const int blocks = min(2, num_kb - 2 * c);
-        if (lane == 0) {
-          mbar_expect_tx(&b_full[ring.stage], blocks * boxes_here * S::BOX_BYTES);
-          for (int i = 0; i < blocks; ++i)
-            for (int b = 0; b < boxes_here; ++b)
-              tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, &b_full[ring.stage], (2 * c + i) * KB,
-                          tok0 + b * S::BOX_ROWS);
+        if (!__all_sync(0xffffffffu, wait_done(done, issued - S::B_STAGES) && *aborted == 0)) {
+          give_up();
+          ok = false;
+          break;
         }
-        __syncwarp();
+        const int blocks = min(2, num_kb - 2 * c);
+        const uint32_t bar = smem_u32(&b_full[ring.stage]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
+        expect(lane == 0, bar, blocks * boxes_here * S::BOX_BYTES);
+        for (int i = 0; i < blocks; ++i)
+          for (int b = 0; b < boxes_here; ++b)
+            load_box(lane == 0, to + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, bar, (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
         ++issued;
       }
     }
@@ -569,27 +594,36 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     Ring<S::A_STAGES> ra;
     Ring<S::B_STAGES> rb;
     Ring<S::ACCS> rd;
-    int done = 0;
-    for (int w = blockIdx.x; w < work && !*aborted; w += gridDim.x, rd.next()) {
+    int tile = 0, items = 0;
+    bool ok = true, there = false;
+    for (int w = blockIdx.x; w < work && ok; w += gridDim.x, rd.next()) {
       int tok0, tok_rows;
       tokens_of(w, tok0, tok_rows);
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ceil_div(tok_rows, 16) * 2) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-      if (rd.round && !wait_for(&acc_empty[rd.stage], (rd.round - 1) & 1)) give_up();
-      if (*aborted) break;
+      if (!__all_sync(0xffffffffu, (rd.round == 0 || wait_for(&acc_empty[rd.stage], (rd.round - 1) & 1)) && *aborted == 0)) {
+        give_up();
+        break;
+      }
       const uint32_t d = tmem_base + rd.stage * MAXN;
-      for (int c = 0; c < k_tiles; ++c, ra.next(), rb.next()) {
-        if (!wait_for(&b_full[rb.stage], rb.round & 1) || !wait_for(&a_full[ra.stage], ra.round & 1)) give_up();
-        if (*aborted) break;
-        multiply_tile(lane == 0, d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
-                      c > 0, 2 * c + 1 < num_kb);
-        commit(lane == 0, &a_empty[ra.stage]);
-        commit(lane == 0, &b_empty[rb.stage]);
+      for (int c = 0; c < k_tiles; ++c, ++tile) {
+        if (!there && !__all_sync(0xffffffffu, wait_for(&b_full[rb.stage], rb.round & 1) && wait_for(&a_full[ra.stage], ra.round & 1))) {
+          give_up();
+          ok = false;
+          break;
+        }
+        const uint32_t a = tmem_base + S::A_AT + ra.stage * S::A_COLS, b = smem_u32(boxes + rb.stage * S::B_BYTES) >> 4;
+        // A look at the next tile's operands in front of this one's products: it costs the tensor pipe nothing there, and a wait behind them would
+        // leave it idle.
+        ra.next(), rb.next();
+        there = __all_sync(0xffffffffu, look(&b_full[rb.stage], rb.round & 1) && look(&a_full[ra.stage], ra.round & 1));
+        multiply_tile(lane == 0, d, a, b, S::HALF_BYTES >> 4, idesc, c > 0, 2 * c + 1 < num_kb);
+        commit(lane == 0, &done[tile % DONE]);
       }
       commit(lane == 0, &acc_full[rd.stage]);          // (also where it gave up: whoever waits learns of it)
-      ++done;
+      ++items;
     }
     // the last products have left tensor memory and shared memory before anybody frees them
-    if (done > 0) mbar_wait(&acc_full[(done - 1) % S::ACCS], ((done - 1) / S::ACCS) & 1);
+    if (items > 0) mbar_wait(&acc_full[(items - 1) % S::ACCS], ((items - 1) / S::ACCS) & 1);
   } else if (warp < 2 + S::CONVERT_WARPS) {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, eight = r >> 3;
@@ -637,7 +671,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       for (int u = 0; u < AHEAD; ++u) {
         if (!ok || now.w >= work) break;
         const int stage = at % S::A_STAGES;
-        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &a_full[stage], &a_empty[stage], at / S::A_STAGES, aborted, [&]() {
+        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &a_full[stage], done, at - S::A_STAGES, aborted, [&]() {
           load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
         });
         if (!ok && lane == 0) give_up();
