@@ -69,20 +69,19 @@ struct Tc {
   static_assert(B_STAGES * B_BYTES >= BN * ROWS * 4, "an accumulator fits the ring of token boxes");
 };
 
-// The products of the CTA's nth tile of 128 k arrive, once done, at done[nth % DONE]: its stages of weights and of token rows are then free. Whoever
-// fills a stage again waits for the tile that had it, at most DONE before its own, so no phase is missed.
-constexpr int DONE = 4;
+// The CTA's nth tile of 128 k has two barriers, full[nth % SLOTS] and done[nth % SLOTS]. Its weights (an arrival of each of the four warps that bring
+// them) and its token rows (the copying warp's arrival and their bytes) complete a phase of the one, its products a phase of the other: then its stages
+// of weights and of token rows are free. Whoever fills a stage again waits for the tile that had it, at most SLOTS before its own, so no phase
+// is missed and none of two tiles mixes.
+constexpr int SLOTS = 4;
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity);
-__device__ __forceinline__ bool wait_done(uint64_t* done, int nth) { return nth < 0 || wait_for(&done[nth % DONE], (nth / DONE) & 1); }
+__device__ __forceinline__ bool wait_nth(uint64_t* bars, int nth) { return nth < 0 || wait_for(&bars[nth % SLOTS], (nth / SLOTS) & 1); }
 
-// A ring's place: its stage and how often it went round, for consumers (the parity to wait for) and producers (nothing to wait for on the first).
+// The stage of a ring, tile by tile.
 template <int STAGES>
 struct Ring {
   int stage = 0;
-  uint32_t round = 0;
-  __device__ __forceinline__ void next() {
-    if (++stage == STAGES) stage = 0, ++round;
-  }
+  __device__ __forceinline__ void next() { stage = stage + 1 == STAGES ? 0 : stage + 1; }
 };
 
 // A shared-memory operand, K-major with 128-byte rows and swizzle (8-row groups 1024 bytes apart), from 16 bytes' number `at16` on.
@@ -129,7 +128,7 @@ __device__ __forceinline__ void expect(uint32_t leader, uint32_t bar, uint32_t b
 }
 
 // Whether the phase with this parity is complete, without waiting.
-__device__ __forceinline__ bool look(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ uint32_t look(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
@@ -241,7 +240,7 @@ template <typename Then>
 __device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* done, int before, volatile uint32_t* aborted, Then then) {
   uint32_t v[32];
   convert<0>(q, v);
-  if (!__all_sync(0xffffffffu, wait_done(done, before) && *aborted == 0)) return false;
+  if (!__all_sync(0xffffffffu, wait_nth(done, before) && *aborted == 0)) return false;
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   tmem_store32(taddr, v);
   convert<1>(q, v);
@@ -251,6 +250,16 @@ __device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(full);
   return true;
+}
+
+// After giving up: the copies of tiles from .. to - 1 that are under way land before the CTA's shared memory goes away. The converting warps may
+// have left without their arrivals, so those are made up for.
+__device__ __forceinline__ void drain(uint64_t* full, int from, int to, int lane) {
+  for (int c = max(0, from); c < to; ++c) {
+    if (lane < 4) mbar_arrive(&full[c % SLOTS]);
+    __syncwarp();
+    mbar_wait(&full[c % SLOTS], (c / SLOTS) & 1);
+  }
 }
 
 // The products of a tile of 128 k (of its first 64 where there is no `second`): weights at `a` in tensor memory, token rows at 16 bytes' number `b` in
@@ -291,18 +300,18 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
-  uint64_t* a_full = b_full + S::B_STAGES;
-  uint64_t* done = a_full + S::A_STAGES;                        // [DONE]: see there
-  uint64_t* acc_full = done + DONE;
+  uint64_t* full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
+  uint64_t* done = full + SLOTS;
+  uint64_t* acc_full = done + SLOTS;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile uint32_t* aborted = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::B_STAGES; ++s) mbar_init(&b_full[s], 1);
-    for (int s = 0; s < S::A_STAGES; ++s) mbar_init(&a_full[s], 4);       // one arrival a warp of the group whose tile it is
-    for (int s = 0; s < DONE; ++s) mbar_init(&done[s], 1);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&full[s], 5);
+      mbar_init(&done[s], 1);
+    }
     mbar_init(acc_full, 1);
     *aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -326,34 +335,34 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     Ring<S::B_STAGES> ring;
     int issued = 0;
     for (int c = 0; c < tiles; ++c, ring.next()) {
-      if (!__all_sync(0xffffffffu, wait_done(done, c - S::B_STAGES) && *aborted == 0)) {
+      if (!__all_sync(0xffffffffu, wait_nth(done, c - S::B_STAGES) && *aborted == 0)) {
         give_up();
         break;
       }
       const int blocks = min(2, num_kb - 2 * c);
-      const uint32_t bar = smem_u32(&b_full[ring.stage]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
+      const uint32_t bar = smem_u32(&full[c % SLOTS]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
       expect(lane == 0, bar, blocks * S::HALF_BYTES);
       for (int i = 0; i < blocks; ++i) load_box(lane == 0, to + i * S::HALF_BYTES, &tmX, bar, (kb0 + 2 * c + i) * KB, tok0);
       issued = c + 1;
     }
     if (*aborted)              // copies already started must land before the CTA's shared memory goes away
-      for (int c = max(0, issued - S::B_STAGES); c < issued; ++c) mbar_wait(&b_full[c % S::B_STAGES], (c / S::B_STAGES) & 1);
+      drain(full, issued - S::B_STAGES, issued, lane);
   } else if (warp == 1) {
     // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     Ring<S::A_STAGES> ra;
     Ring<S::B_STAGES> rb;
     bool there = false;
-    for (int c = 0; c < tiles; ++c) {
-      if (!there && !__all_sync(0xffffffffu, wait_for(&b_full[rb.stage], rb.round & 1) && wait_for(&a_full[ra.stage], ra.round & 1))) {
+    for (int c = 0; c < tiles; ++c, ra.next(), rb.next()) {
+      if (!there && !__all_sync(0xffffffffu, wait_nth(full, c))) {
         give_up();
         break;
       }
-      const uint32_t a = tmem_base + BN + ra.stage * S::A_COLS, b = smem_u32(boxes + rb.stage * S::B_BYTES) >> 4;
-      ra.next(), rb.next();
-      there = __all_sync(0xffffffffu, look(&b_full[rb.stage], rb.round & 1) && look(&a_full[ra.stage], ra.round & 1));
-      multiply_tile(lane == 0, tmem_base, a, b, S::HALF_BYTES >> 4, idesc, c > 0, 2 * c + 1 < num_kb);
-      commit(lane == 0, &done[c % DONE]);
+      const uint32_t next = look(&full[(c + 1) % SLOTS], ((c + 1) / SLOTS) & 1);
+      multiply_tile(lane == 0, tmem_base, tmem_base + BN + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
+                    c > 0, 2 * c + 1 < num_kb);
+      commit(lane == 0, &done[c % SLOTS]);
+      there = __all_sync(0xffffffffu, next);
     }
     commit(lane == 0, acc_full);
   } else {
@@ -376,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
       for (int u = 0; u < AHEAD; ++u) {
         const int c = c0 + 2 * u;
         if (c < tiles && ok) {
-          ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &a_full[half], done, c - S::A_STAGES, aborted, [&]() {
+          ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &full[c % SLOTS], done, c - S::A_STAGES, aborted, [&]() {
             load_row_tile(q[u], codes, scales, c + 2 * AHEAD, valid && c + 2 * AHEAD < tiles);
           });
           if (!ok && lane == 0) give_up();
@@ -520,19 +529,19 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   chain_wait();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* b_full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
-  uint64_t* a_full = b_full + S::B_STAGES;
-  uint64_t* done = a_full + S::A_STAGES;                        // [DONE]: see there
-  uint64_t* acc_full = done + DONE;
+  uint64_t* full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
+  uint64_t* done = full + SLOTS;
+  uint64_t* acc_full = done + SLOTS;
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile uint32_t* aborted = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < S::B_STAGES; ++s) mbar_init(&b_full[s], 1);
-    for (int s = 0; s < S::A_STAGES; ++s) mbar_init(&a_full[s], 4);       // one arrival a warp of the group whose tile it is
-    for (int s = 0; s < DONE; ++s) mbar_init(&done[s], 1);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&full[s], 5);
+      mbar_init(&done[s], 1);
+    }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
       mbar_init(&acc_empty[b], S::FINISH_WARPS);                // one arrival each
@@ -573,13 +582,13 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       tokens_of(w, tok0, tok_rows);
       const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
       for (int c = 0; c < k_tiles; ++c, ring.next()) {
-        if (!__all_sync(0xffffffffu, wait_done(done, issued - S::B_STAGES) && *aborted == 0)) {
+        if (!__all_sync(0xffffffffu, wait_nth(done, issued - S::B_STAGES) && *aborted == 0)) {
           give_up();
           ok = false;
           break;
         }
         const int blocks = min(2, num_kb - 2 * c);
-        const uint32_t bar = smem_u32(&b_full[ring.stage]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
+        const uint32_t bar = smem_u32(&full[issued % SLOTS]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
         expect(lane == 0, bar, blocks * boxes_here * S::BOX_BYTES);
         for (int i = 0; i < blocks; ++i)
           for (int b = 0; b < boxes_here; ++b)
@@ -588,7 +597,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       }
     }
     if (*aborted)              // copies already started must land before the CTA's shared memory goes away
-      for (int c = max(0, issued - S::B_STAGES); c < issued; ++c) mbar_wait(&b_full[c % S::B_STAGES], (c / S::B_STAGES) & 1);
+      drain(full, issued - S::B_STAGES, issued, lane);
   } else if (warp == 1) {
     // ---- products ----
     Ring<S::A_STAGES> ra;
@@ -600,24 +609,24 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       int tok0, tok_rows;
       tokens_of(w, tok0, tok_rows);
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ceil_div(tok_rows, 16) * 2) << 17) | ((uint32_t)(ROWS >> 4) << 24);
-      if (!__all_sync(0xffffffffu, (rd.round == 0 || wait_for(&acc_empty[rd.stage], (rd.round - 1) & 1)) && *aborted == 0)) {
+      if (!__all_sync(0xffffffffu, (items < S::ACCS || wait_for(&acc_empty[rd.stage], (items / S::ACCS - 1) & 1)) && *aborted == 0)) {
         give_up();
         break;
       }
       const uint32_t d = tmem_base + rd.stage * MAXN;
-      for (int c = 0; c < k_tiles; ++c, ++tile) {
-        if (!there && !__all_sync(0xffffffffu, wait_for(&b_full[rb.stage], rb.round & 1) && wait_for(&a_full[ra.stage], ra.round & 1))) {
+      for (int c = 0; c < k_tiles; ++c, ++tile, ra.next(), rb.next()) {
+        if (!there && !__all_sync(0xffffffffu, wait_nth(full, tile))) {
           give_up();
           ok = false;
           break;
         }
-        const uint32_t a = tmem_base + S::A_AT + ra.stage * S::A_COLS, b = smem_u32(boxes + rb.stage * S::B_BYTES) >> 4;
-        // A look at the next tile's operands in front of this one's products: it costs the tensor pipe nothing there, and a wait behind them would
+        // A look at the next tile's operands in front of this one's products, which costs the tensor pipe nothing there; a wait behind them would
         // leave it idle.
-        ra.next(), rb.next();
-        there = __all_sync(0xffffffffu, look(&b_full[rb.stage], rb.round & 1) && look(&a_full[ra.stage], ra.round & 1));
-        multiply_tile(lane == 0, d, a, b, S::HALF_BYTES >> 4, idesc, c > 0, 2 * c + 1 < num_kb);
-        commit(lane == 0, &done[tile % DONE]);
+        const uint32_t next = look(&full[(tile + 1) % SLOTS], ((tile + 1) / SLOTS) & 1);
+        multiply_tile(lane == 0, d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
+                      c > 0, 2 * c + 1 < num_kb);
+        commit(lane == 0, &done[tile % SLOTS]);
+        there = __all_sync(0xffffffffu, next);
       }
       commit(lane == 0, &acc_full[rd.stage]);          // (also where it gave up: whoever waits learns of it)
       ++items;
@@ -671,7 +680,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       for (int u = 0; u < AHEAD; ++u) {
         if (!ok || now.w >= work) break;
         const int stage = at % S::A_STAGES;
-        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &a_full[stage], done, at - S::A_STAGES, aborted, [&]() {
+        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &full[at % SLOTS], done, at - S::A_STAGES, aborted, [&]() {
           load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
         });
         if (!ok && lane == 0) give_up();
