@@ -73,7 +73,7 @@ struct Tc {
 // them) and its token rows (the copying warp's arrival and their bytes) complete a phase of the one, its products a phase of the other: then its stages
 // of weights and of token rows are free. Whoever fills a stage again waits for the tile that had it, at most SLOTS before its own, so no phase
 // is missed and none of two tiles mixes.
-constexpr int SLOTS = 4;
+constexpr int SLOTS = 8;
 __device__ __forceinline__ bool wait_for(uint64_t* bar, uint32_t parity);
 __device__ __forceinline__ bool wait_nth(uint64_t* bars, int nth) { return nth < 0 || wait_for(&bars[nth % SLOTS], (nth / SLOTS) & 1); }
 
@@ -90,41 +90,30 @@ __device__ __forceinline__ uint64_t desc(uint32_t at16) {
   return FIXED | at16;
 }
 
-// The whole warp goes through the products' loop and its lane `leader` issues: in a branch of one lane every operand would have to be moved to a
-// uniform register first (a k-block's four MMAs and two waits took 1100 cycles so, more than the products themselves).
-__device__ __forceinline__ void mma_a_tmem(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+// The whole warp goes through the loops that copy and multiply, and where something is issued, the one lane that `elected` names does it: in a branch of
+// a lane that the compiler cannot tell to be alone, every operand would first have to be made uniform (a k-block's four MMAs and two waits took
+// 1100 cycles so, more than the products themselves).
+__device__ __forceinline__ bool elected() {
+  uint32_t one;
   asm volatile(
-      "{\n\t.reg .pred p, l;\n\t"
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(one));
+  return one;
+}
+
+__device__ __forceinline__ void mma_a_tmem(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 l, %5, 0;\n\t"
-      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(leader)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
-__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
-  asm volatile(
-      "{\n\t.reg .pred l;\n\t"
-      "setp.ne.b32 l, %1, 0;\n\t"
-      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
-      ::"r"(smem_u32(bar)), "r"(leader) : "memory");
-}
-
-// One box from (column x, row y), its bytes counted on `bar`; and the bytes that `bar` is to expect: by the lane `leader`, as above.
-__device__ __forceinline__ void load_box(uint32_t leader, uint32_t to, const CUtensorMap* map, uint32_t bar, int x, int y) {
-  asm volatile(
-      "{\n\t.reg .pred l;\n\t"
-      "setp.ne.b32 l, %5, 0;\n\t"
-      "@l cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
-      ::"r"(to), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(leader)
-      : "memory");
-}
-__device__ __forceinline__ void expect(uint32_t leader, uint32_t bar, uint32_t bytes) {
-  asm volatile(
-      "{\n\t.reg .pred l;\n\t"
-      "setp.ne.b32 l, %2, 0;\n\t"
-      "@l mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}"
-      ::"r"(bar), "r"(bytes), "r"(leader) : "memory");
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
 
 // Whether the phase with this parity is complete, without waiting.
@@ -263,15 +252,20 @@ __device__ __forceinline__ void drain(uint64_t* full, int from, int to, int lane
 }
 
 // The products of a tile of 128 k (of its first 64 where there is no `second`): weights at `a` in tensor memory, token rows at 16 bytes' number `b` in
-// shared memory, the second 64 k `half16` behind the first.
-__device__ __forceinline__ void multiply_tile(uint32_t leader, uint32_t d, uint32_t a, uint32_t b, uint32_t half16, uint32_t idesc, bool add, bool second) {
+// shared memory, the second 64 k `half16` behind the first. Their end arrives at `done`.
+__device__ __forceinline__ void multiply_tile(uint32_t d, uint32_t a, uint32_t b, uint32_t half16, uint32_t idesc, bool add, bool second,
+                                              uint64_t* done) {
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  if (elected()) {
 #pragma unroll
-  for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + k * 8, desc(b + k * 2), idesc, (add || k > 0) ? 1u : 0u);
-  if (second) {
+    for (int k = 0; k < KB / 16; ++k) mma_a_tmem(d, a + k * 8, desc(b + k * 2), idesc, (add || k > 0) ? 1u : 0u);
+    if (second) {
 #pragma unroll
-    for (int k = 0; k < KB / 16; ++k) mma_a_tmem(leader, d, a + KB / 2 + k * 8, desc(b + half16 + k * 2), idesc, 1u);
+      for (int k = 0; k < KB / 16; ++k) mma_a_tmem(d, a + KB / 2 + k * 8, desc(b + half16 + k * 2), idesc, 1u);
+    }
+    commit(done);
   }
+  __syncwarp();
 }
 
 template <typename TOut> __device__ __forceinline__ void store_one(TOut* p, float v) { *p = from_f32<TOut>(v); }
@@ -340,9 +334,12 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
         break;
       }
       const int blocks = min(2, num_kb - 2 * c);
-      const uint32_t bar = smem_u32(&full[c % SLOTS]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
-      expect(lane == 0, bar, blocks * S::HALF_BYTES);
-      for (int i = 0; i < blocks; ++i) load_box(lane == 0, to + i * S::HALF_BYTES, &tmX, bar, (kb0 + 2 * c + i) * KB, tok0);
+      if (elected()) {
+        mbar_expect_tx(&full[c % SLOTS], blocks * S::HALF_BYTES);
+        for (int i = 0; i < blocks; ++i)
+          tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES, &tmX, &full[c % SLOTS], (kb0 + 2 * c + i) * KB, tok0);
+      }
+      __syncwarp();
       issued = c + 1;
     }
     if (*aborted)              // copies already started must land before the CTA's shared memory goes away
@@ -359,12 +356,12 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
         break;
       }
       const uint32_t next = look(&full[(c + 1) % SLOTS], ((c + 1) / SLOTS) & 1);
-      multiply_tile(lane == 0, tmem_base, tmem_base + BN + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
-                    c > 0, 2 * c + 1 < num_kb);
-      commit(lane == 0, &done[c % SLOTS]);
+      multiply_tile(tmem_base, tmem_base + BN + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc, c > 0,
+                    2 * c + 1 < num_kb, &done[c % SLOTS]);
       there = __all_sync(0xffffffffu, next);
     }
-    commit(lane == 0, acc_full);
+    if (elected()) commit(acc_full);
+    __syncwarp();
   } else {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
@@ -489,19 +486,21 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 
 // ---------------------------------------------------------------------------------------------------------------
 // The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240
-// cycles) hides under its products (2 cycles a token row). Tensor memory holds two stages of weights and two accumulators of 192 columns, or four
-// and one of 256 where that saves a round, or (few rows an expert) four and two of 64. Eight warps of their own finish a tile while the next one's
-// products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of 256, 96 or 16.
+// cycles) hides under its products (2 cycles a token row). Tensor memory holds two accumulators of 160 columns and three stages of weights, or one
+// of 256 and four where that saves a round, or (few rows an expert) two of 64 and six: the way of a stage, from its values to its products' end and
+// back, takes some 2000 cycles, of which every stage more hides a part (two stages beside two accumulators of 192: 103 us where these take XX).
+// Eight warps of their own finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up
+// to 16, and they come in boxes of 256, 80 or 16.
 template <int MAXN>
 struct Many {
-  static constexpr int BOX_ROWS = MAXN > 192 ? 256 : MAXN > 64 ? 96 : 16;      // token rows a TMA box
+  static constexpr int BOX_ROWS = MAXN > 160 ? 256 : MAXN > 64 ? 80 : 16;      // token rows a TMA box
   static constexpr int BOX_BYTES = BOX_ROWS * KB * 2;
   static constexpr int HALF_BYTES = MAXN * KB * 2;
   static constexpr int B_BYTES = 2 * HALF_BYTES;                 // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
-  static constexpr int B_STAGES = MAXN > 192 ? 3 : 4;
+  static constexpr int B_STAGES = MAXN > 160 ? 3 : MAXN > 64 ? 5 : 8;
   static constexpr int A_COLS = TILE_K / 2;                      // a stage of weights: a tile of 128 k
-  static constexpr int A_STAGES = MAXN == 192 ? 2 : 4;
-  static constexpr int ACCS = MAXN > 192 ? 1 : 2;
+  static constexpr int A_STAGES = MAXN > 160 ? 4 : MAXN > 64 ? 3 : 6;
+  static constexpr int ACCS = MAXN > 160 ? 1 : 2;
   static constexpr int A_AT = 512 - A_STAGES * A_COLS;           // the accumulators come first
   static constexpr int CONVERT_WARPS = 8;
   static constexpr int FINISH_WARPS = 8;
@@ -509,6 +508,7 @@ struct Many {
   static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
   static_assert(ACCS * MAXN <= A_AT, "accumulators and weights share tensor memory");
   static_assert(BOX_BYTES % 1024 == 0, "a box begins where the swizzle does");
+  static_assert(A_STAGES <= SLOTS && B_STAGES <= SLOTS, "see SLOTS");
 };
 
 __device__ __forceinline__ void gate_all(float (&g)[8], const float (&u)[8], const TcParams& p) {
@@ -588,11 +588,14 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
           break;
         }
         const int blocks = min(2, num_kb - 2 * c);
-        const uint32_t bar = smem_u32(&full[issued % SLOTS]), to = smem_u32(boxes) + ring.stage * S::B_BYTES;
-        expect(lane == 0, bar, blocks * boxes_here * S::BOX_BYTES);
-        for (int i = 0; i < blocks; ++i)
-          for (int b = 0; b < boxes_here; ++b)
-            load_box(lane == 0, to + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, bar, (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
+        if (elected()) {
+          uint64_t* bar = &full[issued % SLOTS];
+          mbar_expect_tx(bar, blocks * boxes_here * S::BOX_BYTES);
+          for (int i = 0; i < blocks; ++i)
+            for (int b = 0; b < boxes_here; ++b)
+              tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, bar, (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
+        }
+        __syncwarp();
         ++issued;
       }
     }
@@ -623,12 +626,12 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
         // A look at the next tile's operands in front of this one's products, which costs the tensor pipe nothing there; a wait behind them would
         // leave it idle.
         const uint32_t next = look(&full[(tile + 1) % SLOTS], ((tile + 1) / SLOTS) & 1);
-        multiply_tile(lane == 0, d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc,
-                      c > 0, 2 * c + 1 < num_kb);
-        commit(lane == 0, &done[tile % SLOTS]);
+        multiply_tile(d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc, c > 0,
+                      2 * c + 1 < num_kb, &done[tile % SLOTS]);
         there = __all_sync(0xffffffffu, next);
       }
-      commit(lane == 0, &acc_full[rd.stage]);          // (also where it gave up: whoever waits learns of it)
+      if (elected()) commit(&acc_full[rd.stage]);      // (also where it gave up: whoever waits learns of it)
+      __syncwarp();
       ++items;
     }
     // the last products have left tensor memory and shared memory before anybody frees them
@@ -851,7 +854,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     const long long work = (long long)ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS) * (tile_group ? max_tiles : ceil_div(M, bn));
     TL_REQUIRE(work <= 0x7FFFFFFF, "mxfp4 product: %lld tiles are too many", work);
     CUtensorMap tmX;
-    const int r = tensor_map(x, x_rows, K, ldx, bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 192 ? mx::Many<192>::BOX_ROWS : mx::Many<256>::BOX_ROWS, &tmX);
+    const int r = tensor_map(x, x_rows, K, ldx, bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 160 ? mx::Many<160>::BOX_ROWS : mx::Many<256>::BOX_ROWS, &tmX);
     if (r) return r;
 #define TL_MX_MANY(N_)                                                                                \
   do {                                                                                                \
@@ -860,7 +863,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     return mx::launch_many<N_, false, bf16>(tmX, p, bn, work, stream);                                \
   } while (0)
     if (bn <= 64) TL_MX_MANY(64);
-    if (bn <= 192) TL_MX_MANY(192);
+    if (bn <= 160) TL_MX_MANY(160);
     TL_MX_MANY(256);
 #undef TL_MX_MANY
   }

@@ -285,7 +285,7 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w
 def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
-    tile = 64 if pairs <= 48 * E else 192
+    tile = 64 if pairs <= 48 * E else 160
     tiles = min(pairs // tile + E, pairs)
     ints = x.new_empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32)
     counts = ints.data_ptr()
