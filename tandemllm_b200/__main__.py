@@ -26,6 +26,8 @@ def _engine_options(p: argparse.ArgumentParser) -> None:
     p.add_argument("--random-weights", type=int, metavar="SEED", help="random weights from this seed instead of --model")
     p.add_argument("--std", type=float, default=0.02, help="standard deviation of random matrices")
     p.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
+    p.add_argument("--feed-forward-weights", default="stored", choices=("stored", "mxfp4"),
+                   help="mxfp4: the feed-forwards' matrices rounded to 4-bit blocks (4.25 bits a weight) when they are loaded")
     p.add_argument("--max-len", type=int, default=8192, help="the window: prompt plus generated tokens of a request")
     p.add_argument("--parallel", type=int, default=8, help="requests running at once")
     p.add_argument("--block-size", type=int, default=16, help="tokens per cache page")
@@ -46,7 +48,8 @@ def _build_engine(a):
     from .engine import Engine, EngineArgs
     args = EngineArgs(dtype=a.dtype, max_len=a.max_len, parallel=a.parallel, block_size=a.block_size,
                       kv_blocks=a.kv_blocks, max_batched_tokens=a.max_batched_tokens, chunk_size=a.chunk_size,
-                      device=a.device, graph=a.graph == "on", log=a.log, record_routing=a.log_routing)
+                      device=a.device, graph=a.graph == "on", log=a.log, record_routing=a.log_routing,
+                      feed_forward_weights=a.feed_forward_weights)
     if a.random_weights is not None:
         if not a.config:
             raise SystemExit("--random-weights needs --config FILE (a config.json)")

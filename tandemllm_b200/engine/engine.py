@@ -52,6 +52,7 @@ class EngineArgs:
     tensorcore: bool = True             # use the tcgen05 kernels in bfloat16
     overlap: bool = True                # launch the next decode step before this one's tokens are read
     log: str | None = None              # a file that gets one JSON line a scheduler step (default: $TANDEMLLM_STEP_LOG)
+    feed_forward_weights: str = "stored"    # "mxfp4": the feed-forwards' matrices rounded to 4-bit blocks when they are loaded
     record_routing: bool = False        # count, step by step, the pairs routed to every expert of every routed layer
 
 
@@ -137,7 +138,7 @@ class Engine:
         dev = require_cuda(args.device)
         if args.dtype not in DTYPES:
             raise ValueError(f"dtype {args.dtype!r}: one of {', '.join(DTYPES)}")
-        runtime = Runtime(dev, DTYPES[args.dtype])
+        runtime = Runtime(dev, DTYPES[args.dtype], feed_forward_weights=args.feed_forward_weights)
         from ..kernels import ops
         ops.core()                                  # built and loaded now; a missing library fails here, loudly
         if runtime.dtype == torch.bfloat16 and args.tensorcore:

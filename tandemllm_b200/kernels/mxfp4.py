@@ -14,6 +14,7 @@ between calls but what the caller passes in. There is no 32-bit product: a 32-bi
 from __future__ import annotations
 
 import ctypes
+import functools
 from ctypes import c_float, c_int, c_longlong, c_void_p
 
 import torch
@@ -22,10 +23,13 @@ from . import ops
 from .build import Launchers, load
 
 BLOCK = 32                      # values a scale
+BYTES_A_VALUE = 17 / 32         # half a byte, and a scale's share
 TILE_ROWS, TILE_K = 8, 128      # the layout's tiles
 FEW_ROWS = 16                   # rows up to which a product goes to the register-only kernel
 EXPERT_ROWS, EXPERT_TOP = 8, 32     # rows of the experts' two-kernel form, experts a row
 TILE_CODES, TILE_BYTES = TILE_ROWS * TILE_K // 2, TILE_ROWS * TILE_K * 17 // 32
+
+ACTIVATIONS = tuple(ops.ACTIVATIONS[a] for a in ("silu", "gelu", "relu2", "identity"))     # those a plain product may end with
 
 _SIGNATURES = {
     "tl_mxfp4_quantize": [c_void_p, c_longlong, c_longlong, c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
@@ -170,31 +174,39 @@ def _output(out, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torc
     return out
 
 
-def token_tile(rows: float) -> int:
-    """Token rows of a tile of the tensor-core product for `rows` rows side by side."""
-    return 16 if rows <= 16 else 32 if rows <= 32 else 64 if rows <= 64 else 128
+@functools.lru_cache(maxsize=4096)
+def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[int, int]:
+    """(token rows a tile, CTAs that share a tile's k, or 0 for the persistent form) of the tensor-core product of `rows` rows with
+    `row_tiles` tiles of 128 weight rows.
 
-
-def splits_of(ctas: int, k: int, sms: int) -> int:
-    """CTAs that share a tile's k where `ctas` alone leave SMs idle (two CTAs an SM, each with at least two tiles of 128)."""
-    return max(1, min(2 * sms // ctas, -(-k // TILE_K) // 2, 8))
-
-
-def shape_of(rows: int, row_tiles: int, k: int, sms: int) -> tuple[int, int]:
-    """(token rows a tile, CTAs that share a tile's k, or 0 for the persistent form) of the tensor-core product of `rows` rows with `row_tiles` tiles of weight rows."""
-    blocks = -(-k // 64)
+    The form with the smallest estimated time, in us: `blocks` (of 128 k) one after the other in every round of CTAs, each as long as its
+    weights take to convert or, persistent, as its tokens take to multiply; a round's start and end; and, where CTAs share a tile's k, adding
+    their sums. The numbers are fitted to 1600 timings of 8 products with 17 to 4096 rows; over these the choice is 1.7 % slower than the
+    fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14.3 us in one persistent tile, 18.7 where two CTAs share
+    its k; 2048 rows 100 in tiles of 160, 107 in tiles of 192. At 2048 outputs of 7168: 256 rows 17.3 with eight CTAs a tile, 28 without;
+    700 rows 32 without, 43 with eight (and two rounds)."""
+    blocks = -(-k // TILE_K)
     best = None
-    for n in range(-(-rows // 256), max(1, rows // 129) + 1):           # the persistent form: tiles of 144 to 256 rows, all about as high
-        h = max(144, -(-rows // (16 * n)) * 16)
-        cost = -(-row_tiles * n // sms) * blocks * max(2 * h, 260) + 12 * h + 4000
+    for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
+        rounds = -(-row_tiles * -(-rows // h) // sms)
+        alone = 0.004 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
+        cost = 3.4 + rounds * (blocks * max(0.52, 0.0025 * h) + 0.96 + alone) + 0.0145 * h
         if best is None or cost < best[0]:
             best = cost, h, 0
-    bn = token_tile(rows)
-    ctas = row_tiles * -(-rows // bn)
-    splits = splits_of(ctas, k, sms)
-    rounds = -(-ctas * splits // (2 * sms))
-    cost = rounds * -(-blocks // splits) * max(4 * bn, 480) * (0.6 if ctas * splits <= sms else 1.0) + 3000 + (2000 if splits > 1 else 0)
-    return best[1:] if best is not None and rows > 128 and best[0] < cost else (bn, splits)
+    for bn in (16, 32, 64, 128):
+        if 4 * bn < min(rows, 128) or bn >= max(32, 2 * rows):
+            continue
+        for splits in (1, 2, 4, 8):
+            ctas = row_tiles * -(-rows // bn) * splits
+            if splits > 1 and (splits > blocks or ctas > 2 * sms):
+                break
+            rounds, rest = divmod(ctas, 2 * sms)                        # two CTAs an SM; one alone is faster
+            rounds += 0.0 if rest == 0 else 0.56 if rest <= sms else 1.0
+            cost = 4.4 + rounds * (-(-blocks // splits) * (0.735 + 0.0012 * bn) * (1.14 if gated else 1.0) + 0.31) + 0.0134 * bn
+            cost += 1.0 + 0.026 * bn if splits > 1 else 0.0
+            if cost < best[0]:
+                best = cost, bn, splits
+    return best[1:]
 
 
 def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, out: torch.Tensor, act: int, constants) -> None:
@@ -207,20 +219,24 @@ def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, o
                                   runtime.status.data_ptr(), ops.stream()), "mxfp4_few")
         return
     x, ld = _boxed(x, rows, w.k, ld)
-    bn, splits = shape_of(rows, -(-w.n // (64 if act > 0 else 128)), w.k, ops.sm_count())
+    bn, splits = shape_of(rows, -(-w.n // (64 if act > 0 else 128)), w.k, ops.sm_count(), act > 0)
     _check(lib().tl_mxfp4_tc(x.data_ptr(), ld, rows, w.codes, w.scales, bias, out.data_ptr(), out.stride(0), rows, w.n, w.k, act, *constants, code,
                              bn, splits, None, None, None, None, 0, None, None, runtime.status.data_ptr(), ops.stream()), "mxfp4_tc")
 
 
 def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
-           out: torch.Tensor | None = None) -> torch.Tensor:
-    """x [rows, k] times the one matrix w [n, k], plus `bias` (32-bit, [n]), in `out_dtype` (default: x's)."""
+           out: torch.Tensor | None = None, act: str | int | None = None) -> torch.Tensor:
+    """x [rows, k] times the one matrix w [n, k], plus `bias` (32-bit, [n]), through the activation `act` (silu, gelu, relu2 or identity, by
+    name or code; None: as it is), in `out_dtype` (default: `out`'s, else x's)."""
     if w.groups != 1:
         raise ops.KernelError(f"mxfp4 product: a stack of {w.groups} matrices where one is wanted")
     rows, ld = _rows(x, w)
     b = _vector(bias, w.n, "the bias", w.index)
     out = _output(out, rows, w.n, out_dtype or (out.dtype if out is not None else x.dtype), x)
-    _product(runtime, x, rows, ld, w, b, out, 0, (0.0, 0.0))
+    code = 0 if act is None else _gate(act)
+    if code and code not in ACTIVATIONS:
+        raise ops.KernelError(f"mxfp4 product: activation {act!r} behind a plain product; silu, gelu, relu2 and identity are implemented")
+    _product(runtime, x, rows, ld, w, b, out, -code, (0.0, 0.0))
     return out
 
 
@@ -245,13 +261,14 @@ def gated(runtime, x: torch.Tensor, w: Mxfp4Matrix, act: str | int = "silu", bia
 
 
 def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_first: Mxfp4Matrix, w_down: Mxfp4Matrix, act: str | int = "silu",
-            weigh: str = "output", out_dtype: torch.dtype | None = None, constants: tuple[float, float] = (0.0, 0.0)) -> torch.Tensor:
+            weigh: str = "output", out_dtype: torch.dtype | None = None, constants: tuple[float, float] = (0.0, 0.0), defer: bool = False):
     """out[r] = sum over the experts e = ids[r, :] (int32) of wts[r, :] (32-bit) times expert e of x[r], in `out_dtype` (default: x's).
 
     `w_down` [E, hidden, inter]; `w_first` [2 E, inter, hidden], the gate and the up matrix of every expert in turn: an expert is
     down( act(gate x) * (up x) ); or [E, inter, hidden] without gates: down( act(up x) ). `weigh` "input": the weight multiplies what the
     first product makes of x, in front of the activation, and the experts' rows are added as they are. An id outside 0 .. E - 1 adds
-    nothing and is recorded in the runtime's status word."""
+    nothing and is recorded in the runtime's status word. With `defer` the result of many rows is an `ops.ExpertRows`, whose consumer
+    weighs and adds the experts' rows itself."""
     E = w_down.groups
     gates = w_first.groups // max(E, 1)
     if gates not in (1, 2) or w_first.groups != gates * E or w_first.n != w_down.k or w_first.k != w_down.n or w_first.index != w_down.index:
@@ -266,23 +283,27 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
     if not 1 <= top <= EXPERT_TOP or not 1 <= E <= 1024:
         raise ops.KernelError(f"mxfp4 experts: top-{top} of {E}; up to top-{EXPERT_TOP} of 1024 are implemented")
     code = _gate(act)
-    out = x.new_empty(rows, w_down.n, dtype=out_dtype)
-    if rows:
-        form = _two_kernels if rows <= EXPERT_ROWS and lib().tl_mxfp4_experts_fit(rows, top, w_first.k, w_down.k) else _sorted
-        form(runtime, x, rows, ld, ids.data_ptr(), top, w, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants, out)
+    if gates == 1 and code not in ACTIVATIONS:
+        raise ops.KernelError(f"mxfp4 experts: activation {act!r} without a gate; silu, gelu, relu2 and identity are implemented")
+    if rows == 0:
+        return x.new_empty(0, w_down.n, dtype=out_dtype)
+    form = _two_kernels if rows <= EXPERT_ROWS and lib().tl_mxfp4_experts_fit(rows, top, w_first.k, w_down.k) else _sorted
+    return form(runtime, x, rows, ld, ids, top, w, wts, w_first, w_down, code if gates == 2 else -code, weigh == "input", constants,
+                out_dtype or x.dtype, defer)
+
+
+def _two_kernels(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first, w_down, act: int, before: bool, constants, dtype, defer):
+    out = x.new_empty(rows, w_down.n, dtype=dtype)
+    E, inter, status, stream = w_down.groups, w_down.k, runtime.status.data_ptr(), ops.stream()
+    between = x.new_empty(lib().tl_mxfp4_experts_between(rows * top, inter), dtype=torch.uint8)
+    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, between.data_ptr(), rows, inter, w_first.k, ids.data_ptr(), w,
+                                        int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
+    _check(lib().tl_mxfp4_experts_second(between.data_ptr(), w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter,
+                                         ids.data_ptr(), top, E, act, ops.dtype_code(dtype), status, stream), "mxfp4_experts_second")
     return out
 
 
-def _two_kernels(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
-    E, inter, status, stream = w_down.groups, w_down.k, runtime.status.data_ptr(), ops.stream()
-    between = x.new_empty(lib().tl_mxfp4_experts_between(rows * top, inter), dtype=torch.uint8)
-    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, between.data_ptr(), rows, inter, w_first.k, ids, wts,
-                                        int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
-    _check(lib().tl_mxfp4_experts_second(between.data_ptr(), w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter, ids, top,
-                                         E, act, ops.dtype_code(out.dtype), status, stream), "mxfp4_experts_second")
-
-
-def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_first, w_down, act: int, before: bool, constants, out) -> None:
+def _sorted(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first, w_down, act: int, before: bool, constants, dtype, defer):
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
     tile = 64 if pairs <= 48 * E else 160
@@ -293,15 +314,19 @@ def _sorted(runtime, x, rows: int, ld: int, ids: int, top: int, wts: int, w_firs
     place = order + 4 * pairs
     group, row0, n_rows = (place + 4 * (pairs + i * tiles) for i in range(3))
     n_tiles = n_rows + 4 * tiles
-    _check(lib().tl_mxfp4_plan(ids, pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, status, stream), "mxfp4_plan")
+    _check(lib().tl_mxfp4_plan(ids.data_ptr(), pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, status, stream), "mxfp4_plan")
     xs, ld = _boxed(x, pairs, w_first.k, ld, order, top)
     wide = -(-inter // 8) * 8
     a = x.new_empty(pairs, wide)
     y = x.new_empty(pairs, hidden, dtype=torch.float32)
     tail = (tile, 0, group, row0, n_rows, n_tiles, tiles)
     _check(lib().tl_mxfp4_tc(xs.data_ptr(), ld, pairs, w_first.codes, w_first.scales, None, a.data_ptr(), wide, pairs, inter, w_first.k, act,
-                             *constants, ops.BF16, *tail, wts if before else None, order if before else None, status, stream), "mxfp4_tc")
+                             *constants, ops.BF16, *tail, w if before else None, order if before else None, status, stream), "mxfp4_tc")
     _check(lib().tl_mxfp4_tc(a.data_ptr(), wide, pairs, w_down.codes, w_down.scales, None, y.data_ptr(), hidden, pairs, hidden, inter, 0, 0.0, 0.0,
                              ops.FP32, *tail, None, None, status, stream), "mxfp4_tc")
-    _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids, None if before else wts, out.data_ptr(), ops.dtype_code(out.dtype), rows, hidden, top, E,
-                              stream), "mxfp4_sum")
+    if defer:
+        return ops.ExpertRows(y, ints[E + pairs:E + 2 * pairs], ids, None if before else wts)
+    out = x.new_empty(rows, hidden, dtype=dtype)
+    _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids.data_ptr(), None if before else w, out.data_ptr(), ops.dtype_code(dtype), rows, hidden, top,
+                              E, stream), "mxfp4_sum")
+    return out

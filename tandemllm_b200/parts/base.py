@@ -86,6 +86,9 @@ def make_part(family: str, spec: PartSpec, **context):
     return table[spec.kind](spec, **context)
 
 
+FEED_FORWARD_WEIGHTS = ("stored", "mxfp4")
+
+
 @dataclass
 class Runtime:
     """Where and in which precision a model runs. `dtype` is the compute dtype: torch.float32 (everything in
@@ -95,10 +98,13 @@ class Runtime:
     status: torch.Tensor | None = None      # int32[1] on the device: kernels record a bad index here instead of faulting
     tensorcore: Any = None                  # the bfloat16 tensor-core kernels (kernels.tensorcore.TensorCore) or None
     attention_kernels: Any = None           # faster attention kernels for bfloat16, or None: the CUDA-core kernel
+    feed_forward_weights: str = "stored"    # the feed-forwards' matrices: in the compute dtype, or "mxfp4": rounded to 4-bit blocks
 
     def __post_init__(self) -> None:
         if self.dtype not in (torch.float32, torch.bfloat16):
             raise ValueError(f"compute dtype {self.dtype}: float32 and bfloat16 are implemented")
+        if self.feed_forward_weights not in FEED_FORWARD_WEIGHTS:
+            raise ValueError(f"feed-forward weights {self.feed_forward_weights!r}: one of {', '.join(FEED_FORWARD_WEIGHTS)}")
         if self.status is None and self.device.type == "cuda":
             self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
 
@@ -136,6 +142,24 @@ class Runtime:
 
     def vector(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(device=self.device, dtype=torch.float32).contiguous()
+
+    def feed_forward_source(self, t: torch.Tensor) -> torch.Tensor:
+        """A feed-forward's stored matrix on the device, in the dtype its matrix is made of: the compute dtype, or, where it is to be
+        rounded to 4-bit blocks, the stored one (both compute dtypes then round the same numbers)."""
+        if self.feed_forward_weights == "stored":
+            return self.matrix(t)
+        return t.to(device=self.device, dtype=t.dtype if t.dtype in (torch.float32, torch.bfloat16) else torch.float32).contiguous()
+
+    def feed_forward_matrix(self, t: torch.Tensor, matrices: int | None = None):
+        """The matrix [n, k] or the matrices [groups, n, k] of a feed-forward from `feed_forward_source`: as they are; with "mxfp4" a
+        `kernels.mxfp4.Mxfp4Matrix` of [groups * matrices, n / matrices, k] (`matrices`: those that lie below one another in each,
+        gate and up, say), or its values as a plain tensor where the products have no 4-bit form (32-bit, and bfloat16 without the
+        tensor-core kernels)."""
+        if self.feed_forward_weights == "stored":
+            return t
+        from ..kernels import mxfp4
+        q = mxfp4.quantize(t if matrices is None else t.view(-1, t.shape[-2] // matrices, t.shape[-1]))
+        return q if self.tensorcore is not None else q.values(self.dtype).view(t.shape)
 
 
 @dataclass(frozen=True)

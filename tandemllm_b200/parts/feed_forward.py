@@ -23,16 +23,26 @@ Gate and up are fused into one matrix at bind time ([2I, H], gate first), per ex
 `<experts>.down_proj [E, H, I]`); what the folder holds decides. Routing never leaves the device: the
 plan of (row, slot) pairs sorted by expert and its tile map are built by kernels, and the expert
 products skip experts nobody chose.
+
+A runtime whose `feed_forward_weights` are "mxfp4" rounds these matrices (not the router's, nor a shared part's gate) to 4-bit blocks at
+bind time, and the parts run the products of `kernels.mxfp4`; in 32-bit, and without the tensor-core kernels, the rounded values are
+plain matrices and everything else is as it is.
 """
 
 from __future__ import annotations
 
 import torch
 
-from ..kernels import ops
+from ..kernels import mxfp4, ops
 from ..weights.loader import TensorSpec
 from .base import FEED_FORWARDS, Part, register_part
 from .linear import linear
+
+
+def matrix_bytes(part, elem: int) -> float:
+    """Bytes of one element of a bound feed-forward's matrices (`elem`: of the compute dtype)."""
+    return mxfp4.BYTES_A_VALUE if isinstance(getattr(part, "w_down", None), mxfp4.Mxfp4Matrix) else elem
+
 
 def gate_constants_of(spec):
     """The constants of a gate form that has some, from a part's spec: `clamped_swish` reads `gate_limit` and `gate_slope`
@@ -67,14 +77,20 @@ class SwiGLU(Part):
     def bind(self, read, runtime):
         self.runtime = runtime
         sfx = self.suffix
-        self.w_gate_up = torch.cat([runtime.matrix(read(self.n["gate"] + sfx)),
-                                    runtime.matrix(read(self.n["up"] + sfx))]).contiguous()
-        self.w_down = runtime.matrix(read(self.n["down"] + sfx))
+        self.w_gate_up = runtime.feed_forward_matrix(torch.cat([runtime.feed_forward_source(read(self.n["gate"] + sfx)),
+                                                                runtime.feed_forward_source(read(self.n["up"] + sfx))]).contiguous(), 2)
+        self.w_down = runtime.feed_forward_matrix(runtime.feed_forward_source(read(self.n["down"] + sfx)))
         if self.bias_names:
             b = {k: runtime.vector(read(name)) for k, name in self.bias_names.items()}
             self.b_gate_up, self.b_down = torch.cat([b["gate"], b["up"]]).contiguous(), b["down"]
 
+    def step_bytes(self, elem: int, **kw) -> int:
+        return int(super().step_bytes(matrix_bytes(self, elem), **kw))
+
     def forward(self, x, step):
+        if isinstance(self.w_gate_up, mxfp4.Mxfp4Matrix):
+            act = mxfp4.gated(self.runtime, x, self.w_gate_up, self.act, self.b_gate_up, self.gate_constants or (0.0, 0.0))
+            return linear(self.runtime, act, self.w_down, self.b_down, out_dtype=torch.float32)
         act = torch.empty(x.shape[0], self.inter, dtype=x.dtype, device=x.device)
         tc = self.runtime.tensorcore
         if self.gate_constants is not None:
@@ -112,15 +128,24 @@ class DenseActivation(Part):
 
     def bind(self, read, runtime):
         self.runtime = runtime
-        self.w_up = runtime.matrix(read(self.n["up"]))
-        self.w_down = runtime.matrix(read(self.n["down"]))
+        self.w_up = runtime.feed_forward_matrix(runtime.feed_forward_source(read(self.n["up"])))
+        self.w_down = runtime.feed_forward_matrix(runtime.feed_forward_source(read(self.n["down"])))
         if self.activation == "xielu":
             pq = read(self.n["act_params"]).to(torch.float32).cpu()
             sp = torch.nn.functional.softplus(pq)
             self.a0, self.a1 = float(sp[0]), float(0.5 + sp[1])
 
+    def step_bytes(self, elem: int, **kw) -> int:
+        return int(super().step_bytes(matrix_bytes(self, elem), **kw))
+
     def forward(self, x, step):
         tc = self.runtime.tensorcore
+        if isinstance(self.w_up, mxfp4.Mxfp4Matrix):
+            fused = self.act in mxfp4.ACTIVATIONS
+            act = mxfp4.linear(self.runtime, x, self.w_up, act=self.act if fused else None)
+            if not fused:
+                ops.activation(act, act, self.act, self.a0, self.a1)
+            return linear(self.runtime, act, self.w_down, out_dtype=torch.float32)
         if tc is not None and x.dtype == torch.bfloat16:
             act = tc.linear_act(x, self.w_up, self.act, self.a0, self.a1)
             if act is not None:
@@ -212,17 +237,20 @@ class SigmoidTopKExperts(Part):
         self.w_router = runtime.vector(read(self.prefix + self.n["router"] + self.suffix))
         self.expert_bias = runtime.vector(read(self.prefix + self.n["bias"])) if self.use_bias else None
         if self.stacked:
-            self.w_gate_up = runtime.matrix(read(self.base + ".gate_up_proj"))
-            self.w_down = runtime.matrix(read(self.base + ".down_proj"))
+            w_gate_up = runtime.feed_forward_source(read(self.base + ".gate_up_proj"))
+            w_down = runtime.feed_forward_source(read(self.base + ".down_proj"))
         else:
             up_at = I if self.gated else 0          # (without a gate the up rows are all there is)
-            self.w_gate_up = torch.empty(E, up_at + I, H, dtype=runtime.dtype, device=runtime.device)
-            self.w_down = torch.empty(E, H, I, dtype=runtime.dtype, device=runtime.device)
+            dtype = runtime.feed_forward_source(read(self._expert(0, "up"))[:1]).dtype
+            w_gate_up = torch.empty(E, up_at + I, H, dtype=dtype, device=runtime.device)
+            w_down = torch.empty(E, H, I, dtype=dtype, device=runtime.device)
             for e in range(E):
                 if self.gated:
-                    self.w_gate_up[e, :I].copy_(read(self._expert(e, "gate")))
-                self.w_gate_up[e, up_at:].copy_(read(self._expert(e, "up")))
-                self.w_down[e].copy_(read(self._expert(e, "down")))
+                    w_gate_up[e, :I].copy_(read(self._expert(e, "gate")))
+                w_gate_up[e, up_at:].copy_(read(self._expert(e, "up")))
+                w_down[e].copy_(read(self._expert(e, "down")))
+        self.w_gate_up = runtime.feed_forward_matrix(w_gate_up, 2 if self.gated else 1)
+        self.w_down = runtime.feed_forward_matrix(w_down)
 
     def expected_experts_read(self, rows: int) -> float:
         """Distinct experts that `rows` rows choose when every expert is as likely as any other."""
@@ -234,7 +262,7 @@ class SigmoidTopKExperts(Part):
         of distinct experts `rows` rows choose)."""
         H, I, E = self.hidden_size, self.inter, self.num_experts
         n = self.expected_experts_read(rows) if experts_read is None else experts_read
-        return int(E * H * 4 + (E * 4 if self.use_bias else 0) + n * (3 if self.gated else 2) * H * I * elem)
+        return int(E * H * 4 + (E * 4 if self.use_bias else 0) + n * (3 if self.gated else 2) * H * I * matrix_bytes(self, elem))
 
     def count_into(self, counts: torch.Tensor | None) -> None:
         """From now on every pass adds the pairs it routed to each expert to `counts` (an integer tensor [experts] on
@@ -288,12 +316,17 @@ class SigmoidTopKExperts(Part):
 
     def forward(self, x, step, x32=None, routing=None):
         """The layer's output as `ops.ExpertRows`: one 32-bit row per (row, slot) pair, which the consuming norm
-        kernel weighs and adds in ascending expert id. `routing` = (ids, wts) when the norm in front already ran
-        the router; else it runs here, on `x32` (the unrounded normed rows) where given."""
+        kernel weighs and adds in ascending expert id; of few rows and 4-bit weights their sum. `routing` = (ids, wts) when
+        the norm in front already ran the router; else it runs here, on `x32` (the unrounded normed rows) where given."""
         R, H = x.shape[0], self.hidden_size
         ids, wts = routing if routing is not None else self.route(x32 if x32 is not None else x.float())
         if step is not None and step.trace is not None:
             step.trace.setdefault("routes", []).append((self.prefix, ids))
+        if isinstance(self.w_gate_up, mxfp4.Mxfp4Matrix):
+            if self.load is not None:
+                self.load.add_(self.plan_for(R * self.top_k, x.device).build(ids).counts)
+            return mxfp4.experts(self.runtime, x, ids, wts, self.w_gate_up, self.w_down, abs(self.act),
+                                 "input" if self.weighs_input else "output", torch.float32, self.gate_constants or (0.0, 0.0), defer=True)
         tc = self.runtime.tensorcore
         if self.gate_constants is not None:
             ops.gate_constants(*self.gate_constants)
@@ -373,4 +406,7 @@ class SharedAndRouted(Part):
         gate = None
         if self.w_gate is not None:
             gate = ops.RowDot(x, self.w_gate)
+        if isinstance(routed, torch.Tensor):            # the sum is there already: one row a row
+            at = self.runtime.tensorcore.pair_order()[:x.shape[0]].view(-1, 1)
+            routed = ops.ExpertRows(routed, at, at, None)
         return ops.GatedSum(shared, gate, routed)

@@ -9,17 +9,21 @@ With `defer` (a branch's last product, whose result only goes into the residual)
 `ops.PartialSums` instead of a tensor: partial sums that the consuming norm kernel adds itself. `defer="rounded"`
 allows the same for a result of any precision, whose consumer adds the sums and rounds them as the product would
 have. `ops.materialize` turns any such result into a plain tensor.
+
+A matrix in 4-bit blocks (`kernels.mxfp4.Mxfp4Matrix`) has products of its own.
 """
 
 from __future__ import annotations
 
 import torch
 
-from ..kernels import ops
+from ..kernels import mxfp4, ops
 
 
 def linear(runtime, x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
            out_dtype: torch.dtype | None = None, out: torch.Tensor | None = None, defer: bool = False):
+    if isinstance(w, mxfp4.Mxfp4Matrix):
+        return mxfp4.linear(runtime, x, w, bias, out_dtype, out)
     M, N = x.shape[0], w.shape[0]
     if defer and out is None and x.dtype == w.dtype == torch.float32 and out_dtype in (None, torch.float32):
         run = ops.simt_runs(M, N, x.shape[1])

@@ -17,6 +17,7 @@ import torch
 
 from ..config.spec import ModelSpec
 from ..kernels import ops
+from ..kernels.mxfp4 import Mxfp4Matrix
 from ..settings import SETTINGS
 from ..weights.loader import TensorSpec
 from .base import Runtime, SlotNeed, StepContext, make_part
@@ -86,6 +87,8 @@ class DecoderModel:
                     if isinstance(v, torch.Tensor) and v.is_cuda and v.data_ptr() not in seen:
                         seen.add(v.data_ptr())
                         total += v.numel() * v.element_size()
+                    elif isinstance(v, Mxfp4Matrix):
+                        total += v.nbytes
                     elif hasattr(v, "weight_specs") and v is not o:
                         stack.append(v)
         return total
