@@ -1373,6 +1373,8 @@ def main() -> int:
     ap.add_argument("--batch", type=int, default=BATCH)
     ap.add_argument("--context", type=int, default=CONTEXT)
     ap.add_argument("--dtype", default="bfloat16", choices=("bfloat16", "float32"))
+    ap.add_argument("--feed-forward-weights", default="stored", choices=("stored", "mxfp4"),
+                    help="mxfp4: the feed-forwards' matrices in 4-bit blocks (the line's dtype says so)")
     ap.add_argument("--graph", default="on", choices=("on", "off"))
     ap.add_argument("--skip-points", action="store_true", help="only the headline batch (for profiling runs)")
     ap.add_argument("--prefill-tokens", type=int, default=PREFILL_TOKENS,
@@ -1433,7 +1435,8 @@ def main() -> int:
     t0 = time.time()
     engine = Engine.from_config(cfg, seed=0, args=EngineArgs(
         dtype=a.dtype, max_len=room, parallel=max(max_batch, a.batch), block_size=16,
-        max_batched_tokens=max(only_tokens, max_batch), chunk_size=only_tokens, graph=a.graph == "on"))
+        max_batched_tokens=max(only_tokens, max_batch), chunk_size=only_tokens, graph=a.graph == "on",
+        feed_forward_weights=a.feed_forward_weights))
     torch.cuda.synchronize()
     load_s = time.time() - t0
     if a.chain == "on":
@@ -1668,7 +1671,8 @@ def main() -> int:
         "metric": f"decode tok/s at batch {a.batch}, context {a.context} ({model_name}, B200)",
         "value": round(main_run["tok_s"], 1), "unit": "tok/s", "n_gpus": 1, "steps": a.steps, "warmup": a.warmup,
         "ms_per_step": round(main_run["ms_per_step"], 4), "higher_is_better": True, "scaling": "weak",
-        "vs_baseline": None, "dtype": "bf16" if bf16 else "fp32",
+        "vs_baseline": None,
+        "dtype": ("bf16" if bf16 else "fp32") + ("" if a.feed_forward_weights == "stored" else ", feed-forward weights mxfp4"),
         "data": "synthetic: random weights N(0, 0.02), uniform random token ids, random keys and values as context",
         "impl": "ours", "repeats": REPEATS, "regions_ms": main_run["regions_ms"],
         "config": {"model": model_name, "layers": a.layers, "layers_of_model": layers_of_model,
