@@ -46,6 +46,12 @@ __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, ui
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma_16816_first(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                ::"r"(smem_u32(dst)), "l"(src), "r"(bytes), "r"(smem_u32(bar)) : "memory");
@@ -76,14 +82,15 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4& lo4, 
       values16(lo[b0 + b], u[b]);
       values16(hi[b0 + b], v[b]);
     }
-    float c[2][NT][4] = {};
+    float c[2][NT][4];
 #pragma unroll
-    for (int h = 0; h < 4; h += 2)
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
+      for (int j = 0; j < NT; ++j) mma_16816_first(c[b][j], u[b][0], v[b][0], u[b][1], v[b][1], x[b0 + b][j].x, x[b0 + b][j].y);
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
-          mma_16816(c[b][j], u[b][h], v[b][h], u[b][h + 1], v[b][h + 1], h ? x[b0 + b][j].z : x[b0 + b][j].x, h ? x[b0 + b][j].w : x[b0 + b][j].y);
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) mma_16816(c[b][j], u[b][2], v[b][2], u[b][3], v[b][3], x[b0 + b][j].z, x[b0 + b][j].w);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float f_lo = scale32(s_lo, b0 + b), f_hi = scale32(s_hi, b0 + b);
@@ -111,7 +118,8 @@ struct Items {
   float weight[MAX_PAIRS];
 };
 
-// All of the CTA's threads; ends with a barrier. `mine`: with up to 32 pairs, the id of pair `lane` in the first copying warp. An id that names no expert is recorded in `status` and its pair counts for nothing.
+// All of the CTA's threads; ends with a barrier. `mine`: with up to 32 pairs, the id of pair `lane` in the first copying warp. An id that names no
+// expert is recorded in `status` and its pair counts for nothing.
 __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids, int mine, int pairs, int top, int experts, int* status) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (pairs <= 32) {
@@ -290,7 +298,8 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   for (int m = threadIdx.x; m < p.M; m += THREADS) tops[m] = 0u;
   __syncthreads();
   if constexpr (KIND == FIRST)
-    for (int i = threadIdx.x - (WARPS + GROUPS) * 32; i >= 0 && i < p.rows * p.top; i += GROUPS * 32) reinterpret_cast<Items*>(&place)->weight[i] = p.wts[i];
+    for (int i = threadIdx.x - (WARPS + GROUPS) * 32; i >= 0 && i < p.rows * p.top; i += GROUPS * 32)
+      reinterpret_cast<Items*>(&place)->weight[i] = p.wts[i];
   if (KIND != SECOND && warp < WARPS) {
     for (int done = 0; done < all_pieces; done += ROUND * WARPS) {
       if (done) load_round();

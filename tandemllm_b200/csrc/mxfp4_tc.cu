@@ -146,8 +146,8 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&v)
       "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]),
       "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
       : "memory");
-  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
+__device__ __forceinline__ void tmem_stored() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 __device__ __forceinline__ void tmem_load16(uint32_t taddr, float (&v)[16]) {
   uint32_t r[16];
@@ -183,8 +183,7 @@ struct RowTile {
   uint4 c[4];
   uint32_t s;
 };
-__device__ __forceinline__ void load_row_tile(RowTile& q, const uint8_t* codes, const uint8_t* scales, int tile, bool valid) {
-  const uint8_t* from = codes + (long long)tile * TILE_CODES;
+__device__ __forceinline__ void load_row_tile(RowTile& q, const uint8_t* codes, const uint8_t* scales, bool valid) {
 #pragma unroll
   for (int t = 0; t < 4; ++t)
     asm volatile(
@@ -192,9 +191,29 @@ __device__ __forceinline__ void load_row_tile(RowTile& q, const uint8_t* codes, 
         "setp.ne.b32 ok, %5, 0;\n\t"
         "mov.b32 %0, 0;\n\tmov.b32 %1, 0;\n\tmov.b32 %2, 0;\n\tmov.b32 %3, 0;\n\t"
         "@ok ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];\n\t}"
-        : "=r"(q.c[t].x), "=r"(q.c[t].y), "=r"(q.c[t].z), "=r"(q.c[t].w) : "l"(from + t * 16), "r"((int)valid));
+        : "=r"(q.c[t].x), "=r"(q.c[t].y), "=r"(q.c[t].z), "=r"(q.c[t].w) : "l"(codes + t * 16), "r"((int)valid));
   asm volatile("{\n\t.reg .pred ok;\n\tsetp.ne.b32 ok, %2, 0;\n\tmov.b32 %0, 0;\n\t@ok ld.global.nc.u32 %0, [%1];\n\t}"
-               : "=r"(q.s) : "l"(scales + (long long)tile * TILE_SCALES), "r"((int)valid));
+               : "=r"(q.s) : "l"(scales), "r"((int)valid));
+}
+
+// Copies to shared memory that the thread waits for itself; zeros where there is nothing.
+__device__ __forceinline__ void copy_16(uint32_t to, const void* from, bool there) {
+  asm volatile("{\n\t.reg .pred no;\n\tsetp.eq.b32 no, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, no;\n\t}"
+               ::"r"(to), "l"(from), "r"((int)there) : "memory");
+}
+__device__ __forceinline__ void copy_4(uint32_t to, const void* from, bool there) {
+  asm volatile("{\n\t.reg .pred no;\n\tsetp.eq.b32 no, %2, 0;\n\tcp.async.ca.shared.global [%0], [%1], 4, no;\n\t}"
+               ::"r"(to), "l"(from), "r"((int)there) : "memory");
+}
+__device__ __forceinline__ uint4 load_shared16(uint32_t from) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t load_shared4(uint32_t from) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(from) : "memory");
+  return v;
 }
 
 // The values of the tile's first or second 64 k, two a register.
@@ -225,16 +244,23 @@ __device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
 
 // A tile's values to a stage of tensor memory, once the products of the tile that had it (`before`; negative: none) are done; `then` runs when
 // the tile's codes are used up. False where the wait ran out or somebody gave up.
+__device__ __forceinline__ void tma_load_if(bool one, void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "@p cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
+      ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"((int)one) : "memory");
+}
 template <typename Then>
-__device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* done, int before, volatile uint32_t* aborted, Then then) {
+__device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* done, int before, volatile uint32_t* aborted,
+                                          Then then) {
   uint32_t v[32];
   convert<0>(q, v);
   if (!__all_sync(0xffffffffu, wait_nth(done, before) && *aborted == 0)) return false;
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   tmem_store32(taddr, v);
   convert<1>(q, v);
-  then();
   tmem_store32(taddr + KB / 2, v);
+  then();
+  tmem_stored();
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncwarp();
   if ((threadIdx.x & 31) == 0) mbar_arrive(full);
@@ -375,7 +401,8 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     constexpr int AHEAD = 2;                                    // tiles of codes a thread has at hand or on their way
     RowTile q[AHEAD];
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) load_row_tile(q[u], codes, scales, half + 2 * u, valid && half + 2 * u < tiles);
+    for (int u = 0; u < AHEAD; ++u)
+      load_row_tile(q[u], codes + (half + 2 * u) * TILE_CODES, scales + (half + 2 * u) * TILE_SCALES, valid && half + 2 * u < tiles);
     bool ok = true;
     for (int c0 = half; c0 < tiles && ok; c0 += 2 * AHEAD) {
 #pragma unroll
@@ -383,7 +410,8 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
         const int c = c0 + 2 * u;
         if (c < tiles && ok) {
           ok = give_tile(t_lane + BN + half * S::A_COLS, q[u], &full[c % SLOTS], done, c - S::A_STAGES, aborted, [&]() {
-            load_row_tile(q[u], codes, scales, c + 2 * AHEAD, valid && c + 2 * AHEAD < tiles);
+            const int after = c + 2 * AHEAD;
+            load_row_tile(q[u], codes + (long long)after * TILE_CODES, scales + (long long)after * TILE_SCALES, valid && after < tiles);
           });
           if (!ok && lane == 0) give_up();
         }
@@ -485,27 +513,36 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that a k-block's conversion (240
-// cycles) hides under its products (2 cycles a token row). Tensor memory holds two accumulators of 160 columns and three stages of weights, or one
-// of 256 and four where that saves a round, or (few rows an expert) two of 64 and six: the way of a stage, from its values to its products' end and
-// back, takes some 2000 cycles, of which every stage more hides a part (two stages beside two accumulators of 192: 103 us where these take XX).
-// Eight warps of their own finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up
-// to 16, and they come in boxes of 256, 80 or 16.
+// The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that the conversion of a tile of
+// weights (480 cycles of a scheduler's integer pipe) hides under its products (4 cycles a token row). Tensor memory holds two accumulators of 160
+// columns and three stages of weights, or one of 256 and four where that saves a round, or (few rows an expert) two of 64 and six: the way of a stage,
+// from its values to its products' end and back, takes some 2000 cycles, of which every stage more hides a part (2048 rows, 7168 gated outputs of
+// 2048: 103 us with two stages beside two accumulators of 192, 99 with these). Eight warps of their own finish a tile while the next one's products
+// run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of 256, 80 or 16.
+//
+// With few rows an expert the converting warps are what takes longest: twelve of them (a layer of 64 experts with 4 rows each, 768 by 2048: 87 us
+// with eight, 76 with twelve, 74 with sixteen, which leaves four to finish and costs a product of 150 rows 2 of its 11 us).
 template <int MAXN>
 struct Many {
   static constexpr int BOX_ROWS = MAXN > 160 ? 256 : MAXN > 64 ? 80 : 16;      // token rows a TMA box
   static constexpr int BOX_BYTES = BOX_ROWS * KB * 2;
   static constexpr int HALF_BYTES = MAXN * KB * 2;
   static constexpr int B_BYTES = 2 * HALF_BYTES;                 // a stage of token rows: a tile of 128 k, its two k-blocks one after the other
-  static constexpr int B_STAGES = MAXN > 160 ? 3 : MAXN > 64 ? 5 : 8;
+  static constexpr int B_STAGES = MAXN > 160 ? 3 : MAXN > 64 ? 4 : 5;
   static constexpr int A_COLS = TILE_K / 2;                      // a stage of weights: a tile of 128 k
   static constexpr int A_STAGES = MAXN > 160 ? 4 : MAXN > 64 ? 3 : 6;
   static constexpr int ACCS = MAXN > 160 ? 1 : 2;
   static constexpr int A_AT = 512 - A_STAGES * A_COLS;           // the accumulators come first
-  static constexpr int CONVERT_WARPS = 8;
+  static constexpr int CONVERT_WARPS = MAXN > 64 ? 8 : 12;
   static constexpr int FINISH_WARPS = 8;
+  static constexpr int GROUPS = CONVERT_WARPS / 4;
   static constexpr int THREADS = (2 + CONVERT_WARPS + FINISH_WARPS) * 32;
-  static constexpr int TOTAL = B_STAGES * B_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+  // Tiles of codes that a converting warp has on their way to its part of shared memory (more than two or three gain nothing); 0: two in registers,
+  // where the token rows leave no room. Through shared memory a warp's copies are whole lines: 768 rows to 32 experts 133 -> 122 us.
+  static constexpr int AHEAD = MAXN > 160 ? 0 : 3;
+  static constexpr int SLOT_BYTES = 4 * (TILE_CODES + TILE_SCALES);
+  static constexpr int TOTAL = B_STAGES * B_BYTES + CONVERT_WARPS * AHEAD * SLOT_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
+  static_assert(TOTAL <= 227 * 1024, "a CTA's shared memory");
   static_assert(ACCS * MAXN <= A_AT, "accumulators and weights share tensor memory");
   static_assert(BOX_BYTES % 1024 == 0, "a box begins where the swizzle does");
   static_assert(A_STAGES <= SLOTS && B_STAGES <= SLOTS, "see SLOTS");
@@ -529,7 +566,8 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   chain_wait();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-  uint64_t* full = (uint64_t*)(boxes + S::B_STAGES * S::B_BYTES);
+  uint8_t* slots = boxes + S::B_STAGES * S::B_BYTES;
+  uint64_t* full = (uint64_t*)(slots + S::CONVERT_WARPS * S::AHEAD * S::SLOT_BYTES);
   uint64_t* done = full + SLOTS;
   uint64_t* acc_full = done + SLOTS;
   uint64_t* acc_empty = acc_full + 2;
@@ -565,11 +603,19 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   const int k_tiles = ceil_div(p.K, TILE_K), num_kb = ceil_div(p.K, KB), row_tiles = ceil_div(p.N, TILE_ROWS);
   const int tiles_n = ceil_div(p.N, OUTS), tiles_m = p.tile_group ? *p.n_tiles : ceil_div(p.M, tile_at_most);
   const int work = tiles_n * tiles_m;
-  // work item w: token tile w / tiles_n, weight tile w % tiles_n (neighbouring CTAs share token rows)
-  auto tokens_of = [&](int w, int& tok0, int& tok_rows) {
-    const int tm = w / tiles_n;
-    tok0 = p.tile_group ? p.tile_row0[tm] : tm * tile_at_most;
-    tok_rows = p.tile_group ? min(p.tile_rows[tm], MAXN) : min(tile_at_most, p.M - tok0);
+  // work item w: token tile w / tiles_n, weight tile w % tiles_n (neighbouring CTAs share token rows). What is to be known of the next item is
+  // read while this one is at work: a read's 700 cycles an item would be as long as one or two of its tiles.
+  struct Tokens {
+    int first, rows;
+  };
+  auto tokens_of = [&](int w) {
+    Tokens t = {0, 0};
+    if (w < work) {
+      const int tm = w / tiles_n;
+      t.first = p.tile_group ? p.tile_row0[tm] : tm * tile_at_most;
+      t.rows = p.tile_group ? p.tile_rows[tm] : min(tile_at_most, p.M - t.first);
+    }
+    return t;
   };
 
   if (warp == 0) {
@@ -577,9 +623,10 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     Ring<S::B_STAGES> ring;
     int issued = 0;
     bool ok = true;
+    Tokens coming = tokens_of(blockIdx.x);
     for (int w = blockIdx.x; w < work && ok; w += gridDim.x) {
-      int tok0, tok_rows;
-      tokens_of(w, tok0, tok_rows);
+      const int tok0 = coming.first, tok_rows = min(coming.rows, MAXN);
+      coming = tokens_of(w + gridDim.x);
       const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
       for (int c = 0; c < k_tiles; ++c, ring.next()) {
         if (!__all_sync(0xffffffffu, wait_nth(done, issued - S::B_STAGES) && *aborted == 0)) {
@@ -588,12 +635,13 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
           break;
         }
         const int blocks = min(2, num_kb - 2 * c);
-        if (elected()) {
-          uint64_t* bar = &full[issued % SLOTS];
-          mbar_expect_tx(bar, blocks * boxes_here * S::BOX_BYTES);
-          for (int i = 0; i < blocks; ++i)
-            for (int b = 0; b < boxes_here; ++b)
-              tma_load_2d(boxes + ring.stage * S::B_BYTES + i * S::HALF_BYTES + b * S::BOX_BYTES, &tmX, bar, (2 * c + i) * KB, tok0 + b * S::BOX_ROWS);
+        const bool one = elected();
+        uint64_t* bar = &full[issued % SLOTS];
+        uint8_t* at = boxes + ring.stage * S::B_BYTES;
+        if (one) mbar_expect_tx(bar, blocks * boxes_here * S::BOX_BYTES);
+        for (int b = 0; b < boxes_here; ++b) {
+          tma_load_if(one, at + b * S::BOX_BYTES, &tmX, bar, 2 * c * KB, tok0 + b * S::BOX_ROWS);
+          if (blocks == 2) tma_load_if(one, at + S::HALF_BYTES + b * S::BOX_BYTES, &tmX, bar, 2 * c * KB + KB, tok0 + b * S::BOX_ROWS);
         }
         __syncwarp();
         ++issued;
@@ -608,9 +656,10 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     Ring<S::ACCS> rd;
     int tile = 0, items = 0;
     bool ok = true, there = false;
+    Tokens coming = tokens_of(blockIdx.x);
     for (int w = blockIdx.x; w < work && ok; w += gridDim.x, rd.next()) {
-      int tok0, tok_rows;
-      tokens_of(w, tok0, tok_rows);
+      const int tok_rows = min(coming.rows, MAXN);
+      coming = tokens_of(w + gridDim.x);
       const uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(ceil_div(tok_rows, 16) * 2) << 17) | ((uint32_t)(ROWS >> 4) << 24);
       if (!__all_sync(0xffffffffu, (items < S::ACCS || wait_for(&acc_empty[rd.stage], (items / S::ACCS - 1) & 1)) && *aborted == 0)) {
         give_up();
@@ -637,76 +686,111 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     // the last products have left tensor memory and shared memory before anybody frees them
     if (items > 0) mbar_wait(&acc_full[(items - 1) % S::ACCS], ((items - 1) / S::ACCS) & 1);
   } else if (warp < 2 + S::CONVERT_WARPS) {
-    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
-    const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane, eight = r >> 3;
+    // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, every GROUPS-th tile of 128 k ----
+    const int turn = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t t_lane = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + S::A_AT;
-    // where a thread is: the work item, the tile of 128 k, and its row's first tile
+    // The warp's 32 rows are four tiles of 8 rows: two and two, or gated two of the gate and two of the up matrix in turn.
+    const int eight0 = (warp & 3) * 4, eight = r >> 3;
+    auto row_tile_of = [&](int n0, int e) { return (n0 >> 3) + (GATED ? e >> 1 : e); };
+    const long long line = (long long)k_tiles * TILE_CODES, matrix_bytes = row_tiles * line;
+    // where a thread is: the work item, the tile of 128 k, and that tile of its row (AHEAD: its 16 bytes of the warp's first row tile)
     struct Cursor {
-      int w, c;
+      int w, c, row_tile, group;                                // (the group: the next item's)
       const uint8_t* codes;
       const uint8_t* scales;
-      bool valid;
     };
+    auto group_of = [&](int w) { return p.tile_group && w < work ? p.tile_group[w / tiles_n] : 0; };
     auto enter = [&](Cursor& q, int w) {
       q.w = w;
-      q.c = half;
-      q.valid = false;
+      q.c = turn;
+      q.row_tile = row_tiles;
       q.codes = p.codes, q.scales = p.scales;
-      if (w >= work || half >= k_tiles) return;
-      const int tm = w / tiles_n, n0 = (w - tm * tiles_n) * OUTS, group = p.tile_group ? p.tile_group[tm] : 0;
-      const int row_tile = (n0 >> 3) + (GATED ? eight >> 1 : eight);
-      q.valid = row_tile < row_tiles;
-      const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (q.valid ? row_tile : 0)) * k_tiles;
-      q.codes = p.codes + first * TILE_CODES + (r & 7) * (TILE_K / 2);
-      q.scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
+      if (w >= work || turn >= k_tiles) return;
+      const int n0 = w % tiles_n * OUTS, group = q.group;
+      q.group = group_of(w + gridDim.x);
+      const int mine = row_tile_of(n0, eight), first = row_tile_of(n0, eight0);
+      q.row_tile = S::AHEAD ? first : mine;
+      const long long matrix = (long long)group * p.matrices * row_tiles;
+      const long long own = (matrix + (GATED ? (long long)(eight & 1) * row_tiles : 0) + min(mine, row_tiles - 1)) * k_tiles;
+      q.codes = S::AHEAD ? p.codes + (matrix + min(first, row_tiles - 1)) * k_tiles * TILE_CODES + lane * 16
+                         : p.codes + own * TILE_CODES + (r & 7) * (TILE_K / 2);
+      q.scales = p.scales + own * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
+      q.codes += turn * TILE_CODES, q.scales += turn * TILE_SCALES;
     };
     auto advance = [&](Cursor& q) {
-      q.c += 2;
+      q.c += S::GROUPS, q.codes += S::GROUPS * TILE_CODES, q.scales += S::GROUPS * TILE_SCALES;
       if (q.c >= k_tiles) enter(q, q.w + gridDim.x);
     };
-    constexpr int AHEAD = 2;
-    RowTile q[AHEAD];
+    constexpr int BUFFERS = S::AHEAD ? 1 : 2;
+    RowTile q[BUFFERS];
     Cursor next, now;
+    next.group = group_of(blockIdx.x);
     enter(next, blockIdx.x);
     now = next;
+    // A slot is four tiles' codes and their rows' scales. A row's 16 bytes of quarter t lie at t ^ (row / 2 % 4), so that both the copies (a lane
+    // 16 bytes of a tile) and the reads (a lane a row) fall on all banks.
+    const uint32_t my_slots = smem_u32(slots + (warp - 2) * (S::AHEAD * S::SLOT_BYTES));
+    const uint32_t put = (lane >> 2) * 64 + (((lane & 3) ^ ((lane >> 3) & 3)) << 4);
+    const uint32_t take = (lane >> 3) * TILE_CODES + (lane & 7) * 64, turned = ((lane & 7) >> 1) << 4;
+    int to = 0, from = 0;                                       // slots' offsets
+    auto fetch = [&](RowTile& q) {                              // the tile at `next`, on its way
+      if constexpr (S::AHEAD > 0) {
+        __syncwarp();                                           // (all lanes have read what the slot held)
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
+        for (int j = 0; j < 4; ++j)
+          copy_16(my_slots + to + j * TILE_CODES + put, next.codes + (GATED ? (j & 1) * matrix_bytes + (j >> 1) * line : j * line),
+                  next.row_tile + (GATED ? j >> 1 : j) < row_tiles);
+        copy_4(my_slots + to + 4 * TILE_CODES + lane * 4, next.scales, next.row_tile + (GATED ? lane >> 4 : lane >> 3) < row_tiles);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        to = to + S::SLOT_BYTES == S::AHEAD * S::SLOT_BYTES ? 0 : to + S::SLOT_BYTES;
+      } else {
+        load_row_tile(q, next.codes, next.scales, next.row_tile < row_tiles);
+      }
       advance(next);
-    }
-    // The tiles of all of the CTA's work items are one sequence; this group's are those of its parity in an item, so the stage of one is its place
-    // in the sequence, and how often the stage was used before it that place's round.
-    int at = half;                                              // the place of the tile at hand
-    bool ok = true;
-    while (ok && now.w < work && half < k_tiles) {
+    };
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
+    for (int u = 0; u < (S::AHEAD ? S::AHEAD : BUFFERS); ++u) fetch(q[u % BUFFERS]);
+    // The tiles of all of the CTA's work items are one sequence; this group's are every GROUPS-th of an item, so the stage of one is its place
+    // in the sequence, and how often the stage was used before it that place's round.
+    int at = turn;                                              // the place of the tile at hand
+    bool ok = true;
+    while (ok && now.w < work && turn < k_tiles) {
+#pragma unroll
+      for (int u = 0; u < BUFFERS; ++u) {
         if (!ok || now.w >= work) break;
+        if constexpr (S::AHEAD > 0) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(S::AHEAD > 0 ? S::AHEAD - 1 : 0) : "memory");
+          __syncwarp();
+#pragma unroll
+          for (int t = 0; t < 4; ++t) q[u].c[t] = load_shared16(my_slots + from + take + ((t << 4) ^ turned));
+          q[u].s = load_shared4(my_slots + from + 4 * TILE_CODES + lane * 4);
+          from = from + S::SLOT_BYTES == S::AHEAD * S::SLOT_BYTES ? 0 : from + S::SLOT_BYTES;
+        }
         const int stage = at % S::A_STAGES;
-        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &full[at % SLOTS], done, at - S::A_STAGES, aborted, [&]() {
-          load_row_tile(q[u], next.codes, next.scales, next.c, next.valid && next.w < work);
-        });
+        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &full[at % SLOTS], done, at - S::A_STAGES, aborted, [&]() { fetch(q[u]); });
         if (!ok && lane == 0) give_up();
-        advance(next);
         const int before = now.c;
-        now.c += 2;
+        now.c += S::GROUPS;
         if (now.c >= k_tiles) {
-          now.c = half, now.w += gridDim.x;
-          at += k_tiles - before + half;
+          now.c = turn, now.w += gridDim.x;
+          at += k_tiles - before + turn;
         } else {
-          at += 2;
+          at += S::GROUPS;
         }
       }
     }
+    // (also where it gave up: nothing may arrive in shared memory that is another CTA's by then)
+    if constexpr (S::AHEAD > 0) asm volatile("cp.async.wait_all;" ::: "memory");
   } else {
     // ---- results: accumulator rows 32 (warp % 4) .. + 31 ----
     const int r = (warp & 3) * 32 + lane, eight = r >> 3;
     const bool up = GATED && (eight & 1);
-    const int other = (warp - 2 - S::CONVERT_WARPS) >> 2;       // two warps a quarter of the rows, every other 16 columns each
+    const int other = (warp - 2 - S::CONVERT_WARPS) >> 2;       // of the warps of a quarter of the rows, which take 16 columns in turn
     int nth = 0;
+    Tokens coming = tokens_of(blockIdx.x);
     for (int w = blockIdx.x; w < work; w += gridDim.x, ++nth) {
-      int tok0, tok_rows;
-      tokens_of(w, tok0, tok_rows);
+      const int tok0 = coming.first, tok_rows = min(coming.rows, MAXN);
+      coming = tokens_of(w + gridDim.x);
       const int acc = nth % S::ACCS, n = (w % tiles_n) * OUTS + (GATED ? (r >> 4) * 8 + (r & 7) : r);
       const bool mine = n < p.N;
       const float bias = p.bias && mine ? p.bias[up ? p.N + n : n] : 0.f;
@@ -718,7 +802,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       const uint32_t from = tmem_base + ((uint32_t)((warp & 3) * 32) << 16) + acc * MAXN;
       TOut* C = (TOut*)p.C;
 #pragma unroll 1
-      for (int c0 = other * 16; c0 < tok_rows; c0 += 32) {
+      for (int c0 = other * 16; c0 < tok_rows; c0 += S::FINISH_WARPS * 4) {
         float v[16];
         tmem_load16(from + c0, v);
         const int left = tok_rows - c0;
@@ -854,7 +938,8 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     const long long work = (long long)ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS) * (tile_group ? max_tiles : ceil_div(M, bn));
     TL_REQUIRE(work <= 0x7FFFFFFF, "mxfp4 product: %lld tiles are too many", work);
     CUtensorMap tmX;
-    const int r = tensor_map(x, x_rows, K, ldx, bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 160 ? mx::Many<160>::BOX_ROWS : mx::Many<256>::BOX_ROWS, &tmX);
+    const int box = bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 160 ? mx::Many<160>::BOX_ROWS : mx::Many<256>::BOX_ROWS;
+    const int r = tensor_map(x, x_rows, K, ldx, box, &tmX);
     if (r) return r;
 #define TL_MX_MANY(N_)                                                                                \
   do {                                                                                                \

@@ -50,7 +50,8 @@ class KernelFault(RuntimeError):
 
 _STATUS = {1: "a token id outside the vocabulary", 2: "a key/value write to a position without a page",
            3: "a visible key without a page", 4: "an attention tile with more rows than its kernel takes",
-           5: "a plan tile with more rows than its kernel takes", 6: "a row routed to an expert that does not exist", 11: "a pipeline wait that ran out in a tensor-core kernel"}
+           5: "a plan tile with more rows than its kernel takes", 6: "a row routed to an expert that does not exist",
+           11: "a pipeline wait that ran out in a tensor-core kernel"}
 
 CONTEXT_BUCKET = 1024       # the smallest context bucket of a decode graph
 

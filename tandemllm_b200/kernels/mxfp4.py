@@ -181,16 +181,16 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
 
     The form with the smallest estimated time, in us: `blocks` (of 128 k) one after the other in every round of CTAs, each as long as its
     weights take to convert or, persistent, as its tokens take to multiply; a round's start and end; and, where CTAs share a tile's k, adding
-    their sums. The numbers are fitted to 1600 timings of 8 products with 17 to 4096 rows; over these the choice is 1.7 % slower than the
-    fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14.3 us in one persistent tile, 18.7 where two CTAs share
-    its k; 2048 rows 100 in tiles of 160, 107 in tiles of 192. At 2048 outputs of 7168: 256 rows 17.3 with eight CTAs a tile, 28 without;
-    700 rows 32 without, 43 with eight (and two rounds)."""
+    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 2 % slower than the
+    fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 15 us in one persistent tile, 19 where two CTAs share
+    its k; 2048 rows 99 in tiles of 160, 107 in tiles of 192. At 2048 outputs of 7168: 256 rows 17 with eight CTAs a tile, 31 without;
+    700 rows 32 without, 36 with two."""
     blocks = -(-k // TILE_K)
     best = None
     for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
         rounds = -(-row_tiles * -(-rows // h) // sms)
-        alone = 0.004 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
-        cost = 3.4 + rounds * (blocks * max(0.52, 0.0025 * h) + 0.96 + alone) + 0.0145 * h
+        alone = 0.011 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
+        cost = 4.4 + rounds * (blocks * max(0.51 if h > 64 else 0.44, 0.0022 * h) + 0.96 + alone) + 0.0068 * h
         if best is None or cost < best[0]:
             best = cost, h, 0
     for bn in (16, 32, 64, 128):
@@ -202,8 +202,8 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
                 break
             rounds, rest = divmod(ctas, 2 * sms)                        # two CTAs an SM; one alone is faster
             rounds += 0.0 if rest == 0 else 0.56 if rest <= sms else 1.0
-            cost = 4.4 + rounds * (-(-blocks // splits) * (0.735 + 0.0012 * bn) * (1.14 if gated else 1.0) + 0.31) + 0.0134 * bn
-            cost += 1.0 + 0.026 * bn if splits > 1 else 0.0
+            cost = 4.3 + rounds * (-(-blocks // splits) * (0.7 + 0.0014 * bn) * (1.17 if gated else 1.0) + 0.48) + 0.0123 * bn
+            cost += 1.0 + 0.027 * bn if splits > 1 else 0.0
             if cost < best[0]:
                 best = cost, bn, splits
     return best[1:]
@@ -268,7 +268,7 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
     down( act(gate x) * (up x) ); or [E, inter, hidden] without gates: down( act(up x) ). `weigh` "input": the weight multiplies what the
     first product makes of x, in front of the activation, and the experts' rows are added as they are. An id outside 0 .. E - 1 adds
     nothing and is recorded in the runtime's status word. With `defer` the result of many rows is an `ops.ExpertRows`, whose consumer
-    weighs and adds the experts' rows itself."""
+    weighs and adds the experts' rows itself; every id has to be an expert's then."""
     E = w_down.groups
     gates = w_first.groups // max(E, 1)
     if gates not in (1, 2) or w_first.groups != gates * E or w_first.n != w_down.k or w_first.k != w_down.n or w_first.index != w_down.index:
@@ -277,7 +277,8 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
         raise ops.KernelError(f"experts weighed at their {weigh!r}: input or output")
     rows, ld = _rows(x, w_first)
     if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != rows or ids.get_device() != w_down.index or not ids.is_contiguous():
-        raise ops.KernelError(f"mxfp4 experts: ids {ids.dtype} {tuple(ids.shape)} on {ids.device}; contiguous int32 [{rows}, top] on {x.device} is wanted")
+        raise ops.KernelError(f"mxfp4 experts: ids {ids.dtype} {tuple(ids.shape)} on {ids.device}; contiguous int32 [{rows}, top] on {x.device} is "
+                              "wanted")
     top = ids.shape[1]
     w = _vector(wts, rows * top, "the experts' weights", w_down.index)
     if not 1 <= top <= EXPERT_TOP or not 1 <= E <= 1024:
@@ -296,8 +297,8 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_f
     out = x.new_empty(rows, w_down.n, dtype=dtype)
     E, inter, status, stream = w_down.groups, w_down.k, runtime.status.data_ptr(), ops.stream()
     between = x.new_empty(lib().tl_mxfp4_experts_between(rows * top, inter), dtype=torch.uint8)
-    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, between.data_ptr(), rows, inter, w_first.k, ids.data_ptr(), w,
-                                        int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
+    _check(lib().tl_mxfp4_experts_first(x.data_ptr(), ld, w_first.codes, w_first.scales, between.data_ptr(), rows, inter, w_first.k,
+                                        ids.data_ptr(), w, int(before), top, E, act, *constants, status, stream), "mxfp4_experts_first")
     _check(lib().tl_mxfp4_experts_second(between.data_ptr(), w_down.codes, w_down.scales, out.data_ptr(), w_down.n, rows, w_down.n, inter,
                                          ids.data_ptr(), top, E, act, ops.dtype_code(dtype), status, stream), "mxfp4_experts_second")
     return out
