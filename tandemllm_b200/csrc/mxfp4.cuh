@@ -31,13 +31,15 @@ __device__ __forceinline__ uint32_t factor(uint32_t s) { return (min(s, 128u) + 
 __device__ __forceinline__ uint32_t factor_left(uint32_t s) {
   return s <= 128u ? 0x3F803F80u : s == 255u ? 0x7FFF7FFFu : (s - 1u) * 0x00800080u;
 }
-// The four pairs of a word, times `f`: pair j is values 2 j (lower half) and 2 j + 1.
+// The four pairs of a word, times `f`: pair j is values 2 j (lower half) and 2 j + 1. A pair alone in its word times two powers of two is its sign at a
+// half's top and its other bits at their place, beside copies that the mask takes away: a multiplication, which another pipe than the logic does.
 __device__ __forceinline__ void values(uint32_t w, uint32_t f, uint32_t (&v)[4]) {
   constexpr uint32_t SIGN = 0x80008000u, REST = 0x01C001C0u;
-  v[0] = mul2(((w << 12) & SIGN) | ((w << 6) & REST), f);
-  v[1] = mul2(((w << 8) & SIGN) | ((w << 2) & REST), f);
-  v[2] = mul2(((w << 4) & SIGN) | ((w >> 2) & REST), f);
-  v[3] = mul2((w & SIGN) | ((w >> 6) & REST), f);
+  const uint32_t y = w >> 6;
+  v[0] = mul2((w & 0x000F000Fu) * (4096u + 64u) & (SIGN | REST), f);
+  v[1] = mul2((w & 0x00F000F0u) * (256u + 4u) & (SIGN | REST), f);
+  v[2] = mul2((y & 0x003C003Cu) * (1024u + 16u) & (SIGN | REST), f);
+  v[3] = mul2((w & SIGN) | (y & REST), f);
 }
 
 // As float16 numbers without their scale, pairs as the conversion finds them in the word's bytes: values (0, 2), (4, 6), (1, 3), (5, 7).

@@ -12,8 +12,8 @@
 //   warp 1       one thread issues the MMAs (kind::f16, A in tensor memory, B in shared memory) and releases both operands' stages
 //   warps 2..9   two groups of four that take every other tile of 128 k of the weights; then the epilogue, each group every other 16 columns
 //
-// An MMA of 128 x 128 x 64 takes 256 cycles of the tensor pipe and its weights 134 issue cycles of each scheduler, so with tiles of 128
-// token rows the conversion runs under the products; two CTAs an SM run under each other's ends.
+// The products of a tile of 128 k with 128 token rows take 512 cycles of the tensor pipe and its weights' conversion 290 of each scheduler's integer
+// pipe (nine operations a word, at half rate), so with as many rows the conversion runs under the products; two CTAs an SM run under each other's ends.
 //
 // SPLIT: a cluster of CTAs shares a tile, each with a run of k; each leaves its accumulator in its shared memory, the cluster meets, and
 // every CTA adds the sums of some of the tokens in rank order and stores them, so the result does not depend on timing.
@@ -514,14 +514,16 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 
 // ---------------------------------------------------------------------------------------------------------------
 // The same for prompts and routed experts: a persistent CTA an SM, whose token tiles are up to MAXN rows high, so that the conversion of a tile of
-// weights (480 cycles of a scheduler's integer pipe) hides under its products (4 cycles a token row). Tensor memory holds two accumulators of 160
-// columns and three stages of weights, or one of 256 and four where that saves a round, or (few rows an expert) two of 64 and six: the way of a stage,
-// from its values to its products' end and back, takes some 2000 cycles, of which every stage more hides a part (2048 rows, 7168 gated outputs of
-// 2048: 103 us with two stages beside two accumulators of 192, 99 with these). Eight warps of their own finish a tile while the next one's products
-// run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in boxes of 256, 80 or 16.
+// weights hides under its products (4 cycles a token row; both with what they wait for: 0.45 us a tile up to 200 rows). Tensor memory holds two
+// accumulators of 160 columns and three stages of weights, or one of 256 and four where that saves a round, or (few rows an expert) two of 64 and
+// six: the way of a stage, from its values to its products' end and back, takes some 2000 cycles, of which every stage more hides a part (2048
+// rows, 7168 gated outputs of 2048: 103 us with two stages beside two accumulators of 192 where these took 99; 92 since). Eight warps of their own
+// finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in
+// boxes of 256, 80 or 16.
 //
 // With few rows an expert the converting warps are what takes longest: twelve of them (a layer of 64 experts with 4 rows each, 768 by 2048: 87 us
-// with eight, 76 with twelve, 74 with sixteen, which leaves four to finish and costs a product of 150 rows 2 of its 11 us).
+// with eight, 76 with twelve, 74 with sixteen, which leaves four to finish and costs a product of 150 rows 2 of its 11 us; 73 with the sign and the
+// rest of a pair put in place by one multiplication, which took 5 to 10 % off all of these products).
 template <int MAXN>
 struct Many {
   static constexpr int BOX_ROWS = MAXN > 160 ? 256 : MAXN > 64 ? 80 : 16;      // token rows a TMA box
