@@ -131,14 +131,16 @@ def quantize(w: torch.Tensor) -> Mxfp4Matrix:
     return m
 
 
-def _rows(x: torch.Tensor, w: Mxfp4Matrix) -> tuple[int, int]:
-    """(rows, elements from one to the next) of x, which has to be what the products take."""
+def _rows(runtime, x: torch.Tensor, w: Mxfp4Matrix) -> tuple[int, int]:
+    """(rows, elements from one to the next) of x, which has to be what the products take; the runtime's status word is where x is."""
     if x.dim() != 2 or x.shape[1] != w.k:
         raise ops.KernelError(f"mxfp4 product: rows of shape {tuple(x.shape)} with a matrix of shape {w.shape}")
     if x.dtype is not torch.bfloat16:
         raise ops.KernelError(f"mxfp4 product: rows of {x.dtype}; bfloat16 is implemented")
     if _here(x, "x") != w.index:
         raise ops.KernelError(f"mxfp4 product: rows on {x.device}, the matrix on {w.device}")
+    if runtime.status is None or runtime.status.get_device() != w.index:
+        raise ops.KernelError(f"mxfp4 product: rows on {x.device}, the runtime on {runtime.device}")
     ld, inner = x.stride()
     if inner != 1 and w.k > 1:
         raise ops.KernelError(f"mxfp4 product: rows of {w.k} elements that lie {inner} apart; unit inner stride is implemented")
@@ -146,9 +148,10 @@ def _rows(x: torch.Tensor, w: Mxfp4Matrix) -> tuple[int, int]:
 
 
 def _boxed(x: torch.Tensor, rows: int, k: int, ld: int, order: int | None = None, div: int = 1) -> tuple[torch.Tensor, int]:
-    """(x, its row stride) for the tensor-core product: as it is where its rows begin at multiples of 16 bytes, else a copy that does. With
+    """(x, its row stride) for the tensor-core product: as it is where its rows lie behind one another from multiples of 16 bytes, else a copy
+    that does. With
     `order` (`rows` row numbers on the device, to be divided by `div`) a copy of these rows."""
-    if order is None and ld % 8 == 0 and x.data_ptr() % 16 == 0:
+    if order is None and ld % 8 == 0 and ld >= k and x.data_ptr() % 16 == 0:
         return x, ld
     wide = -(-k // 8) * 8
     copy = torch.empty(rows, wide, dtype=torch.bfloat16, device=x.device)
@@ -230,7 +233,7 @@ def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None =
     name or code; None: as it is), in `out_dtype` (default: `out`'s, else x's)."""
     if w.groups != 1:
         raise ops.KernelError(f"mxfp4 product: a stack of {w.groups} matrices where one is wanted")
-    rows, ld = _rows(x, w)
+    rows, ld = _rows(runtime, x, w)
     b = _vector(bias, w.n, "the bias", w.index)
     out = _output(out, rows, w.n, out_dtype or (out.dtype if out is not None else x.dtype), x)
     code = 0 if act is None else _gate(act)
@@ -253,7 +256,7 @@ def gated(runtime, x: torch.Tensor, w: Mxfp4Matrix, act: str | int = "silu", bia
     [2 n]). `act`: a gate of `ops.ACTIVATIONS`, by name or code; `constants`: those of one that has some."""
     if w.groups != 2:
         raise ops.KernelError(f"mxfp4 gated product: {w.groups} matrices where a gate and an up matrix are wanted")
-    rows, ld = _rows(x, w)
+    rows, ld = _rows(runtime, x, w)
     b = _vector(bias, 2 * w.n, "the bias", w.index)
     out = x.new_empty(rows, w.n)
     _product(runtime, x, rows, ld, w, b, out, _gate(act), constants)
@@ -275,7 +278,7 @@ def experts(runtime, x: torch.Tensor, ids: torch.Tensor, wts: torch.Tensor, w_fi
         raise ops.KernelError(f"mxfp4 experts: matrices of shapes {w_first.shape} on {w_first.device} and {w_down.shape} on {w_down.device}")
     if weigh not in ("input", "output"):
         raise ops.KernelError(f"experts weighed at their {weigh!r}: input or output")
-    rows, ld = _rows(x, w_first)
+    rows, ld = _rows(runtime, x, w_first)
     if ids.dtype is not torch.int32 or ids.dim() != 2 or ids.shape[0] != rows or ids.get_device() != w_down.index or not ids.is_contiguous():
         raise ops.KernelError(f"mxfp4 experts: ids {ids.dtype} {tuple(ids.shape)} on {ids.device}; contiguous int32 [{rows}, top] on {x.device} is "
                               "wanted")

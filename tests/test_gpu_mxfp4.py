@@ -147,6 +147,50 @@ def test_views_of_rows_and_outputs(runtime, m):
         assert (out == 7.0).all()
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu2", "identity"])
+@pytest.mark.parametrize("m", [1, 9, 40, 70, 300])
+def test_an_activation_behind_a_plain_product(runtime, m, act):
+    from tandemllm_b200.kernels import mxfp4
+    g = torch.Generator().manual_seed(m)
+    x, w, b = rows(g, m, 264), weights(g, 100, 264), torch.randn(100, generator=g)
+    want, off = P.product(x, P.rounded(w))
+    want = want + b.double()
+    want, off = P.activated(want, off + 2.0 ** -24 * want.abs(), act)
+    for out in DT.values():
+        P.hold(mxfp4.linear(runtime, x.to(DEV), mxfp4.quantize(w.to(DEV)), b.to(DEV), out_dtype=out, act=act), want, off)
+
+
+@pytest.fixture(scope="module")
+def many(runtime):
+    """Products with more tiles than SMs, of one to five tiles of k: (rows, matrices, their plain and gated products with bounds)."""
+    from tandemllm_b200.kernels import mxfp4
+    g, out = torch.Generator().manual_seed(5), []
+    for k in (100, 136, 264, 392, 520):
+        x, w = rows(g, 700, k), weights(g, 2, 3001, k)
+        v = P.rounded(w)
+        out.append((x.to(DEV), mxfp4.quantize(w[0].to(DEV)), mxfp4.quantize(w.to(DEV)), P.product(x, v[0]), P.gated(x, v[0], v[1], "silu")))
+    return out
+
+
+@pytest.mark.parametrize("form", [(h, 0) for h in (16, 48, 64, 80, 112, 144, 160, 176, 240, 256)] + [(b, s) for b in (16, 32, 64, 128) for s in (1, 2, 4, 8)])
+def test_every_form_of_the_tensor_core_product(runtime, many, form, monkeypatch):
+    from tandemllm_b200.kernels import mxfp4
+    for x, one, pair, plain, gated in many:
+        splits = min(form[1], -(-one.k // 128))
+        monkeypatch.setattr(mxfp4, "shape_of", lambda *a: (form[0], splits))
+        for out in DT.values():
+            P.hold(mxfp4.linear(runtime, x, one, out_dtype=out), *plain)
+        P.hold(mxfp4.gated(runtime, x, pair), *gated)
+
+
+@pytest.mark.parametrize("m", [1, 12, 40, 150])
+def test_one_row_seen_as_many(runtime, m):
+    from tandemllm_b200.kernels import mxfp4
+    g = torch.Generator().manual_seed(m)
+    x, w = rows(g, 1, 136), weights(g, 48, 136)
+    P.hold(mxfp4.linear(runtime, x.to(DEV).expand(m, 136), mxfp4.quantize(w.to(DEV))), *P.product(x.expand(m, 136), P.rounded(w)))
+
+
 # ---- routed experts ----
 
 def routed(g, m, e, top):
@@ -230,14 +274,59 @@ def test_results_repeat_bit_for_bit_and_do_not_depend_on_the_stream(runtime):
         assert all(torch.equal(once, t) for t in both)
 
 
+@pytest.mark.parametrize("weigh", ["input", "output"])
+@pytest.mark.parametrize("m", [3, 8, 9, 60, 500])
+def test_rows_that_a_consumer_adds(runtime, m, weigh):
+    """With `defer` many rows come as the experts' own; added by the framework's combining kernel they are what the layer gives itself."""
+    from tandemllm_b200.kernels import mxfp4, ops
+    g = torch.Generator().manual_seed(m)
+    first, down, v_first, v_down = layer(g, 6, 2, 72, 136)
+    q = mxfp4.quantize(first.to(DEV)), mxfp4.quantize(down.to(DEV))
+    x = rows(g, m, 136)
+    ids, wts = routed(g, m, 6, 3)
+    got = mxfp4.experts(runtime, x.to(DEV), ids.to(DEV), wts.to(DEV), *q, weigh=weigh, out_dtype=torch.float32, defer=True)
+    assert isinstance(got, ops.ExpertRows) == (m > mxfp4.EXPERT_ROWS)
+    P.hold(ops.materialize(got), *P.experts(x, ids, wts, v_first, v_down, "silu", weigh))
+
+
+def test_two_captured_graphs_replayed_in_turn(runtime):
+    """Products, both forms of the experts and the quantiser captured with inputs of their own: the replays do not disturb one another."""
+    from tandemllm_b200.kernels import mxfp4
+    g = torch.Generator().manual_seed(9)
+    first, down, *_ = layer(g, 8, 2, 200, 264)
+    w, w_first, w_down = weights(g, 264, 264).to(DEV), first.to(DEV), down.to(DEV)
+
+    def run(x, ids, wts):
+        q = mxfp4.quantize(w), mxfp4.quantize(w_first), mxfp4.quantize(w_down)
+        h = mxfp4.linear(runtime, x, q[0])
+        return mxfp4.experts(runtime, h, ids, wts, *q[1:], out_dtype=torch.float32)
+
+    inputs = [(rows(g, m, 264).to(DEV), *(t.to(DEV) for t in routed(g, m, 8, 3))) for m in (4, 70, 8)]
+    want = [run(*i) for i in inputs]
+    graphs, outs = [], []
+    for i in inputs:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(run(*i))
+        graphs.append(graph)
+    for order in ((0, 1, 2), (2, 1, 0, 0, 2, 1)):
+        for i in order:
+            outs[i].zero_()
+        for i in order:
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+
+
 # ---- refusals ----
 
 def test_refusals(runtime):
     from tandemllm_b200.kernels import mxfp4
     from tandemllm_b200.kernels.ops import KernelError
+    from tandemllm_b200.parts.base import Runtime
     x = torch.zeros(4, 64, dtype=torch.bfloat16, device=DEV)
     m, pair = mxfp4.quantize(torch.ones(16, 64, device=DEV)), mxfp4.quantize(torch.ones(2, 16, 64, device=DEV))
-    down = mxfp4.quantize(torch.ones(1, 64, 16, device=DEV))
+    up, down = mxfp4.quantize(torch.ones(1, 16, 64, device=DEV)), mxfp4.quantize(torch.ones(1, 64, 16, device=DEV))
     ids, wts = torch.zeros(4, 1, dtype=torch.int32, device=DEV), torch.ones(4, 1, device=DEV)
     for bad in (lambda: mxfp4.quantize(torch.ones(64, device=DEV)), lambda: mxfp4.quantize(torch.ones(2, 2, 2, 2, device=DEV)),
                 lambda: mxfp4.quantize(torch.ones(4, 64, dtype=torch.float16, device=DEV)), lambda: mxfp4.quantize(torch.ones(4, 64)),
@@ -250,6 +339,8 @@ def test_refusals(runtime):
                 lambda: mxfp4.experts(runtime, x, ids.long(), wts, pair, down), lambda: mxfp4.experts(runtime, x, ids[:3], wts[:3], pair, down),
                 lambda: mxfp4.experts(runtime, x, ids, wts[:, :0], pair, down), lambda: mxfp4.experts(runtime, x, ids, wts, down, pair),
                 lambda: mxfp4.experts(runtime, x, ids, wts, pair, down, "xielu"), lambda: mxfp4.experts(runtime, x, ids, wts, pair, down, weigh="both"),
+                lambda: mxfp4.linear(Runtime(torch.device("cpu"), torch.bfloat16), x, m), lambda: mxfp4.linear(runtime, x, m, act="gelu_tanh"),
+                lambda: mxfp4.linear(runtime, x, m, act=0), lambda: mxfp4.experts(runtime, x, ids, wts, up, down, "clamped_swish"),
                 lambda: mxfp4.experts(runtime, x, ids.expand(4, 40).contiguous(), wts.expand(4, 40).contiguous(), pair, down)):
         with pytest.raises(KernelError):
             bad()
