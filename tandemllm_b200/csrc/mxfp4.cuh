@@ -55,5 +55,22 @@ __device__ __forceinline__ float scale32(uint32_t four, int b) {
   return __uint_as_float((b < 3 ? four << (23 - 8 * b) : four >> 1) & 0x7F800000u);
 }
 
+// A launch that, with `behind`, may begin before the kernel in front of it in the stream has ended (programmatic dependent launch); the kernel waits
+// for that one's end itself (chain_wait). For the kernels of one call behind one another: the second's CTAs are on their SMs when the first's leave.
+template <typename... KernelArgs, typename... Args>
+inline int launch_behind(bool behind, void (*kernel)(KernelArgs...), dim3 grid, int threads, size_t smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = behind || chained_launches() ? 1 : 0;
+  return (int)cudaLaunchKernelEx(&cfg, kernel, static_cast<KernelArgs>(args)...);
+}
+
 }  // namespace mx
 }  // namespace tl

@@ -560,17 +560,8 @@ int launch_few(const mx::FewParams& p, mx::Kind kind, int nt, long long units, c
   }
   const long long ctas = ceil_div64(units, mx::GROUPS / p.team);
   const int bytes = mx::few_bytes(kind, nt, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)(ctas < sm_count() ? ctas : sm_count()));
-  cfg.blockDim = dim3(mx::THREADS);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = kind == mx::SECOND || chained_launches() ? 1 : 0;
-  return (int)cudaLaunchKernelEx(&cfg, kernel, p);
+  const dim3 grid((unsigned)(ctas < sm_count() ? ctas : sm_count()));
+  return mx::launch_behind(kind == mx::SECOND, kernel, grid, mx::THREADS, bytes, stream, p);
 }
 
 // Groups a unit: one where the groups of the GPU have units enough each, else two or four.

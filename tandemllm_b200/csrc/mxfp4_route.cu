@@ -154,7 +154,7 @@ extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_ro
   if (pairs == 0) return 0;
   TL_REQUIRE(pairs > 0 && experts >= 1 && experts <= mx::PLAN_EXPERTS && tile_rows_at_most >= 1, "mxfp4 experts: %d pairs of %d experts", pairs,
              experts);
-  return (int)launch_chained(mx::plan_kernel, dim3(1), dim3(mx::PLAN_THREADS), 0, stream, ids, pairs, experts, tile_rows_at_most, counts, sorted,
+  return mx::launch_behind(false, mx::plan_kernel, dim3(1), mx::PLAN_THREADS, 0, stream, ids, pairs, experts, tile_rows_at_most, counts, sorted,
                              place, tile_group, tile_row0, tile_rows, n_tiles, status);
 }
 
@@ -168,8 +168,8 @@ extern "C" int tl_mxfp4_gather(const void* x, long long ldx, const int* order, i
   TL_REQUIRE(blocks <= 0x7FFFFFFF, "mxfp4 product: %d rows of %d numbers are too many", rows, width);
   const bool whole = width % 8 == 0 && width == ld_to && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
 #define TL_GATHER(W_)                                                                                                                       \
-  return (int)launch_chained(mx::gather_kernel<W_>, dim3((unsigned)blocks), dim3(256), 0, stream, (const bf16*)x, ldx, order, div, (bf16*)to, \
-                             (int)ld_to, width, total)
+  return mx::launch_behind(order != nullptr, mx::gather_kernel<W_>, dim3((unsigned)blocks), 256, 0, stream, (const bf16*)x, ldx, order, div, \
+                           (bf16*)to, (int)ld_to, width, total)
   if (whole) TL_GATHER(true);
   TL_GATHER(false);
 #undef TL_GATHER
@@ -184,7 +184,7 @@ extern "C" int tl_mxfp4_sum(const float* y, const int* place, const int* ids, co
   const bool whole = N % 4 == 0 && ((uintptr_t)y % 16) == 0 && ((uintptr_t)out % 16) == 0;
   const dim3 grid(rows, ceil_div(N, 1024));
 #define TL_SUM(W_, T_) \
-  return (int)launch_chained(mx::sum_kernel<W_, T_>, grid, dim3(256), 0, stream, y, (long long)N, place, ids, wts, (T_*)out, N, top, experts)
+  return mx::launch_behind(true, mx::sum_kernel<W_, T_>, grid, 256, 0, stream, y, (long long)N, place, ids, wts, (T_*)out, N, top, experts)
   if (out_dtype == TL_FP32) {
     if (whole) TL_SUM(true, float);
     TL_SUM(false, float);

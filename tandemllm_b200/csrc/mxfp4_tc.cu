@@ -565,7 +565,6 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   using S = Many<MAXN>;
   constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
   chain_next();
-  chain_wait();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* slots = boxes + S::B_STAGES * S::B_BYTES;
@@ -597,6 +596,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
+  chain_wait();
   auto give_up = [&]() {
     *aborted = 1;
     atomicExch(p.status, 11);
@@ -872,8 +872,8 @@ int launch_many(const CUtensorMap& tmX, const TcParams& p, int tile_at_most, lon
     if (e != cudaSuccess) return (int)e;
     set_on = dev;
   }
-  kernel<<<(unsigned)(work < sm_count() ? work : sm_count()), S::THREADS, S::TOTAL, stream>>>(tmX, p, tile_at_most);
-  return (int)cudaGetLastError();
+  const dim3 grid((unsigned)(work < sm_count() ? work : sm_count()));
+  return launch_behind(p.tile_group != nullptr, kernel, grid, S::THREADS, S::TOTAL, stream, tmX, p, tile_at_most);
 }
 
 template <int BN, bool GATED, bool SPLIT, typename TOut>
