@@ -523,7 +523,8 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 //
 // With few rows an expert the converting warps are what takes longest: twelve of them (a layer of 64 experts with 4 rows each, 768 by 2048: 87 us
 // with eight, 76 with twelve, 74 with sixteen, which leaves four to finish and costs a product of 150 rows 2 of its 11 us; 73 with the sign and the
-// rest of a pair put in place by one multiplication, which took 5 to 10 % off all of these products).
+// rest of a pair put in place by one multiplication, which took 5 to 10 % off all of these products; 71 with a tile's codes read from shared
+// memory while the stores of the one before are under way).
 template <int MAXN>
 struct Many {
   static constexpr int BOX_ROWS = MAXN > 160 ? 256 : MAXN > 64 ? 80 : 16;      // token rows a TMA box
@@ -752,6 +753,17 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     };
 #pragma unroll
     for (int u = 0; u < (S::AHEAD ? S::AHEAD : BUFFERS); ++u) fetch(q[u % BUFFERS]);
+    auto read = [&](RowTile& q) {                               // the oldest tile of those on their way
+      if constexpr (S::AHEAD > 0) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(S::AHEAD > 0 ? S::AHEAD - 1 : 0) : "memory");
+        __syncwarp();
+#pragma unroll
+        for (int t = 0; t < 4; ++t) q.c[t] = load_shared16(my_slots + from + take + ((t << 4) ^ turned));
+        q.s = load_shared4(my_slots + from + 4 * TILE_CODES + lane * 4);
+        from = from + S::SLOT_BYTES == S::AHEAD * S::SLOT_BYTES ? 0 : from + S::SLOT_BYTES;
+      }
+    };
+    read(q[0]);
     // The tiles of all of the CTA's work items are one sequence; this group's are every GROUPS-th of an item, so the stage of one is its place
     // in the sequence, and how often the stage was used before it that place's round.
     int at = turn;                                              // the place of the tile at hand
@@ -760,16 +772,11 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
 #pragma unroll
       for (int u = 0; u < BUFFERS; ++u) {
         if (!ok || now.w >= work) break;
-        if constexpr (S::AHEAD > 0) {
-          asm volatile("cp.async.wait_group %0;" ::"n"(S::AHEAD > 0 ? S::AHEAD - 1 : 0) : "memory");
-          __syncwarp();
-#pragma unroll
-          for (int t = 0; t < 4; ++t) q[u].c[t] = load_shared16(my_slots + from + take + ((t << 4) ^ turned));
-          q[u].s = load_shared4(my_slots + from + 4 * TILE_CODES + lane * 4);
-          from = from + S::SLOT_BYTES == S::AHEAD * S::SLOT_BYTES ? 0 : from + S::SLOT_BYTES;
-        }
         const int stage = at % S::A_STAGES;
-        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &full[at % SLOTS], done, at - S::A_STAGES, aborted, [&]() { fetch(q[u]); });
+        ok = give_tile(t_lane + stage * S::A_COLS, q[u], &full[at % SLOTS], done, at - S::A_STAGES, aborted, [&]() {
+          fetch(q[u]);
+          read(q[u]);
+        });
         if (!ok && lane == 0) give_up();
         const int before = now.c;
         now.c += S::GROUPS;
