@@ -184,7 +184,7 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
 
     The form with the smallest estimated time, in us: `blocks` (of 128 k) one after the other in every round of CTAs, each as long as its
     weights take to convert or, persistent, as its tokens take to multiply; a round's start and end; and, where CTAs share a tile's k, adding
-    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 2 % slower than the
+    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 1.4 % slower than the
     fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14 us in one persistent tile, 18 where two CTAs share
     its k; 2048 rows 92 in tiles of 160, 106 in tiles of 192. At 2048 outputs of 7168: 256 rows 17 with eight CTAs a tile, 29 without;
     700 rows 30 without, 35 with two."""
@@ -193,7 +193,7 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
     for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
         rounds = -(-row_tiles * -(-rows // h) // sms)
         alone = 0.016 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
-        cost = 4.1 + rounds * (blocks * max(0.45 if h > 64 else 0.42, 0.0021 * h) + 0.96 + alone) + 0.0062 * h
+        cost = 4.2 + rounds * (blocks * max(0.45 if h > 64 else 0.415, 0.0021 * h) + 0.96 + alone) + 0.0055 * h
         if best is None or cost < best[0]:
             best = cost, h, 0
     for bn in (16, 32, 64, 128):
@@ -201,12 +201,12 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
             continue
         for splits in (1, 2, 4, 8):
             ctas = row_tiles * -(-rows // bn) * splits
-            if splits > 1 and (splits > blocks or ctas > 2 * sms):
+            if splits > 1 and (splits > blocks or 4 * ctas > 7 * sms):      # (clusters do not fill every SM twice: 288 CTAs take two rounds)
                 break
             rounds, rest = divmod(ctas, 2 * sms)                        # two CTAs an SM; one alone is faster
-            rounds += 0.0 if rest == 0 else 0.56 if rest <= sms else 1.0
-            cost = 4.3 + rounds * (-(-blocks // splits) * (0.63 + 0.0016 * bn) * (1.17 if gated else 1.0) + 0.52) + 0.0122 * bn
-            cost += 1.0 + 0.026 * bn if splits > 1 else 0.0
+            rounds += 0.0 if rest == 0 else 0.585 if rest <= sms else 1.0
+            cost = 4.4 + rounds * (-(-blocks // splits) * (0.614 + 0.0014 * bn) * (1.18 if gated else 1.0) + 0.34 + 0.0038 * bn) + 0.008 * bn
+            cost += 1.0 + 0.0265 * bn if splits > 1 else 0.0
             if cost < best[0]:
                 best = cost, bn, splits
     return best[1:]

@@ -53,7 +53,7 @@ def test_the_form_of_a_product_is_one_that_the_kernels_have(gated):
                     assert 64 <= h <= 256 and h % 16 == 0
                 else:
                     assert h in (16, 32, 64, 128) and splits in (1, 2, 4, 8) and splits <= -(-k // 128)
-                    assert splits == 1 or tiles * -(-rows // h) * splits <= 2 * 148
+                    assert splits == 1 or tiles * -(-rows // h) * splits <= 7 * 148 // 4
                     assert -(-rows // h) <= 65535
                 assert h == 64 or h < 2 * max(rows, 16)
 
