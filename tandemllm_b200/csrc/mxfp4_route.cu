@@ -9,24 +9,23 @@ constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_EXPERTS = 1024;
 constexpr int SUM_TOP = 32;
 
-// The sum of `v` over the threads before this one; `total` gets all of it. `scratch`: 33 integers.
-__device__ __forceinline__ int before_me(int v, int* scratch, int& total) {
+// The sum of `v` over the threads before this one; `total` gets all of it. `scratch`: 33 of them.
+__device__ __forceinline__ long long before_me(long long v, long long* scratch, long long& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int run = v;
+  long long run = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, run, o);
+    const long long a = __shfl_up_sync(0xffffffffu, run, o);
     if (lane >= o) run += a;
   }
-  __syncthreads();
   if (lane == 31) scratch[warp] = run;
   __syncthreads();
   if (warp == 0) {
-    const int mine = scratch[lane];
-    int sum = mine;
+    const long long mine = scratch[lane];
+    long long sum = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int a = __shfl_up_sync(0xffffffffu, sum, o);
+      const long long a = __shfl_up_sync(0xffffffffu, sum, o);
       if (lane >= o) sum += a;
     }
     scratch[lane] = sum - mine;
@@ -44,23 +43,40 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restric
                                                             int* __restrict__ tile_group, int* __restrict__ tile_row0, int* __restrict__ tile_rows,
                                                             int* __restrict__ n_tiles, int* status) {
   __shared__ int at[PLAN_EXPERTS + 1];
-  __shared__ int scratch[33];
+  __shared__ long long scratch[33];
   chain_next();
   chain_wait();
   const int tid = threadIdx.x;
+  // Eight ids a thread at once, on their way together; up to 8192 pairs they stay for the second pass. -1: none, else what names no expert is `experts`.
+  constexpr int HELD = 8;
+  int held[HELD];
+  auto load = [&](int p0) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      const int p = p0 + j * PLAN_THREADS;
+      held[j] = p < pairs ? ids[p] : -1;
+    }
+#pragma unroll
+    for (int j = 0; j < HELD; ++j)
+      if (p0 + j * PLAN_THREADS < pairs && (unsigned)held[j] >= (unsigned)experts) held[j] = experts;
+  };
   for (int e = tid; e <= experts; e += PLAN_THREADS) at[e] = 0;
+  load(tid);
   __syncthreads();
-  for (int p = tid; p < pairs; p += PLAN_THREADS) {
-    const int id = ids[p];
-    const bool ok = (unsigned)id < (unsigned)experts;
-    atomicAdd(&at[ok ? id : experts], 1);
-    if (!ok) atomicExch(status, 6);
+  for (int p0 = tid; p0 < pairs; p0 += HELD * PLAN_THREADS) {
+    if (p0 != tid) load(p0);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (held[j] >= 0) atomicAdd(&at[held[j]], 1);
+      if (held[j] == experts) atomicExch(status, 6);
+    }
   }
   __syncthreads();
+  // (two sums in one: pairs above, tiles below)
   const int mine = tid < experts ? at[tid] : 0, tiles = (mine + tile_rows_at_most - 1) / tile_rows_at_most;
-  int all, all_tiles;
-  const int first = before_me(mine, scratch, all);
-  const int first_tile = before_me(tiles, scratch, all_tiles);
+  long long total;
+  const long long before = before_me((long long)mine << 32 | tiles, scratch, total);
+  const int first = (int)(before >> 32), first_tile = (int)(before & 0x7FFFFFFF), all = (int)(total >> 32), all_tiles = (int)(total & 0x7FFFFFFF);
   if (tid < experts) {
     counts[tid] = mine;
     at[tid] = first;
@@ -75,11 +91,15 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restric
     *n_tiles = all_tiles;
   }
   __syncthreads();
-  for (int p = tid; p < pairs; p += PLAN_THREADS) {
-    const int id = ids[p];
-    const int to = atomicAdd(&at[(unsigned)id < (unsigned)experts ? id : experts], 1);
-    sorted[to] = p;
-    place[p] = to;
+  for (int p0 = tid; p0 < pairs; p0 += HELD * PLAN_THREADS) {
+    if (pairs > HELD * PLAN_THREADS) load(p0);
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (held[j] < 0) continue;
+      const int p = p0 + j * PLAN_THREADS, to = atomicAdd(&at[held[j]], 1);
+      sorted[to] = p;
+      place[p] = to;
+    }
   }
 }
 
@@ -152,8 +172,8 @@ using namespace tl;
 extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_rows_at_most, int* counts, int* sorted, int* place, int* tile_group,
                              int* tile_row0, int* tile_rows, int* n_tiles, int* status, cudaStream_t stream) {
   if (pairs == 0) return 0;
-  TL_REQUIRE(pairs > 0 && experts >= 1 && experts <= mx::PLAN_EXPERTS && tile_rows_at_most >= 1, "mxfp4 experts: %d pairs of %d experts", pairs,
-             experts);
+  TL_REQUIRE(pairs > 0 && pairs <= 1 << 30 && experts >= 1 && experts <= mx::PLAN_EXPERTS && tile_rows_at_most >= 1,
+             "mxfp4 experts: %d pairs of %d experts", pairs, experts);
   return mx::launch_behind(false, mx::plan_kernel, dim3(1), mx::PLAN_THREADS, 0, stream, ids, pairs, experts, tile_rows_at_most, counts, sorted,
                              place, tile_group, tile_row0, tile_rows, n_tiles, status);
 }

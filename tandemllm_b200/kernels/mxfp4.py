@@ -105,7 +105,7 @@ class Mxfp4Matrix:
         """The values as a plain tensor of `shape`, exact in either dtype."""
         code = ops.dtype_code(dtype)
         _here(self.data, "the matrix")
-        out = torch.empty(self.shape, dtype=dtype, device=self.device)
+        out = self.data.new_empty(self.shape, dtype=dtype)
         _check(lib().tl_mxfp4_values(self.codes, self.scales, out.data_ptr(), code, self.groups, self.n, self.k, ops.stream()), "mxfp4_values",
                kernels=int(out.numel() > 0))
         return out
@@ -124,7 +124,7 @@ def quantize(w: torch.Tensor) -> Mxfp4Matrix:
         w = w.contiguous()
         stride = w.stride()
     groups, n, k = (1, *shape) if len(shape) == 2 else shape
-    data = torch.empty(groups * -(-n // TILE_ROWS) * -(-k // TILE_K) * TILE_BYTES, dtype=torch.uint8, device=w.device)
+    data = w.new_empty(groups * -(-n // TILE_ROWS) * -(-k // TILE_K) * TILE_BYTES, dtype=torch.uint8)
     m = Mxfp4Matrix(data, shape)
     _check(lib().tl_mxfp4_quantize(w.data_ptr(), stride[-2], stride[0] if len(shape) == 3 else 0, code, m.codes, m.scales, groups, n, k,
                                    ops.stream()), "mxfp4_quantize", kernels=int(data.numel() > 0))
@@ -154,7 +154,7 @@ def _boxed(x: torch.Tensor, rows: int, k: int, ld: int, order: int | None = None
     if order is None and ld % 8 == 0 and ld >= k and x.data_ptr() % 16 == 0:
         return x, ld
     wide = -(-k // 8) * 8
-    copy = torch.empty(rows, wide, dtype=torch.bfloat16, device=x.device)
+    copy = x.new_empty(rows, wide)
     _check(lib().tl_mxfp4_gather(x.data_ptr(), ld, order, div, copy.data_ptr(), wide, rows, k, ops.stream()), "mxfp4_gather")
     return copy, wide
 
