@@ -18,6 +18,8 @@ requests at a context of 8192 tokens. A "step" is one decode step of the whole b
   points     decoded tokens a second at batch 1 and 64 with their roofline fractions, and the headline batch without
              CUDA graphs
 
+`--feed-forward-weights mxfp4` rounds the feed-forwards' matrices to 4-bit blocks when the engine makes them; the line's `dtype` says so.
+
 `--design puripel` does the same for Puripel beside an LFM2 MoE model of short-convolution and attention layers.
 `--design sebilorn` does the same for Sebilorn beside an LFM2 model of short-convolution and attention layers with dense
 feed-forwards.

@@ -7,8 +7,9 @@
 // Such a product reads every weight once and does little with it: its bounds are the weights' stream and their conversion. Codes become float16
 // numbers two at a time by a conversion of the GPU's, and a block's 32 products are two mma.sync m16n8k16 whose sum joins the others times the block's
 // scale, in 32 bits. (As bfloat16 numbers made of bits and times their scale, a word of eight codes takes 32 cycles of a scheduler with its MMA;
-// converted and times a float16 scale 19; so about 12.) The token rows become float16 numbers relative to their largest, which keeps all bits of a bfloat16
-// number down to 2^-31 of it; the power of two comes back with the sum.
+// converted and times a float16 scale 19; so about 12.) The token rows become float16 numbers relative to their largest, which becomes 2^14 or a
+// little more: that keeps all bits of a bfloat16 number down to 2^-31 of it; the power of two comes back with the sum (which weights beyond 2^100 can
+// make infinite before).
 //
 // A persistent CTA an SM has four groups of four warps. A group's producer (one thread of a warp of its own) keeps a ring of stages full
 // with bulk copies, which the layout's tiles make long: a stage is 16 weight rows by up to `slice` tiles of 128 k. The group's four warps take
@@ -218,7 +219,8 @@ __host__ __device__ __forceinline__ int stage_bytes(int slice) { return 2 * slic
 // of the sums two each a group), the rows' largest numbers.
 __host__ __device__ __forceinline__ int rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
 __host__ __device__ __forceinline__ int few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
-  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + GROUPS * (2 * stages + 4) * 8 + m * 4;
+  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + GROUPS * (2 * stages + 4) * 8 +
+         m * 4;
 }
 
 // Eight numbers of a token row from element k on, zeros past K and where there is no row. ALIGNED: rows begin at multiples of 16 bytes and K is a

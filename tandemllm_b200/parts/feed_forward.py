@@ -241,13 +241,14 @@ class SigmoidTopKExperts(Part):
             w_down = runtime.feed_forward_source(read(self.base + ".down_proj"))
         else:
             up_at = I if self.gated else 0          # (without a gate the up rows are all there is)
-            dtype = runtime.feed_forward_source(read(self._expert(0, "up"))[:1]).dtype
+            up = read(self._expert(0, "up"))
+            dtype = runtime.feed_forward_source(up[:1]).dtype
             w_gate_up = torch.empty(E, up_at + I, H, dtype=dtype, device=runtime.device)
             w_down = torch.empty(E, H, I, dtype=dtype, device=runtime.device)
             for e in range(E):
                 if self.gated:
                     w_gate_up[e, :I].copy_(read(self._expert(e, "gate")))
-                w_gate_up[e, up_at:].copy_(read(self._expert(e, "up")))
+                w_gate_up[e, up_at:].copy_(up if e == 0 else read(self._expert(e, "up")))
                 w_down[e].copy_(read(self._expert(e, "down")))
         self.w_gate_up = runtime.feed_forward_matrix(w_gate_up, 2 if self.gated else 1)
         self.w_down = runtime.feed_forward_matrix(w_down)
