@@ -521,10 +521,11 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
 // finish a tile while the next one's products run. The N side of an MMA is as many token rows as the tile has, rounded up to 16, and they come in
 // boxes of 256, 80 or 16.
 //
-// With few rows an expert the converting warps are what takes longest: twelve of them (a layer of 64 experts with 4 rows each, 768 by 2048: 87 us
-// with eight, 76 with twelve, 74 with sixteen, which leaves four to finish and costs a product of 150 rows 2 of its 11 us; 73 with the sign and the
-// rest of a pair put in place by one multiplication, which took 5 to 10 % off all of these products; 71 with a tile's codes read from shared
-// memory while the stores of the one before are under way).
+// With few rows an expert the converting warps are what takes longest: sixteen of them, and four that finish (a layer of 64 experts with 4 rows
+// each, 768 by 2048: 87 us with eight, 76 with twelve, 74 with sixteen; 72 with the sign and the rest of a pair put in place by one multiplication,
+// which took 5 to 10 % off all of these products; 69 with a tile's codes read from shared memory while the stores of the one before are under way).
+// Tiles as low of one matrix have the form of 160 rows, whose eight finishing warps are sooner done when nothing runs beside them (150 rows, 2500
+// gated outputs of 1096: 10.8 us, 13.4 with four).
 template <int MAXN>
 struct Many {
   static constexpr int BOX_ROWS = MAXN > 160 ? 256 : MAXN > 64 ? 80 : 16;      // token rows a TMA box
@@ -536,13 +537,13 @@ struct Many {
   static constexpr int A_STAGES = MAXN > 160 ? 4 : MAXN > 64 ? 3 : 6;
   static constexpr int ACCS = MAXN > 160 ? 1 : 2;
   static constexpr int A_AT = 512 - A_STAGES * A_COLS;           // the accumulators come first
-  static constexpr int CONVERT_WARPS = MAXN > 64 ? 8 : 12;
-  static constexpr int FINISH_WARPS = 8;
+  static constexpr int CONVERT_WARPS = MAXN > 64 ? 8 : 16;
+  static constexpr int FINISH_WARPS = MAXN > 64 ? 8 : 4;
   static constexpr int GROUPS = CONVERT_WARPS / 4;
   static constexpr int THREADS = (2 + CONVERT_WARPS + FINISH_WARPS) * 32;
-  // Tiles of codes that a converting warp has on their way to its part of shared memory (more than two or three gain nothing); 0: two in registers,
+  // Tiles of codes that a converting warp has on their way to its part of shared memory (more gain nothing); 0: two in registers,
   // where the token rows leave no room. Through shared memory a warp's copies are whole lines: 768 rows to 32 experts 133 -> 122 us.
-  static constexpr int AHEAD = MAXN > 160 ? 0 : 3;
+  static constexpr int AHEAD = MAXN > 160 ? 0 : MAXN > 64 ? 3 : 2;
   static constexpr int SLOT_BYTES = 4 * (TILE_CODES + TILE_SCALES);
   static constexpr int TOTAL = B_STAGES * B_BYTES + CONVERT_WARPS * AHEAD * SLOT_BYTES + 1024 /* alignment slack */ + 256 /* barriers */;
   static_assert(TOTAL <= 227 * 1024, "a CTA's shared memory");
@@ -947,7 +948,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     const long long work = (long long)ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS) * (tile_group ? max_tiles : ceil_div(M, bn));
     TL_REQUIRE(work <= 0x7FFFFFFF, "mxfp4 product: %lld tiles are too many", work);
     CUtensorMap tmX;
-    const int box = bn <= 64 ? mx::Many<64>::BOX_ROWS : bn <= 160 ? mx::Many<160>::BOX_ROWS : mx::Many<256>::BOX_ROWS;
+    const int box = bn <= 64 && tile_group ? mx::Many<64>::BOX_ROWS : bn <= 160 ? mx::Many<160>::BOX_ROWS : mx::Many<256>::BOX_ROWS;
     const int r = tensor_map(x, x_rows, K, ldx, box, &tmX);
     if (r) return r;
 #define TL_MX_MANY(N_)                                                                                \
@@ -956,7 +957,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     if (out_dtype == TL_FP32) return mx::launch_many<N_, false, float>(tmX, p, bn, work, stream);     \
     return mx::launch_many<N_, false, bf16>(tmX, p, bn, work, stream);                                \
   } while (0)
-    if (bn <= 64) TL_MX_MANY(64);
+    if (bn <= 64 && tile_group) TL_MX_MANY(64);
     if (bn <= 160) TL_MX_MANY(160);
     TL_MX_MANY(256);
 #undef TL_MX_MANY

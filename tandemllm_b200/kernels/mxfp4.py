@@ -194,7 +194,7 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
     for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
         rounds = -(-row_tiles * -(-rows // h) // sms)
         alone = 0.016 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
-        cost = 4.2 + rounds * (blocks * max(0.45 if h > 64 else 0.415, 0.0021 * h) + 0.96 + alone) + 0.0055 * h
+        cost = 4.2 + rounds * (blocks * max(0.45, 0.0021 * h) + 0.96 + alone) + 0.0055 * h
         if best is None or cost < best[0]:
             best = cost, h, 0
     for bn in (16, 32, 64, 128):
