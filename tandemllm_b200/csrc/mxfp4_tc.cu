@@ -566,7 +566,6 @@ template <int MAXN, bool GATED, typename TOut>
 __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const __grid_constant__ CUtensorMap tmX, TcParams p, int tile_at_most) {
   using S = Many<MAXN>;
   constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
-  chain_next();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* boxes = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* slots = boxes + S::B_STAGES * S::B_BYTES;
@@ -598,6 +597,9 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
+  // The next kernel of a layer may come only when every CTA of this one has its tensor memory: it takes its own before it waits for this kernel's end,
+  // and a CTA here that waited for what a cluster of another stream holds, while that cluster waits for what the next kernel holds, would close a circle.
+  chain_next();
   chain_wait();
   auto give_up = [&]() {
     *aborted = 1;

@@ -185,7 +185,7 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
 
     The form with the smallest estimated time, in us: `blocks` (of 128 k) one after the other in every round of CTAs, each as long as its
     weights take to convert or, persistent, as its tokens take to multiply; a round's start and end; and, where CTAs share a tile's k, adding
-    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 1.4 % slower than the
+    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 1.1 % slower than the
     fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14 us in one persistent tile, 18 where two CTAs share
     its k; 2048 rows 92 in tiles of 160, 106 in tiles of 192. At 2048 outputs of 7168: 256 rows 17 with eight CTAs a tile, 29 without;
     700 rows 30 without, 35 with two."""
@@ -193,8 +193,8 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
     best = None
     for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
         rounds = -(-row_tiles * -(-rows // h) // sms)
-        alone = 0.016 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
-        cost = 4.2 + rounds * (blocks * max(0.45, 0.0021 * h) + 0.96 + alone) + 0.0055 * h
+        alone = 0.024 * h if h > 160 else 0.0                           # (one accumulator: a tile is stored before the next is multiplied)
+        cost = 4.2 + rounds * (blocks * max(0.45, 0.0021 * h) + 0.96 + alone) + 0.0045 * h
         if best is None or cost < best[0]:
             best = cost, h, 0
     for bn in (16, 32, 64, 128):
@@ -206,7 +206,7 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
                 break
             rounds, rest = divmod(ctas, 2 * sms)                        # two CTAs an SM; one alone is faster
             rounds += 0.0 if rest == 0 else 0.585 if rest <= sms else 1.0
-            cost = 4.4 + rounds * (-(-blocks // splits) * (0.614 + 0.0014 * bn) * (1.18 if gated else 1.0) + 0.34 + 0.0038 * bn) + 0.008 * bn
+            cost = 4.4 + rounds * (-(-blocks // splits) * (0.66 + 0.0014 * bn) * (1.18 if gated else 1.0) + 0.34 + 0.009 * bn) + 0.008 * bn
             cost += 1.0 + 0.0265 * bn if splits > 1 else 0.0
             if cost < best[0]:
                 best = cost, bn, splits
