@@ -216,10 +216,10 @@ template <> struct Place<DENSE> { typedef int Type; };              // (never lo
 
 __host__ __device__ __forceinline__ int stage_bytes(int slice) { return 2 * slice * (TILE_CODES + TILE_SCALES); }
 // Dynamic shared memory: token rows (SECOND: and one of zeros), rings, two sets of the warps' sums, barriers (full and empty ones of the rings,
-// of the sums two each a group), the rows' largest numbers.
+// of the sums two each a group, and one of SECOND's rows), the rows' largest numbers.
 __host__ __device__ __forceinline__ int rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
 __host__ __device__ __forceinline__ int few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
-  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + GROUPS * (2 * stages + 4) * 8 +
+  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + (GROUPS * (2 * stages + 4) + 1) * 8 +
          m * 4;
 }
 
@@ -290,10 +290,15 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   uint64_t* empty = full + p.stages * GROUPS;
   uint64_t* summed = empty + p.stages * GROUPS;                 // [2][GROUPS]: a team's sums are there
   uint64_t* taken = summed + 2 * GROUPS;                        // and read
-  uint32_t* tops = reinterpret_cast<uint32_t*>(taken + 2 * GROUPS);       // the bits of a token row's largest number
+  uint64_t* rows_there = taken + 2 * GROUPS;                    // SECOND
+  uint32_t* tops = reinterpret_cast<uint32_t*>(rows_there + 1);           // the bits of a token row's largest number
   if (threadIdx.x < (2 * p.stages + 4) * GROUPS) {
     const int i = threadIdx.x / GROUPS - p.stages;
     mbar_init(&full[threadIdx.x], i < 0 ? 1 : i < p.stages ? GROUP_WARPS : i < p.stages + 2 ? p.team * GROUP_WARPS : p.team);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (KIND == SECOND && threadIdx.x == THREADS - 1) {
+    mbar_init(rows_there, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (threadIdx.x == 0) aborted_ = 0;
@@ -357,6 +362,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
       }
       // no CTA leaves with copies under way, whether it gave up or not
       for (int i = max(0, it - p.stages); i < it; ++i) mbar_wait(&full[(i % p.stages) * GROUPS + group], (i / p.stages) & 1);
+      if (KIND == SECOND) mbar_wait(rows_there, 0);
     }
     return;
   }
@@ -418,36 +424,58 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
 
   // ---- token rows into shared memory ----
   if (KIND == SECOND) {
+    // whole rows by bulk copies, which no register waits for, made float16 numbers where they lie
+    const uint32_t bytes = k_tiles * TILE_K * 2;
     chain_wait();
-    load_round();
+    if (lane == 0) {
+      asm volatile("fence.proxy.async;" ::: "memory");          // (the rows were written by ordinary stores)
+      for (int m = warp; m < p.M; m += WARPS) copy_bulk(xs + m * x_bytes, static_cast<const bf16*>(p.x) + m * p.ldx, bytes, rows_there);
+      if (warp == 0) mbar_expect_tx(rows_there, p.M * bytes);
+    }
+    __syncwarp();
     for (int m = warp; m < p.M; m += WARPS) {
       uint32_t top = 0u;
-#pragma unroll 4
-      for (int i = lane; i < p.parts; i += 32) top = max(top, __float_as_uint(p.largest[(long long)m * p.parts + i]));
+      for (int i0 = lane; i0 < p.parts; i0 += 8 * 32) {
+        uint32_t some[8];                                       // on their way together
+#pragma unroll
+        for (int j = 0; j < 8; ++j) some[j] = i0 + 32 * j < p.parts ? __float_as_uint(p.largest[(long long)m * p.parts + i0 + 32 * j]) : 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = max(top, some[j]);
+      }
       top = __reduce_max_sync(0xffffffffu, top);
       if (lane == 0) tops[m] = top;
     }
   }
   asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
-  if (KIND != SECOND && all_pieces > ROUND * WARPS) {
-    next_m = 0, next_c = warp;
-    load_round();
-  }
-  for (int done = 0; done < all_pieces; done += ROUND * WARPS) {
-    if (done) load_round();
+  auto put_piece = [&](int m, int k, const uint4& eight) {
+    const float f = power(14 - row_exponent(tops[m]));
+    float v[8];
+    unpack8(eight, v);
+    __half2 h[4];
 #pragma unroll
-    for (int j = 0; j < ROUND; ++j) {
-      if (m_of[j] >= p.M || k_of[j] >= k_tiles * TILE_K) continue;
-      const float f = power(14 - row_exponent(tops[m_of[j]]));
-      float v[8];
-      unpack8(raw[j], v);
-      __half2 h[4];
+    for (int e = 0; e < 4; ++e) {
+      const int at = (e & 1) * 4 + (e >> 1);
+      h[e] = __floats2half2_rn(v[at] * f, v[at + 2] * f);
+    }
+    *reinterpret_cast<uint4*>(xs + m * x_bytes + k * 2) = *reinterpret_cast<const uint4*>(h);
+  };
+  if constexpr (KIND == SECOND) {
+    if (!__all_sync(0xffffffffu, mbar_wait(rows_there, 0)) && lane == 0) give_up();
+#pragma unroll 4
+    for (int piece = warp; piece < all_pieces; piece += WARPS) {
+      const int m = piece / a_row, k = (piece - m * a_row) * 256 + lane * 8;
+      if (k < k_tiles * TILE_K) put_piece(m, k, *reinterpret_cast<const uint4*>(xs + m * x_bytes + k * 2));
+    }
+  } else {
+    if (all_pieces > ROUND * WARPS) {
+      next_m = 0, next_c = warp;
+      load_round();
+    }
+    for (int done = 0; done < all_pieces; done += ROUND * WARPS) {
+      if (done) load_round();
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = (e & 1) * 4 + (e >> 1);
-        h[e] = __floats2half2_rn(v[at] * f, v[at + 2] * f);
-      }
-      *reinterpret_cast<uint4*>(xs + m_of[j] * x_bytes + k_of[j] * 2) = *reinterpret_cast<const uint4*>(h);
+      for (int j = 0; j < ROUND; ++j)
+        if (m_of[j] < p.M && k_of[j] < k_tiles * TILE_K) put_piece(m_of[j], k_of[j], raw[j]);
     }
   }
   if (KIND == SECOND)
