@@ -447,8 +447,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
     }
   }
   asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
-  auto put_piece = [&](int m, int k, const uint4& eight) {
-    const float f = power(14 - row_exponent(tops[m]));
+  auto put_piece = [&](int m, int k, const uint4& eight, float f) {
     float v[8];
     unpack8(eight, v);
     __half2 h[4];
@@ -461,10 +460,20 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   };
   if constexpr (KIND == SECOND) {
     if (!__all_sync(0xffffffffu, mbar_wait(rows_there, 0)) && lane == 0) give_up();
+    auto in_place = [&](int m, int k, float f) {
+      if (k < k_tiles * TILE_K) put_piece(m, k, *reinterpret_cast<const uint4*>(xs + m * x_bytes + k * 2), f);
+    };
+    if (p.M >= WARPS) {                                         // a warp whole rows
+      for (int m = warp; m < p.M; m += WARPS) {
+        const float f = power(14 - row_exponent(tops[m]));
 #pragma unroll 4
-    for (int piece = warp; piece < all_pieces; piece += WARPS) {
-      const int m = piece / a_row, k = (piece - m * a_row) * 256 + lane * 8;
-      if (k < k_tiles * TILE_K) put_piece(m, k, *reinterpret_cast<const uint4*>(xs + m * x_bytes + k * 2));
+        for (int k = lane * 8; k < k_tiles * TILE_K; k += 256) in_place(m, k, f);
+      }
+    } else {
+      for (int piece = warp; piece < all_pieces; piece += WARPS) {
+        const int m = piece / a_row;
+        in_place(m, (piece - m * a_row) * 256 + lane * 8, power(14 - row_exponent(tops[m])));
+      }
     }
   } else {
     if (all_pieces > ROUND * WARPS) {
@@ -475,7 +484,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
       if (done) load_round();
 #pragma unroll
       for (int j = 0; j < ROUND; ++j)
-        if (m_of[j] < p.M && k_of[j] < k_tiles * TILE_K) put_piece(m_of[j], k_of[j], raw[j]);
+        if (m_of[j] < p.M && k_of[j] < k_tiles * TILE_K) put_piece(m_of[j], k_of[j], raw[j], power(14 - row_exponent(tops[m_of[j]])));
     }
   }
   if (KIND == SECOND)
