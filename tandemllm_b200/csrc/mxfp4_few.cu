@@ -113,7 +113,7 @@ struct Items {
   int count;
   short expert[MAX_PAIRS];
   short pair[MAX_PAIRS][MAX_ROWS];        // -1: the row did not choose it
-  int key[MAX_PAIRS];
+  alignas(16) int key[MAX_PAIRS];
   short leader[MAX_PAIRS];
   uint32_t firsts[MAX_PAIRS / 32];
   float weight[MAX_PAIRS];
@@ -165,8 +165,11 @@ __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids
   for (int p = threadIdx.x; p < MAX_PAIRS; p += THREADS) {
     const int key = s.key[p];
     int leader = 0;
-    if (key >= 0)
-      while (s.key[leader] != key) ++leader;
+    for (bool found = key < 0; !found; leader += found ? 0 : 4) {       // (four at a time, at the latest its own)
+      const int4 four = *reinterpret_cast<const int4*>(s.key + leader);
+      found = four.x == key || four.y == key || four.z == key || four.w == key;
+      if (found) leader += four.x == key ? 0 : four.y == key ? 1 : four.z == key ? 2 : 3;
+    }
     s.leader[p] = (short)leader;
     const uint32_t firsts = __ballot_sync(0xffffffffu, key >= 0 && leader == p);
     if (lane == 0) s.firsts[p >> 5] = firsts;
