@@ -114,14 +114,21 @@ struct Items {
   short expert[MAX_PAIRS];
   short pair[MAX_PAIRS][MAX_ROWS];        // -1: the row did not choose it
   alignas(16) int key[MAX_PAIRS];
-  short leader[MAX_PAIRS];
+  short leader[MAX_PAIRS];                // the id, until the leaders are known
   uint32_t firsts[MAX_PAIRS / 32];
   float weight[MAX_PAIRS];
 };
 
+// From L2: what the SM has held of this memory since an earlier kernel does not count.
+__device__ __forceinline__ int load_id(const int* p) {
+  int v;
+  asm volatile("ld.relaxed.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+
 // All of the CTA's threads; ends with a barrier. `mine`: with up to 32 pairs, the id of pair `lane` in the first copying warp. An id that names no
 // expert is recorded in `status` and its pair counts for nothing.
-__device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids, int mine, int pairs, int top, int experts, int* status) {
+__device__ __forceinline__ void find_items(Items& s, const int* ids, int mine, int pairs, int top, int experts, int* status) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (pairs <= 32) {
     if (warp == WARPS) {                    // (the others may be at the token rows meanwhile)
@@ -145,19 +152,24 @@ __device__ __forceinline__ void find_items(Items& s, const int* __restrict__ ids
     __syncthreads();
     return;
   }
+  for (int p = threadIdx.x; p < pairs; p += THREADS) {
+    const int id = load_id(ids + p);
+    s.leader[p] = (short)(id >= 0 && id < experts ? id : -1);
+#pragma unroll
+    for (int r = 0; r < MAX_ROWS; ++r) s.pair[p][r] = -1;
+  }
+  __syncthreads();
   for (int p = threadIdx.x; p < MAX_PAIRS; p += THREADS) {
     int key = -1;
     if (p < pairs) {
-      const int id = ids[p];
-      if (id >= 0 && id < experts) {
+      const int id = s.leader[p];
+      if (id >= 0) {
         int again = 0;
-        for (int q = p - p % top; q < p; ++q) again += ids[q] == id;
+        for (int q = p - p % top; q < p; ++q) again += s.leader[q] == id;
         key = id * 32 + again;
       } else {
         atomicExch(status, 6);
       }
-#pragma unroll
-      for (int r = 0; r < MAX_ROWS; ++r) s.pair[p][r] = -1;
     }
     s.key[p] = key;
   }
@@ -259,13 +271,14 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   __shared__ int aborted_;
   volatile int* aborted = &aborted_;
   // SECOND starts behind FIRST's end on its SM, not behind all of it (programmatic dependent launch): it sets itself up, finds its items and has its
-  // first weights on their way before it waits for the rows that FIRST makes.
-  chain_next();
+  // first weights on their way before it waits for the rows that FIRST makes. The ids that it reads in front of its wait are another kernel's results.
+  // They are final by then, because FIRST opens the door only behind its own wait, and they are read where all SMs see the same (load_id).
   if (KIND != SECOND) chain_wait();
+  chain_next();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = warp < WARPS ? warp / GROUP_WARPS : (warp - WARPS) % GROUPS;
   int my_id = -1;
-  if (KIND != DENSE && warp == WARPS && lane < p.rows * p.top) my_id = p.ids[lane];
+  if (KIND != DENSE && warp == WARPS && lane < p.rows * p.top) my_id = load_id(p.ids + lane);
   const int k_tiles = ceil_div(p.K, TILE_K), row_tiles = ceil_div(p.N, TILE_ROWS);
   const int x_bytes = row_bytes(k_tiles), one_stage = stage_bytes(p.slice);
   // The token rows: a warp takes 256 numbers of a row at a time, ROUND such pieces on their way. Their largest numbers come first; what fits one
