@@ -1,5 +1,8 @@
 // Around the routed experts' products of a step that is too large for the two-kernel form (mxfp4_few.cu): which pairs (row, slot) an expert
 // has, its token rows side by side, and the weighed sum of what the experts made of a row.
+//
+// The kernels begin before the ones in front of them have ended. What those leave is read behind chain_wait() and through pointers that promise
+// nothing: of a `const __restrict__` one the compiler may read early, and by the read-only path.
 #include "mxfp4.cuh"
 
 namespace tl {
@@ -38,10 +41,8 @@ __device__ __forceinline__ long long before_me(long long v, long long* scratch, 
 
 // One block. Pairs of an expert lie together, in any order among themselves: a row's products do not depend on the rows beside it, so the
 // order, which the atomics leave open, changes no result. Pairs without an expert come last and are in no tile.
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restrict__ ids, int pairs, int experts, int tile_rows_at_most,
-                                                            int* __restrict__ counts, int* __restrict__ sorted, int* __restrict__ place,
-                                                            int* __restrict__ tile_group, int* __restrict__ tile_row0, int* __restrict__ tile_rows,
-                                                            int* __restrict__ n_tiles, int* status) {
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* ids, int pairs, int experts, int tile_rows_at_most, int* counts, int* sorted,
+                                                            int* place, int* tile_group, int* tile_row0, int* tile_rows, int* n_tiles, int* status) {
   __shared__ int at[PLAN_EXPERTS + 1];
   __shared__ long long scratch[33];
   chain_next();
@@ -105,8 +106,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* __restric
 
 // to[i] = from[order[i] / div] (without an order from[i]), eight numbers a thread; those past `width` stay as they are.
 template <bool WHOLE>
-__global__ void __launch_bounds__(256) gather_kernel(const bf16* __restrict__ from, long long ld, const int* __restrict__ order, int div,
-                                                     bf16* __restrict__ to, int ld_to, int width, long long total) {
+__global__ void __launch_bounds__(256) gather_kernel(const bf16* from, long long ld, const int* order, int div, bf16* to, int ld_to, int width,
+                                                     long long total) {
   chain_next();
   chain_wait();
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -124,9 +125,8 @@ __global__ void __launch_bounds__(256) gather_kernel(const bf16* __restrict__ fr
 
 // out[r] = sum over r's slots, one after the other, of wts * y[place]; without weights the rows as they are. Four outputs a thread.
 template <bool WHOLE, typename TOut>
-__global__ void __launch_bounds__(256) sum_kernel(const float* __restrict__ y, long long ldy, const int* __restrict__ place,
-                                                  const int* __restrict__ ids, const float* __restrict__ wts, TOut* __restrict__ out, int N, int top,
-                                                  int experts) {
+__global__ void __launch_bounds__(256) sum_kernel(const float* y, long long ldy, const int* place, const int* ids, const float* wts, TOut* out, int N,
+                                                  int top, int experts) {
   __shared__ int s_place[SUM_TOP];
   __shared__ float s_weight[SUM_TOP];
   chain_next();

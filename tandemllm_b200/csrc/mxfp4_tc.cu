@@ -47,10 +47,14 @@ struct TcParams {
   const int* n_tiles;
   int act;                    // the gate's activation (TL_ACT_*), 0 for a plain product; negated: an activation on a plain product's results
   float ga0, ga1;
-  const float* row_weight;    // grouped (or null): a (row, slot) pair's own weight on its sums, see `pair_weight`
+  const float* row_weight;    // grouped (or null): a (row, slot) pair's own weight on its sums, row_weight[weight_index[position]]
   const int* weight_index;
   int* status;
 };
+
+__device__ __forceinline__ float weight_of(const TcParams& p, long long position) {
+  return p.row_weight[p.weight_index ? (long long)p.weight_index[position] : position];
+}
 
 template <int BN>
 struct Tc {
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
           continue;
         }
         if (p.row_weight) {
-          const float w = (lane & 15) < left ? pair_weight(p.row_weight, p.weight_index, (long long)tok0 + c0 + (lane & 15)) : 1.f;
+          const float w = (lane & 15) < left ? weight_of(p, (long long)tok0 + c0 + (lane & 15)) : 1.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] *= __shfl_sync(0xffffffffu, w, j);
         }
@@ -489,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
             if (GATED) u += load_from(part + m * ROWS + r + 8, s);
           }
           if (p.row_weight) {
-            const float w = pair_weight(p.row_weight, p.weight_index, (long long)tok0 + m);
+            const float w = weight_of(p, (long long)tok0 + m);
             v *= w, u *= w;
           }
           if (p.bias) {
@@ -819,7 +823,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
         tmem_load16(from + c0, v);
         const int left = tok_rows - c0;
         if (p.row_weight) {
-          const float weight = (lane & 15) < left ? pair_weight(p.row_weight, p.weight_index, (long long)tok0 + c0 + (lane & 15)) : 1.f;
+          const float weight = (lane & 15) < left ? weight_of(p, (long long)tok0 + c0 + (lane & 15)) : 1.f;
 #pragma unroll
           for (int j = 0; j < 16; ++j) v[j] *= __shfl_sync(0xffffffffu, weight, j);
         }

@@ -11,3 +11,15 @@ def test_the_experts_second_half_finds_final_ids():
     assert body.index("if (KIND != SECOND) chain_wait();") < body.index("chain_next();")
     text = source("mxfp4_few.cu")
     assert "ids[" not in text and "ld.relaxed.gpu.global.s32" in text
+
+
+def test_results_of_the_kernel_in_front_are_not_read_through_the_read_only_path():
+    """A `const __restrict__` pointer lets the compiler read early and through the read-only path, whatever stands between. The quantiser
+    and its way back begin when everything in front of them has ended."""
+    for name in ("mxfp4_few.cu", "mxfp4_route.cu", "mxfp4_tc.cu"):
+        assert "__restrict__" not in source(name) and "__ldg" not in source(name) and "pair_weight" not in source(name)
+        for kernel, (parameters, body) in kernels(name).items():
+            assert "chain_wait();" in body, kernel
+    for kernel, (parameters, body) in kernels("mxfp4.cu").items():
+        assert "chain" not in body
+    assert "launch_behind" not in source("mxfp4.cu") and "cudaLaunchKernelEx" not in source("mxfp4.cu")
