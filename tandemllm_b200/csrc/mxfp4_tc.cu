@@ -304,7 +304,6 @@ template <int BN, bool GATED, bool SPLIT, typename TOut>
 __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ CUtensorMap tmX, TcParams p) {
   using S = Tc<BN>;
   constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
-  chain_next();
   chain_wait();
   int tok0, tok_rows, group = 0;
   if (p.tile_group) {
@@ -348,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   __syncthreads();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem_base = *tmem_slot;
+  chain_next();               // (only now: see the persistent form)
   auto give_up = [&]() {
     *aborted = 1;
     atomicExch(p.status, 11);

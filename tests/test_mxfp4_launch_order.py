@@ -23,3 +23,14 @@ def test_results_of_the_kernel_in_front_are_not_read_through_the_read_only_path(
     for kernel, (parameters, body) in kernels("mxfp4.cu").items():
         assert "chain" not in body
     assert "launch_behind" not in source("mxfp4.cu") and "cudaLaunchKernelEx" not in source("mxfp4.cu")
+
+
+def test_the_next_kernel_comes_when_this_one_has_its_tensor_memory():
+    """A kernel that begins early may take tensor memory before it waits for this one's end. What it took a CTA here would wait for, for good."""
+    found = 0
+    for kernel, (parameters, body) in kernels("mxfp4_tc.cu").items():
+        assert body.count("chain_next();") == 1
+        taken = body.index("__syncthreads();", body.index("tcgen05.alloc"))
+        assert taken < body.index("chain_next();"), kernel
+        found += 1
+    assert found == 2
