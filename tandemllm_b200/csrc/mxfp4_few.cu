@@ -39,8 +39,8 @@ constexpr int MAX_PAIRS = 256;                        // of the experts' form
 constexpr int MAX_ROWS = 8;
 
 // Token rows in shared memory: a row's length is 64 modulo 128 bytes, so that the 16 bytes of eight lanes (two rows, four quarters of a
-// block) fall on all banks. Eight numbers lie as the codes' conversion leaves theirs: 0 2, 4 6, 1 3, 5 7.
-__host__ __device__ __forceinline__ int row_bytes(int k_tiles) { return k_tiles * TILE_K * 2 + 64; }
+// block) fall on all banks. Eight numbers lie as the codes' conversion leaves theirs: 0 2, 4 6, 1 3, 5 7. (64 bits: it is asked of any length.)
+__host__ __device__ __forceinline__ long long row_bytes(int k_tiles) { return k_tiles * (TILE_K * 2ll) + 64; }
 
 __device__ __forceinline__ void mma_16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -232,8 +232,8 @@ template <> struct Place<DENSE> { typedef int Type; };              // (never lo
 __host__ __device__ __forceinline__ int stage_bytes(int slice) { return 2 * slice * (TILE_CODES + TILE_SCALES); }
 // Dynamic shared memory: token rows (SECOND: and one of zeros), rings, two sets of the warps' sums, barriers (full and empty ones of the rings,
 // of the sums two each a group, and one of SECOND's rows), the rows' largest numbers.
-__host__ __device__ __forceinline__ int rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
-__host__ __device__ __forceinline__ int few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
+__host__ __device__ __forceinline__ long long rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
+inline long long few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
   return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + (GROUPS * (2 * stages + 4) + 1) * 8 +
          m * 4;
 }
@@ -280,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   int my_id = -1;
   if (KIND != DENSE && warp == WARPS && lane < p.rows * p.top) my_id = load_id(p.ids + lane);
   const int k_tiles = ceil_div(p.K, TILE_K), row_tiles = ceil_div(p.N, TILE_ROWS);
-  const int x_bytes = row_bytes(k_tiles), one_stage = stage_bytes(p.slice);
+  const int x_bytes = (int)row_bytes(k_tiles), one_stage = stage_bytes(p.slice);
   // The token rows: a warp takes 256 numbers of a row at a time, ROUND such pieces on their way. Their largest numbers come first; what fits one
   // round stays in registers until these are known, the rest is read again.
   constexpr int ROUND = 4;
@@ -299,7 +299,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   };
   if (KIND != SECOND && warp < WARPS) load_round();
   uint8_t* xs = smem;
-  uint8_t* rings = smem + rows_bytes(KIND, p.M, k_tiles);
+  uint8_t* rings = smem + (int)rows_bytes(KIND, p.M, k_tiles);
   uint8_t* ring = rings + group * p.stages * one_stage;
   float (*part)[WARPS][16][COLS + 1] = reinterpret_cast<float (*)[WARPS][16][COLS + 1]>(rings + GROUPS * p.stages * one_stage);
   uint64_t* full = reinterpret_cast<uint64_t*>(part + 2);       // [stages][GROUPS], and so on
@@ -614,7 +614,7 @@ int launch_few(const mx::FewParams& p, mx::Kind kind, int nt, long long units, c
     set_on = dev;
   }
   const long long ctas = ceil_div64(units, mx::GROUPS / p.team);
-  const int bytes = mx::few_bytes(kind, nt, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);
+  const int bytes = (int)mx::few_bytes(kind, nt, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);        // (few_fits has passed it)
   const dim3 grid((unsigned)(ctas < sm_count() ? ctas : sm_count()));
   return mx::launch_behind(kind == mx::SECOND, kernel, grid, mx::THREADS, bytes, stream, p);
 }
