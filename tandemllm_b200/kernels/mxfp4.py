@@ -85,19 +85,48 @@ def _here(t: torch.Tensor, what: str) -> int:
     return index
 
 
+def data_bytes(shape: tuple[int, ...]) -> int:
+    """Bytes of the matrix or matrices of this shape."""
+    return (1 if len(shape) == 2 else shape[0]) * -(-shape[-2] // TILE_ROWS) * -(-shape[-1] // TILE_K) * TILE_BYTES
+
+
 class Mxfp4Matrix:
-    """`groups` matrices [n, k] in 4-bit blocks, in the kernels' layout (csrc/mxfp4.cuh): `data` (uint8) holds the codes of all tiles of 8 rows by
-    128 k, both sizes rounded up, and behind them their scales. `shape` is the shape of the tensor it was made of."""
+    """`groups` matrices [n, k] in 4-bit blocks, in the kernels' layout (csrc/mxfp4.cuh): `data` (uint8, contiguous) holds the codes of all tiles
+    of 8 rows by 128 k, both sizes rounded up, and behind them their scales. `shape` is the shape of the tensor it was made of. A copy, also a
+    pickled one, has the bytes of its own `data`."""
 
     def __init__(self, data: torch.Tensor, shape: tuple[int, ...]):
-        self.data, self.shape, self.device = data, tuple(shape), data.device
+        shape = tuple(int(s) for s in shape)
+        if len(shape) not in (2, 3) or min(shape) < 0:
+            raise ops.KernelError(f"mxfp4: a matrix of shape {shape}; [n, k] or [groups, n, k] is wanted")
         self.groups, self.n, self.k = (1 if len(shape) == 2 else shape[0]), shape[-2], shape[-1]
-        self.index, self.codes = data.get_device(), data.data_ptr()
-        self.scales = self.codes + data.numel() // TILE_BYTES * TILE_CODES
+        size = data_bytes(shape)
+        if data.dtype is not torch.uint8 or data.numel() != size or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ops.KernelError(f"mxfp4: {data.dtype} data of {data.numel()} bytes for a matrix of shape {shape}; {size} contiguous bytes (uint8) "
+                                  "from a multiple of 16 on are wanted")
+        self._data, self.shape, self.device, self.index = data, shape, data.device, data.get_device()
+        self._codes_bytes = size // TILE_BYTES * TILE_CODES
+
+    @property
+    def data(self) -> torch.Tensor:
+        return self._data
+
+    @property
+    def codes(self) -> int:
+        """The address of the codes."""
+        return self._data.data_ptr()
+
+    @property
+    def scales(self) -> int:
+        """The address of the scales."""
+        return self._data.data_ptr() + self._codes_bytes
+
+    def __reduce__(self):
+        return Mxfp4Matrix, (self._data, self.shape)
 
     @property
     def nbytes(self) -> int:
-        return self.data.numel()
+        return self._data.numel()
 
     def numel(self) -> int:
         return self.groups * self.n * self.k
@@ -105,8 +134,8 @@ class Mxfp4Matrix:
     def values(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
         """The values as a plain tensor of `shape`, exact in either dtype."""
         code = ops.dtype_code(dtype)
-        _here(self.data, "the matrix")
-        out = self.data.new_empty(self.shape, dtype=dtype)
+        _here(self._data, "the matrix")
+        out = self._data.new_empty(self.shape, dtype=dtype)
         _check(lib().tl_mxfp4_values(self.codes, self.scales, out.data_ptr(), code, self.groups, self.n, self.k, ops.stream()), "mxfp4_values",
                kernels=int(out.numel() > 0))
         return out
@@ -125,7 +154,7 @@ def quantize(w: torch.Tensor) -> Mxfp4Matrix:
         w = w.contiguous()
         stride = w.stride()
     groups, n, k = (1, *shape) if len(shape) == 2 else shape
-    data = w.new_empty(groups * -(-n // TILE_ROWS) * -(-k // TILE_K) * TILE_BYTES, dtype=torch.uint8)
+    data = w.new_empty(data_bytes(shape), dtype=torch.uint8)
     m = Mxfp4Matrix(data, shape)
     _check(lib().tl_mxfp4_quantize(w.data_ptr(), stride[-2], stride[0] if len(shape) == 3 else 0, code, m.codes, m.scales, groups, n, k,
                                    ops.stream()), "mxfp4_quantize", kernels=int(data.numel() > 0))
