@@ -222,7 +222,13 @@ struct FewParams {
   int rows, top, experts;     // FIRST, SECOND
   int team, slice, stages;    // groups a unit, tiles a stage, stages a ring
   int* status;
+  int skip;                   // -1; a test sets the group's stage whose copies are left out, so that a wait runs out
 };
+
+inline int& skip_stage_for_test() {
+  static int stage = -1;
+  return stage;
+}
 
 enum Kind { DENSE, FIRST, SECOND };
 
@@ -369,6 +375,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
           const long long matrix = KIND == DENSE ? 0 : (long long)items->expert[item] * (GATED ? 2 : 1);
           const long long lo = (matrix * row_tiles + row_lo) * k_tiles + tile0;
           const long long hi = ((matrix + (GATED ? 1 : 0)) * row_tiles + row_hi) * k_tiles + tile0;
+          if (it == p.skip) continue;
           mbar_expect_tx(bar, 2 * n * (TILE_CODES + TILE_SCALES));
           copy_bulk(to, p.codes + lo * TILE_CODES, n * TILE_CODES, bar);
           copy_bulk(to + p.slice * TILE_CODES, p.codes + hi * TILE_CODES, n * TILE_CODES, bar);
@@ -377,7 +384,8 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
         }
       }
       // no CTA leaves with copies under way, whether it gave up or not
-      for (int i = max(0, it - p.stages); i < it; ++i) mbar_wait(&full[(i % p.stages) * GROUPS + group], (i / p.stages) & 1);
+      for (int i = max(0, it - p.stages); i < it; ++i)
+        if (i != p.skip) mbar_wait(&full[(i % p.stages) * GROUPS + group], (i / p.stages) & 1);
       if (KIND == SECOND) mbar_wait(rows_there, 0);
     }
     return;
@@ -603,7 +611,8 @@ bool few_fits(mx::Kind kind, int nt, int m, int k_tiles, mx::FewParams& p) {
 }
 
 template <auto kernel>
-int launch_few(const mx::FewParams& p, mx::Kind kind, int nt, long long units, cudaStream_t stream) {
+int launch_few(mx::FewParams& p, mx::Kind kind, int nt, long long units, cudaStream_t stream) {
+  p.skip = mx::skip_stage_for_test();
   static thread_local int set_on = -1;              // the device whose function has its shared memory
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -730,3 +739,11 @@ extern "C" int tl_mxfp4_experts_second(void* between, const void* codes, const v
   if (out_dtype == TL_FP32) return launch_few<mx::few_kernel<1, false, mx::SECOND, true, float>>(p, mx::SECOND, 1, units, stream);
   return launch_few<mx::few_kernel<1, false, mx::SECOND, true, bf16>>(p, mx::SECOND, 1, units, stream);
 }
+
+// For tests of the bounded waits: the polls after which a wait of this file's kernels gives up (0 puts the default back), and the stage of
+// weights, counted over a group's work, that is not copied (-1: none).
+extern "C" int tl_mxfp4_few_set_wait_limit(unsigned int polls) {
+  const uint32_t v = polls ? polls : (1u << 22);
+  return (int)cudaMemcpyToSymbol(wait_limit, &v, sizeof(v));
+}
+extern "C" void tl_mxfp4_few_test_skip_stage(int stage) { mx::skip_stage_for_test() = stage; }

@@ -19,7 +19,8 @@
 // every CTA adds the sums of some of the tokens in rank order and stores them, so the result does not depend on timing.
 //
 // Every wait on an mbarrier is bounded: when a bound is hit the CTA records status 11, stops issuing work, waits (bounded again) for the
-// copies and products in flight, meets its cluster, frees its tensor memory and returns.
+// copies and products in flight, meets its cluster, frees its tensor memory and returns. The copies' barriers also count the warps that convert
+// weights; for one that leaves early its arrivals are made up at the CTA's end.
 #include "mxfp4.cuh"
 #include "tma.cuh"
 
@@ -50,7 +51,16 @@ struct TcParams {
   const float* row_weight;    // grouped (or null): a (row, slot) pair's own weight on its sums, row_weight[weight_index[position]]
   const int* weight_index;
   int* status;
+  int copies, products;       // a test's: the tiles of 128 k, counted over a CTA's work, behind which no token rows are copied any more, and
+};                            // those behind which the products give up as if their wait had run out
+
+struct StopForTest {
+  int copies = 0x7fffffff, products = 0x7fffffff;
 };
+inline StopForTest& stop_for_test() {
+  static StopForTest stop;
+  return stop;
+}
 
 __device__ __forceinline__ float weight_of(const TcParams& p, long long position) {
   return p.row_weight[p.weight_index ? (long long)p.weight_index[position] : position];
@@ -271,11 +281,12 @@ __device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint
   return true;
 }
 
-// After giving up: the copies of tiles from .. to - 1 that are under way land before the CTA's shared memory goes away. The converting warps may
-// have left without their arrivals, so those are made up for.
-__device__ __forceinline__ void drain(uint64_t* full, int from, int to, int lane) {
-  for (int c = max(0, from); c < to; ++c) {
-    if (lane < 4) mbar_arrive(&full[c % SLOTS]);
+// At a CTA's end, where somebody gave up: of the `copied` tiles the last `STAGES` may not be there yet, and they land before the CTA's shared memory
+// goes away. A converting warp that left early (of a tile's group of four, in place `left` of the CTA's tiles) owes its arrivals from there on.
+template <int STAGES, int GROUPS>
+__device__ __forceinline__ void drain(uint64_t* full, int copied, int k_tiles, volatile int* left, int lane) {
+  for (int c = max(0, copied - STAGES); c < copied; ++c) {
+    if (lane < 4 && left[c % k_tiles % GROUPS * 4 + lane] <= c) mbar_arrive(&full[c % SLOTS]);
     __syncwarp();
     mbar_wait(&full[c % SLOTS], (c / SLOTS) & 1);
   }
@@ -328,6 +339,8 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   uint64_t* acc_full = done + SLOTS;
   uint32_t* tmem_slot = (uint32_t*)(acc_full + 1);
   volatile uint32_t* aborted = tmem_slot + 1;
+  volatile int* copied = (int*)(tmem_slot + 2);
+  volatile int* left = copied + 1;                              // see drain()
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -339,6 +352,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     *aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x < EPI_WARPS) left[threadIdx.x] = 0x7fffffff;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"((uint32_t)S::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -358,7 +372,8 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     // ---- token rows ----
     Ring<S::B_STAGES> ring;
     int issued = 0;
-    for (int c = 0; c < tiles; ++c, ring.next()) {
+    const int copies = min(tiles, p.copies);
+    for (int c = 0; c < copies; ++c, ring.next()) {
       if (!__all_sync(0xffffffffu, wait_nth(done, c - S::B_STAGES) && *aborted == 0)) {
         give_up();
         break;
@@ -372,15 +387,15 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
       __syncwarp();
       issued = c + 1;
     }
-    if (*aborted)              // copies already started must land before the CTA's shared memory goes away
-      drain(full, issued - S::B_STAGES, issued, lane);
+    *copied = issued;
   } else if (warp == 1) {
     // ---- products: f32 sums, bf16 operands, both K-major, M = 128, N = BN ----
     constexpr uint32_t idesc = (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
     Ring<S::A_STAGES> ra;
     Ring<S::B_STAGES> rb;
     bool there = false;
-    for (int c = 0; c < tiles; ++c, ra.next(), rb.next()) {
+    const int products = min(tiles, p.products);
+    for (int c = 0; c < products; ++c, ra.next(), rb.next()) {
       if (!there && !__all_sync(0xffffffffu, wait_nth(full, c))) {
         give_up();
         break;
@@ -390,8 +405,10 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
                     2 * c + 1 < num_kb, &done[c % SLOTS]);
       there = __all_sync(0xffffffffu, next);
     }
+    if (products < tiles) give_up();
     if (elected()) commit(acc_full);
     __syncwarp();
+    mbar_wait(acc_full, 0);                 // the products have left tensor memory and shared memory before anybody frees them
   } else {
     // ---- weights: tensor-memory lanes 32 (warp % 4) .. + 31, tiles of 128 k of this group's parity ----
     const int half = (warp - 2) >> 2, r = (warp & 3) * 32 + lane;
@@ -417,7 +434,10 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
             const int after = c + 2 * AHEAD;
             load_row_tile(q[u], codes + (long long)after * TILE_CODES, scales + (long long)after * TILE_SCALES, valid && after < tiles);
           });
-          if (!ok && lane == 0) give_up();
+          if (!ok && lane == 0) {
+            give_up();
+            left[warp - 2] = c;
+          }
         }
       }
     }
@@ -510,6 +530,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (warp == 0 && *aborted) drain<S::B_STAGES, 2>(full, *copied, tiles, left, lane);
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"((uint32_t)S::TMEM_COLS));
@@ -579,6 +600,8 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   uint64_t* acc_empty = acc_full + 2;
   uint32_t* tmem_slot = (uint32_t*)(acc_empty + 2);
   volatile uint32_t* aborted = tmem_slot + 1;
+  volatile int* copied = (int*)(tmem_slot + 2);
+  volatile int* left = copied + 1;                              // see drain()
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -593,6 +616,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
     *aborted = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
+  if (threadIdx.x < S::CONVERT_WARPS) left[threadIdx.x] = 0x7fffffff;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::);
@@ -638,7 +662,8 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
       const int tok0 = coming.first, tok_rows = min(coming.rows, MAXN);
       coming = tokens_of(w + gridDim.x);
       const int boxes_here = ceil_div(tok_rows, S::BOX_ROWS);
-      for (int c = 0; c < k_tiles; ++c, ring.next()) {
+      const int copies = min(k_tiles, p.copies - issued);
+      for (int c = 0; c < copies; ++c, ring.next()) {
         if (!__all_sync(0xffffffffu, wait_nth(done, issued - S::B_STAGES) && *aborted == 0)) {
           give_up();
           ok = false;
@@ -656,9 +681,9 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
         __syncwarp();
         ++issued;
       }
+      if (copies < k_tiles) break;
     }
-    if (*aborted)              // copies already started must land before the CTA's shared memory goes away
-      drain(full, issued - S::B_STAGES, issued, lane);
+    *copied = issued;
   } else if (warp == 1) {
     // ---- products ----
     Ring<S::A_STAGES> ra;
@@ -676,7 +701,8 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
         break;
       }
       const uint32_t d = tmem_base + rd.stage * MAXN;
-      for (int c = 0; c < k_tiles; ++c, ++tile, ra.next(), rb.next()) {
+      const int products = min(k_tiles, p.products - tile);
+      for (int c = 0; c < products; ++c, ++tile, ra.next(), rb.next()) {
         if (!there && !__all_sync(0xffffffffu, wait_nth(full, tile))) {
           give_up();
           ok = false;
@@ -688,6 +714,10 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
         multiply_tile(d, tmem_base + S::A_AT + ra.stage * S::A_COLS, smem_u32(boxes + rb.stage * S::B_BYTES) >> 4, S::HALF_BYTES >> 4, idesc, c > 0,
                       2 * c + 1 < num_kb, &done[tile % SLOTS]);
         there = __all_sync(0xffffffffu, next);
+      }
+      if (products < k_tiles) {
+        give_up();
+        ok = false;
       }
       if (elected()) commit(&acc_full[rd.stage]);      // (also where it gave up: whoever waits learns of it)
       __syncwarp();
@@ -784,7 +814,10 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
           fetch(q[u]);
           read(q[u]);
         });
-        if (!ok && lane == 0) give_up();
+        if (!ok && lane == 0) {
+          give_up();
+          left[warp - 2] = at;
+        }
         const int before = now.c;
         now.c += S::GROUPS;
         if (now.c >= k_tiles) {
@@ -867,6 +900,7 @@ __global__ void __launch_bounds__(Many<MAXN>::THREADS, 1) tc_many_kernel(const _
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (warp == 0 && *aborted) drain<S::B_STAGES, S::GROUPS>(full, *copied, k_tiles, left, lane);
   if (warp == 1) {
     __syncwarp();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(512u));
@@ -948,6 +982,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     splits = ceil_div(k_tiles, p.tiles_a_split);                // (rounding up may leave the last ones nothing)
   }
   p.tile_group = tile_group, p.tile_row0 = tile_row0, p.tile_rows = tile_rows, p.n_tiles = n_tiles;
+  p.copies = mx::stop_for_test().copies, p.products = mx::stop_for_test().products;
   p.act = act, p.ga0 = a0, p.ga1 = a1, p.row_weight = row_weight, p.weight_index = weight_index, p.status = status;
   if (splits == 0) {
     TL_REQUIRE(bn >= 1 && bn <= 256, "mxfp4 product: token tiles of %d rows", bn);
@@ -991,4 +1026,14 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
   TL_MX_TC(128);
 #undef TL_MX_TC
 #undef TL_MX_TC_
+}
+
+// For tests of the bounded waits: the polls after which a wait of this file's kernels gives up (0 puts the default back), and the tiles of 128 k,
+// counted over a CTA's work, behind which no token rows are copied and behind which the products give up (-1: none).
+extern "C" int tl_mxfp4_tc_set_wait_limit(unsigned int polls) {
+  const uint32_t v = polls ? polls : (1u << 22);
+  return (int)cudaMemcpyToSymbol(wait_limit, &v, sizeof(v));
+}
+extern "C" void tl_mxfp4_tc_test_stop(int copies, int products) {
+  mx::stop_for_test() = {copies < 0 ? 0x7fffffff : copies, products < 0 ? 0x7fffffff : products};
 }
