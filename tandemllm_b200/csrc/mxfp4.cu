@@ -89,14 +89,14 @@ __global__ void __launch_bounds__(CODER_WARPS * 32, 4) quantize_kernel(const T* 
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t e = top >> 23;
       const bool finite = e < 255u;
-      const uint32_t s = finite ? max(e, 2u) - 2u : 255u;
-      const float inverse = __uint_as_float((254u - min(s, 253u)) << 23);                       // 2^(127 - s), a normal number
+      const uint32_t t = finite ? max(e, 2u) - 1u : 255u;
+      const float inverse = __uint_as_float((255u - min(t, 254u)) << 23);                       // 2^(128 - t), a normal number
       float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) y[j] = v[i][j] * inverse;
       const uint32_t word = finite ? encode4(y[2], y[0], y[6], y[4], y[3], y[1], y[7], y[5]) : 0u;
       reinterpret_cast<uint32_t*>(codes + tile * TILE_CODES)[to.at + 32 * i] = word;
-      if ((threadIdx.x & 3) == 0) scales[tile * TILE_SCALES + to.scale_at + 2 * i * (TILE_K / BLOCK)] = (uint8_t)s;
+      if ((threadIdx.x & 3) == 0) scales[tile * TILE_SCALES + to.scale_at + 2 * i * (TILE_K / BLOCK)] = (uint8_t)t;
     }
   }
 }

@@ -5,7 +5,8 @@
 // are zeros). A word of codes holds eight consecutive values of a row, those of even places in its lower half, those of odd places in its
 // upper one. A tile's codes are 512 bytes, [row r][quarter t of 4][block b of 4]: the word of row r's values 32 b + 8 t .. + 7. So 16 bytes at (r, t)
 // are what lane (r, t) of a warp multiplies in an MMA of each of the tile's four blocks, and 64 bytes what a lane of tensor memory needs. Behind the
-// codes of all tiles come their scales, 32 bytes a tile, [row][block].
+// codes of all tiles come their scales, 32 bytes a tile, [row][block], as t = s + 1 (255 stays): the exponent of a 32-bit number, 2^(t - 127), which
+// is twice the scale and a normal number for every s.
 #pragma once
 #include "common.cuh"
 
@@ -25,11 +26,12 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
 }
 
 // As bfloat16 numbers, exactly. With a code's lower three bits at the lowest exponent bits and the highest mantissa bit a bfloat16 number is
-// value * 2^-126 (E2M1's subnormal falls on bfloat16's), and one multiplication by 2^(s - 1) makes it the value. `factor` is 2^(min(s, 128) - 1)
-// twice in a word, `factor_left` what is missing where s > 128 (not a number for 255).
-__device__ __forceinline__ uint32_t factor(uint32_t s) { return (min(s, 128u) + 126u) * 0x00800080u; }
-__device__ __forceinline__ uint32_t factor_left(uint32_t s) {
-  return s <= 128u ? 0x3F803F80u : s == 255u ? 0x7FFF7FFFu : (s - 1u) * 0x00800080u;
+// value * 2^-126 (E2M1's subnormal falls on bfloat16's), and one multiplication by 2^(t - 2) makes it the value. `factor` is 2^(min(t, NEAR) - 2)
+// twice in a word, `factor_left` what is missing where t > NEAR (not a number for 255).
+constexpr uint32_t NEAR = 129;
+__device__ __forceinline__ uint32_t factor(uint32_t t) { return (min(t, NEAR) + 125u) * 0x00800080u; }
+__device__ __forceinline__ uint32_t factor_left(uint32_t t) {
+  return t <= NEAR ? 0x3F803F80u : t == 255u ? 0x7FFF7FFFu : (t - 2u) * 0x00800080u;
 }
 // The four pairs of a word, times `f`: pair j is values 2 j (lower half) and 2 j + 1. A pair alone in its word times two powers of two is its sign at a
 // half's top and its other bits at their place, beside copies that the mask takes away: a multiplication, which another pipe than the logic does.
@@ -49,8 +51,7 @@ __device__ __forceinline__ void values16(uint32_t w, uint32_t (&v)[4]) {
       "cvt.rn.f16x2.e2m1x2 %0, b0;\n\tcvt.rn.f16x2.e2m1x2 %1, b1;\n\tcvt.rn.f16x2.e2m1x2 %2, b2;\n\tcvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(w));
 }
-// The scale of block b from a row's four in a word, in 32 bits: 2^(s - 127); 0 for s = 0 (2^-127 times a sum of float16 products is below 32-bit's
-// normal numbers), infinite for 255, which the zeros that such a block has for codes make a NaN.
+// Twice the scale of block b from a row's four in a word, in 32 bits; infinite for 255, which the zeros that such a block has for codes make a NaN.
 __device__ __forceinline__ float scale32(uint32_t four, int b) {
   return __uint_as_float((b < 3 ? four << (23 - 8 * b) : four >> 1) & 0x7F800000u);
 }

@@ -8,8 +8,8 @@
 // numbers two at a time by a conversion of the GPU's, and a block's 32 products are two mma.sync m16n8k16 whose sum joins the others times the block's
 // scale, in 32 bits. (As bfloat16 numbers made of bits and times their scale, a word of eight codes takes 32 cycles of a scheduler with its MMA;
 // converted and times a float16 scale 19; so about 12.) The token rows become float16 numbers relative to their largest, which becomes 2^14 or a
-// little more: that keeps all bits of a bfloat16 number down to 2^-31 of it; the power of two comes back with the sum (which weights beyond 2^100 can
-// make infinite before).
+// little more: that keeps all bits of a bfloat16 number down to 2^-31 of it, and nothing below 2^-39; the power of two comes back with the sum (which
+// weights of 2^112 / K, 2^95 for the longest rows taken, can make infinite before).
 //
 // A persistent CTA an SM has four groups of four warps. A group's producer (one thread of a warp of its own) keeps a ring of stages full
 // with bulk copies, which the layout's tiles make long: a stage is 16 weight rows by up to `slice` tiles of 128 k. The group's four warps take
@@ -60,8 +60,11 @@ __device__ __forceinline__ void copy_bulk(void* dst, const void* src, uint32_t b
 
 // 2^e for e in -126 .. 127
 __device__ __forceinline__ float power(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
-// The exponent of a row whose largest number has the bits `top` (without the sign): its numbers times 2^(14 - exponent) are float16 numbers.
-__device__ __forceinline__ int row_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -112); }
+// The exponent of a row whose largest number has the bits `top` (without the sign): its numbers times `to_half` are float16 numbers, and sums of
+// these times twice the blocks' scales (scale32) are what they are times `from_half`.
+__device__ __forceinline__ int row_exponent(uint32_t top) { return max((int)(top >> 23) - 127, -111); }
+__device__ __forceinline__ float to_half(uint32_t top) { return power(14 - row_exponent(top)); }
+__device__ __forceinline__ float from_half(uint32_t top) { return power(row_exponent(top) - 15); }
 
 // acc[j] += 16 weight rows by 128 k times the token rows of every tile j of eight. `lo` and `hi`: a lane's words of the four blocks in row g and
 // in row g + 8; `s_lo` and `s_hi` these rows' scales.
@@ -419,7 +422,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
           if (GATED) u += part[buffer][s][o + 8][m];
         }
         if (KIND != SECOND && mine) {
-          const float f = power(row_exponent(tops[m]) - 14);
+          const float f = from_half(tops[m]);
           v *= f;
           if (GATED) u *= f;
         }
@@ -489,14 +492,14 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
     };
     if (p.M >= WARPS) {                                         // a warp whole rows
       for (int m = warp; m < p.M; m += WARPS) {
-        const float f = power(14 - row_exponent(tops[m]));
+        const float f = to_half(tops[m]);
 #pragma unroll 4
         for (int k = lane * 8; k < k_tiles * TILE_K; k += 256) in_place(m, k, f);
       }
     } else {
       for (int piece = warp; piece < all_pieces; piece += WARPS) {
         const int m = piece / a_row;
-        in_place(m, (piece - m * a_row) * 256 + lane * 8, power(14 - row_exponent(tops[m])));
+        in_place(m, (piece - m * a_row) * 256 + lane * 8, to_half(tops[m]));
       }
     }
   } else {
@@ -508,7 +511,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
       if (done) load_round();
 #pragma unroll
       for (int j = 0; j < ROUND; ++j)
-        if (m_of[j] < p.M && k_of[j] < k_tiles * TILE_K) put_piece(m_of[j], k_of[j], raw[j], power(14 - row_exponent(tops[m_of[j]])));
+        if (m_of[j] < p.M && k_of[j] < k_tiles * TILE_K) put_piece(m_of[j], k_of[j], raw[j], to_half(tops[m_of[j]]));
     }
   }
   if (KIND == SECOND)
@@ -553,7 +556,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
         for (int c = 0; c < 2; ++c) {
           const int pair = items->pair[item][2 * t + c];
           if (pair >= 0) {
-            const float f = power(row_exponent(tops[pair]) - 14);
+            const float f = from_half(tops[pair]);
             acc[0][c] = fmaf(sum[0][c], f, acc[0][c]);
             acc[0][c + 2] = fmaf(sum[0][c + 2], f, acc[0][c + 2]);
           }

@@ -234,7 +234,7 @@ __device__ __forceinline__ uint32_t load_shared4(uint32_t from) {
 template <int HALF>
 __device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
   const uint32_t s[2] = {(q.s >> (16 * HALF)) & 255u, (q.s >> (16 * HALF + 8)) & 255u};
-  const bool far = __any_sync(0xffffffffu, max(s[0], s[1]) > 128u);
+  const bool far = __any_sync(0xffffffffu, max(s[0], s[1]) > NEAR);
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
     const uint32_t w[2] = {HALF ? q.c[t].z : q.c[t].x, HALF ? q.c[t].w : q.c[t].y};

@@ -9,7 +9,8 @@
 Rows are bfloat16 and every sum is 32-bit: the weights are exact in bfloat16, so a product is what the bfloat16 path would give for the
 rounded weights. The compute happens on the device of the rows, which has to be the current one, on its current stream; nothing is kept
 between calls but what the caller passes in. There is no 32-bit product: a 32-bit runtime takes the values as a plain matrix. Products of
-up to 16 rows take a row relative to its largest number (as 2^14): weights beyond 2^100 can make their sums infinite.
+up to 16 rows take a row relative to its largest number: what is below 2^-31 of it loses bits, what is below 2^-39 counts as zero, and weights
+beyond 2^95 can make their sums infinite.
 """
 
 from __future__ import annotations
