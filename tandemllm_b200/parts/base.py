@@ -143,12 +143,16 @@ class Runtime:
     def vector(self, t: torch.Tensor) -> torch.Tensor:
         return t.to(device=self.device, dtype=torch.float32).contiguous()
 
-    def feed_forward_source(self, t: torch.Tensor) -> torch.Tensor:
-        """A feed-forward's stored matrix on the device, in the dtype its matrix is made of: the compute dtype, or, where it is to be
-        rounded to 4-bit blocks, the stored one (both compute dtypes then round the same numbers)."""
+    def feed_forward_dtype(self, *tensors: torch.Tensor) -> torch.dtype:
+        """The dtype that a matrix made of these stored tensors is made in: the compute dtype, or, where it is to be rounded to 4-bit blocks,
+        one that holds them all as they are (both compute dtypes then round the same numbers)."""
         if self.feed_forward_weights == "stored":
-            return self.matrix(t)
-        return t.to(device=self.device, dtype=t.dtype if t.dtype in (torch.float32, torch.bfloat16) else torch.float32).contiguous()
+            return self.dtype
+        return torch.bfloat16 if all(t.dtype is torch.bfloat16 for t in tensors) else torch.float32
+
+    def feed_forward_source(self, t: torch.Tensor) -> torch.Tensor:
+        """A feed-forward's stored matrix on the device, in its `feed_forward_dtype`."""
+        return t.to(device=self.device, dtype=self.feed_forward_dtype(t)).contiguous()
 
     def feed_forward_matrix(self, t: torch.Tensor, matrices: int | None = None):
         """The matrix [n, k] or the matrices [groups, n, k] of a feed-forward from `feed_forward_source`: as they are; with "mxfp4" a

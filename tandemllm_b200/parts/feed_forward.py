@@ -241,17 +241,26 @@ class SigmoidTopKExperts(Part):
             w_down = runtime.feed_forward_source(read(self.base + ".down_proj"))
         else:
             up_at = I if self.gated else 0          # (without a gate the up rows are all there is)
-            up = read(self._expert(0, "up"))
-            dtype = runtime.feed_forward_source(up[:1]).dtype
-            w_gate_up = torch.empty(E, up_at + I, H, dtype=dtype, device=runtime.device)
-            w_down = torch.empty(E, H, I, dtype=dtype, device=runtime.device)
+            w_gate_up = w_down = None
             for e in range(E):
+                gate = [read(self._expert(e, "gate"))] if self.gated else []
+                up, down = read(self._expert(e, "up")), read(self._expert(e, "down"))
+                w_gate_up = self._staged(w_gate_up, (E, up_at + I, H), *gate, up)
+                w_down = self._staged(w_down, (E, H, I), down)
                 if self.gated:
-                    w_gate_up[e, :I].copy_(read(self._expert(e, "gate")))
-                w_gate_up[e, up_at:].copy_(up if e == 0 else read(self._expert(e, "up")))
-                w_down[e].copy_(read(self._expert(e, "down")))
+                    w_gate_up[e, :I].copy_(gate[0])
+                w_gate_up[e, up_at:].copy_(up)
+                w_down[e].copy_(down)
         self.w_gate_up = runtime.feed_forward_matrix(w_gate_up, 2 if self.gated else 1)
         self.w_down = runtime.feed_forward_matrix(w_down)
+
+    def _staged(self, w, shape, *tensors):
+        """Where the experts' matrices are put side by side (None: not there yet), for these tensors: as it is, or in a wider type where they need
+        one."""
+        dtype = self.runtime.feed_forward_dtype(*tensors)
+        if w is None:
+            return torch.empty(shape, dtype=dtype, device=self.runtime.device)
+        return w.to(torch.promote_types(w.dtype, dtype))
 
     def expected_experts_read(self, rows: int) -> float:
         """Distinct experts that `rows` rows choose when every expert is as likely as any other."""
