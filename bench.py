@@ -18,7 +18,8 @@ requests at a context of 8192 tokens. A "step" is one decode step of the whole b
   points     decoded tokens a second at batch 1 and 64 with their roofline fractions, and the headline batch without
              CUDA graphs
 
-`--feed-forward-weights mxfp4` rounds the feed-forwards' matrices to 4-bit blocks when the engine makes them; the line's `dtype` says so.
+`--feed-forward-weights mxfp4` rounds the feed-forwards' matrices to 4-bit blocks when the engine makes them; the line's `dtype` says so. The mixed
+scenario and the profile table take it, the design comparisons and the reference do not.
 
 `--design puripel` does the same for Puripel beside an LFM2 MoE model of short-convolution and attention layers.
 `--design sebilorn` does the same for Sebilorn beside an LFM2 model of short-convolution and attention layers with dense
@@ -295,6 +296,10 @@ def reference_arm(a) -> int:
 
 
 # ------------------------------------------------------------------------------------------ helpers of our arm
+def dtype_label(a) -> str:
+    return ("bf16" if a.dtype == "bfloat16" else "fp32") + ("" if a.feed_forward_weights == "stored" else ", feed-forward weights mxfp4")
+
+
 def prefill_flops(cfg, tokens: int) -> dict:
     """Flops of a prompt of `tokens` tokens by family (multiply-adds times two; the head for the last row only)."""
     H, T = cfg.hidden_size, tokens
@@ -334,15 +339,15 @@ def start_with_context(engine, prompt: list[int], params):
 
 
 class LaunchTimer:
-    """Times every launcher call of the package's two libraries with a pair of CUDA events (a launcher is one kernel,
+    """Times every launcher call of the package's libraries with a pair of CUDA events (a launcher is one kernel,
     sometimes two), so that a step's time can be summed by kernel family without a profiler. The events themselves
     cost a little: compare shares, and the sum with the step's own time."""
 
     def __init__(self):
         import torch
-        from tandemllm_b200.kernels import ops, tensorcore
+        from tandemllm_b200.kernels import mxfp4, ops, tensorcore
         self.torch = torch
-        self.libs = [ops.core(), tensorcore.lib()]
+        self.libs = [ops.core(), tensorcore.lib()] + ([mxfp4.lib()] if mxfp4._lib is not None else [])
         self.saved = []
         self.calls = []
 
@@ -360,6 +365,10 @@ class LaunchTimer:
             return "dense products (tcgen05, pairs of SMs)"
         if name == "tl_gemm_tc_pair_act":
             return "dense products (tcgen05, pairs of SMs, activation in the epilogue)"
+        if name == "tl_mxfp4_tc":                # args: ..., act at 11, ..., tile_group at 17
+            if args[17]:
+                return "experts gate/up + activation (MXFP4, tcgen05)" if args[11] else "experts down (MXFP4, tcgen05)"
+            return "dense products (MXFP4, tcgen05)"
         if name == "tl_gemm_skinny_grouped":
             return "experts gate/up + SwiGLU (register-only)" if args[11] else "experts down (register-only)"
         return {"tl_gemm_skinny_mma": "dense products (register-only)", "tl_gemm_skinny_mma_runs": "dense products (register-only)",
@@ -370,6 +379,10 @@ class LaunchTimer:
                 "tl_paged_attention_mma": "attention", "tl_paged_attention_tc": "attention",
                 "tl_paged_attention_split": "attention", "tl_paged_attention_simt": "attention",
                 "tl_attention_join": "attention join", "tl_qk_prepare": "q/k norm + rotary + cache write",
+                "tl_mxfp4_few": "dense products (MXFP4, few rows)", "tl_mxfp4_experts_first": "experts gate/up + activation (MXFP4, few rows)",
+                "tl_mxfp4_experts_second": "experts down + combine (MXFP4, few rows)", "tl_mxfp4_plan": "routing plan",
+                "tl_mxfp4_gather": "rows into expert order", "tl_mxfp4_sum": "expert combine", "tl_mxfp4_quantize": "weights to MXFP4",
+                "tl_mxfp4_values": "weights from MXFP4",
                 "tl_moe_plan": "routing plan", "tl_gather_rows": "rows into expert order", "tl_short_conv": "short conv",
                 "tl_short_conv_decode": "short conv", "tl_short_conv_state": "short conv", "tl_embed_rows": "embedding",
                 "tl_gemm_simt": "32-bit products", "tl_gemm_simt_grouped": "32-bit expert products",
@@ -438,7 +451,8 @@ def mixed_serving(cfg, model_name: str, a) -> int:
     requests, longest, new_tokens, budget_tokens = a.requests, a.longest, a.new_tokens, a.budget_tokens
     engine = Engine.from_config(cfg, seed=0, args=EngineArgs(
         dtype=a.dtype, max_len=longest + new_tokens + 16, parallel=requests, block_size=16, kv_blocks=budget_tokens // 16,
-        max_batched_tokens=2048, chunk_size=512, graph=a.graph == "on", log=a.log, record_routing=True))
+        max_batched_tokens=2048, chunk_size=512, graph=a.graph == "on", log=a.log, record_routing=True,
+        feed_forward_weights=a.feed_forward_weights))
     g = torch.Generator().manual_seed(5)
     lengths = [int(math.exp(math.log(128) + float(torch.rand(1, generator=g)) * math.log(longest / 128))) for _ in range(requests)]
     reqs = []
@@ -475,7 +489,7 @@ def mixed_serving(cfg, model_name: str, a) -> int:
                         "smallest_share_of_a_layer": round(float(share.min()), 4), "even_share": round(1.0 / cfg.num_experts, 4),
                         "experts_touched_a_layer_per_step": {"min": round(min(touched), 2), "median": round(statistics.median(touched), 2),
                                                              "max": round(max(touched), 2)}},
-        "dtype": "bf16" if a.dtype == "bfloat16" else "fp32", "data": "synthetic: random weights, uniform random token ids"}))
+        "dtype": dtype_label(a), "data": "synthetic: random weights, uniform random token ids"}))
     return 0
 
 
@@ -1405,6 +1419,8 @@ def main() -> int:
                     + " (niralix) or " + ", ".join(GIFOPEL_SIZES) + " (gifopel) or " + ", ".join(DIPIVIK_SIZES)
                     + " (dipivik) (default: all)")
     a = ap.parse_args()
+    if a.feed_forward_weights != "stored" and (a.design or a.impl == "reference"):
+        ap.error("--feed-forward-weights: the design comparisons and the reference run stored weights")
     if a.impl == "reference":
         return reference_arm(a)
     if a.design:
@@ -1639,7 +1655,7 @@ def main() -> int:
             if ms:
                 pre[f"= {key}, all forms"] = {"ms": round(ms, 4), "flops": flops[key], "TFLOPs": round(flops[key] / ms / 1e9, 1),
                                               "frac_bf16_burst": round(flops[key] / ms / 1e9 / pk["bf16_tflops"], 4)}
-        print(json.dumps({"profile_table": {"model": model_name, "layers": a.layers, "dtype": a.dtype, "batch": a.batch,
+        print(json.dumps({"profile_table": {"model": model_name, "layers": a.layers, "dtype": dtype_label(a), "batch": a.batch,
                                             "context": a.context, "peaks": pk,
                                             "decode_step": {"eager_ms": round(eager_ms, 4), "sum_of_launches_ms": round(total, 4),
                                                             "families": decode},
@@ -1674,7 +1690,7 @@ def main() -> int:
         "value": round(main_run["tok_s"], 1), "unit": "tok/s", "n_gpus": 1, "steps": a.steps, "warmup": a.warmup,
         "ms_per_step": round(main_run["ms_per_step"], 4), "higher_is_better": True, "scaling": "weak",
         "vs_baseline": None,
-        "dtype": ("bf16" if bf16 else "fp32") + ("" if a.feed_forward_weights == "stored" else ", feed-forward weights mxfp4"),
+        "dtype": dtype_label(a),
         "data": "synthetic: random weights N(0, 0.02), uniform random token ids, random keys and values as context",
         "impl": "ours", "repeats": REPEATS, "regions_ms": main_run["regions_ms"],
         "config": {"model": model_name, "layers": a.layers, "layers_of_model": layers_of_model,
