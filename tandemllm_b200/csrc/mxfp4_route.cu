@@ -41,8 +41,8 @@ __device__ __forceinline__ long long before_me(long long v, long long* scratch, 
 
 // One block. Pairs of an expert lie together, in any order among themselves: a row's products do not depend on the rows beside it, so the
 // order, which the atomics leave open, changes no result. Pairs without an expert come last and are in no tile.
-__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* ids, int pairs, int experts, int tile_rows_at_most, int* counts, int* sorted,
-                                                            int* place, int* tile_group, int* tile_row0, int* tile_rows, int* n_tiles, int* status) {
+__global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* ids, int pairs, int experts, int tile_rows_at_most, int* sorted, int* place,
+                                                            int* tile_group, int* tile_row0, int* tile_rows, int* n_tiles, int* status) {
   __shared__ int at[PLAN_EXPERTS + 1];
   __shared__ long long scratch[33];
   chain_next();
@@ -79,7 +79,6 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* ids, int 
   const long long before = before_me((long long)mine << 32 | tiles, scratch, total);
   const int first = (int)(before >> 32), first_tile = (int)(before & 0x7FFFFFFF), all = (int)(total >> 32), all_tiles = (int)(total & 0x7FFFFFFF);
   if (tid < experts) {
-    counts[tid] = mine;
     at[tid] = first;
     for (int t = 0; t < tiles; ++t) {
       tile_group[first_tile + t] = tid;
@@ -169,13 +168,13 @@ __global__ void __launch_bounds__(256) sum_kernel(const float* y, long long ldy,
 
 using namespace tl;
 
-extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_rows_at_most, int* counts, int* sorted, int* place, int* tile_group,
-                             int* tile_row0, int* tile_rows, int* n_tiles, int* status, cudaStream_t stream) {
+extern "C" int tl_mxfp4_plan(const int* ids, int pairs, int experts, int tile_rows_at_most, int* sorted, int* place, int* tile_group, int* tile_row0,
+                             int* tile_rows, int* n_tiles, int* status, cudaStream_t stream) {
   if (pairs == 0) return 0;
   TL_REQUIRE(pairs > 0 && pairs <= 1 << 30 && experts >= 1 && experts <= mx::PLAN_EXPERTS && tile_rows_at_most >= 1,
              "mxfp4 experts: %d pairs of %d experts", pairs, experts);
-  return mx::launch_behind(false, mx::plan_kernel, dim3(1), mx::PLAN_THREADS, 0, stream, ids, pairs, experts, tile_rows_at_most, counts, sorted,
-                             place, tile_group, tile_row0, tile_rows, n_tiles, status);
+  return mx::launch_behind(false, mx::plan_kernel, dim3(1), mx::PLAN_THREADS, 0, stream, ids, pairs, experts, tile_rows_at_most, sorted, place,
+                             tile_group, tile_row0, tile_rows, n_tiles, status);
 }
 
 // to [rows, width] bfloat16 (row stride ld_to, a multiple of 8, 16-byte aligned) from x (row stride ldx): row i is x[order[i] / div], or x[i].

@@ -42,7 +42,7 @@ struct TcParams {
   int M, N, K;                // tokens, outputs, reduction length
   int matrices;               // matrices a group: 1, or 2 where gate and up matrix come in turn
   int tiles_a_split;          // tiles of 128 k a CTA of a cluster takes
-  const int* tile_group;      // grouped (or null): per token tile its group, first row and rows; tiles past *n_tiles leave
+  const int* tile_group;      // grouped, persistent (or null): per token tile its group, first row and rows, `*n_tiles` of them
   const int* tile_row0;
   const int* tile_rows;
   const int* n_tiles;
@@ -316,17 +316,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
   using S = Tc<BN>;
   constexpr int OUTS = GATED ? ROWS / 2 : ROWS;
   chain_wait();
-  int tok0, tok_rows, group = 0;
-  if (p.tile_group) {
-    const int t = blockIdx.y;
-    if (t >= *p.n_tiles) return;
-    tok0 = p.tile_row0[t];
-    tok_rows = min(p.tile_rows[t], BN);
-    group = p.tile_group[t];
-  } else {
-    tok0 = blockIdx.y * BN;
-    tok_rows = min(BN, p.M - tok0);
-  }
+  const int tok0 = blockIdx.y * BN, tok_rows = min(BN, p.M - tok0);
   const int n0 = blockIdx.x * OUTS;
   const int k_tiles = ceil_div(p.K, TILE_K);
   const int tile0 = SPLIT ? (int)blockIdx.z * p.tiles_a_split : 0;              // first tile of 128 k
@@ -416,7 +406,7 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
     const int eight = r >> 3, row_tiles = ceil_div(p.N, TILE_ROWS);
     const int row_tile = (n0 >> 3) + (GATED ? eight >> 1 : eight);
     const bool valid = row_tile < row_tiles;
-    const long long first = (((long long)group * p.matrices + (GATED ? eight & 1 : 0)) * row_tiles + (valid ? row_tile : 0)) * k_tiles + tile0;
+    const long long first = ((GATED ? (long long)(eight & 1) * row_tiles : 0) + (valid ? row_tile : 0)) * k_tiles + tile0;
     const uint8_t* codes = p.codes + first * TILE_CODES + (r & 7) * (TILE_K / 2);
     const uint8_t* scales = p.scales + first * TILE_SCALES + (r & 7) * (TILE_K / BLOCK);
     constexpr int AHEAD = 2;                                    // tiles of codes a thread has at hand or on their way
@@ -462,34 +452,29 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
         if constexpr (SPLIT) {
 #pragma unroll
           for (int j = 0; j < 16; ++j) part[(c0 + j) * ROWS + r] = v[j];
-          continue;
-        }
-        if (p.row_weight) {
-          const float w = (lane & 15) < left ? weight_of(p, (long long)tok0 + c0 + (lane & 15)) : 1.f;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) v[j] *= __shfl_sync(0xffffffffu, w, j);
-        }
-#pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] += bias;
-        if constexpr (GATED) {
-          // of two tokens the lane with the gate row finishes the first and the one with the up row the second
-#pragma unroll
-          for (int j = 0; j < 16; j += 2) {
-            const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 8);
-            const float out = gated(up ? other : v[j], up ? v[j + 1] : other, p.act, p.ga0, p.ga1);
-            const int m = up ? j + 1 : j;
-            if (mine && m < left) store_one(C + (long long)(tok0 + c0 + m) * p.ldc + n, out);
-          }
         } else {
-          if (p.act < 0) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) v[j] = gate_activation(v[j], -p.act);
-          }
-          if (mine) {
-            TOut* to = C + (long long)(tok0 + c0) * p.ldc + n;
+          for (int j = 0; j < 16; ++j) v[j] += bias;
+          if constexpr (GATED) {
+            // of two tokens the lane with the gate row finishes the first and the one with the up row the second
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              if (j < left) store_one(to + (long long)j * p.ldc, v[j]);
+            for (int j = 0; j < 16; j += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 8);
+              const float out = gated(up ? other : v[j], up ? v[j + 1] : other, p.act, p.ga0, p.ga1);
+              const int m = up ? j + 1 : j;
+              if (mine && m < left) store_one(C + (long long)(tok0 + c0 + m) * p.ldc + n, out);
+            }
+          } else {
+            if (p.act < 0) {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) v[j] = gate_activation(v[j], -p.act);
+            }
+            if (mine) {
+              TOut* to = C + (long long)(tok0 + c0) * p.ldc + n;
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                if (j < left) store_one(to + (long long)j * p.ldc, v[j]);
+            }
           }
         }
       }
@@ -511,10 +496,6 @@ __global__ void __launch_bounds__(THREADS, 2) tc_kernel(const __grid_constant__ 
           for (int s = 0; s < ranks; ++s) {
             v += load_from(part + m * ROWS + r, s);
             if (GATED) u += load_from(part + m * ROWS + r + 8, s);
-          }
-          if (p.row_weight) {
-            const float w = weight_of(p, (long long)tok0 + m);
-            v *= w, u *= w;
           }
           if (p.bias) {
             v += p.bias[n];
@@ -958,7 +939,7 @@ int launch_tc(const CUtensorMap& tmX, const TcParams& p, dim3 grid, cudaStream_t
 
 using namespace tl;
 
-// x [x_rows, K] bfloat16 (row stride ldx); the matrix N x K, or with `matrices` 2 a gate and an up matrix; grouped (tile_group ...): as many for
+// x [x_rows, K] bfloat16 (row stride ldx); the matrix N x K, or gated a gate and an up matrix; grouped (tile_group ..., `splits` 0): as many for
 // every group, x in the plan's order, tiles of at most `bn` rows. bias [N] (gated: [2 N]) 32-bit or null. out [M, N] (row stride ldc). `act`
 // as in tl_mxfp4_few. `splits` 0: the persistent form, in
 // tiles of up to `bn` <= 256 token rows; else token tiles of `bn` rows, 16, 32, 64 or 128, and the CTAs, 1 to 8, that share a tile's k.
@@ -974,6 +955,9 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
   const int k_tiles = ceil_div(K, mx::TILE_K);
   TL_REQUIRE(splits >= 0 && splits <= mx::MAX_SPLITS && splits <= k_tiles, "mxfp4 product: k %d in %d runs", K, splits);
   TL_REQUIRE(!tile_group || (tile_row0 && tile_rows && n_tiles), "mxfp4 product: an incomplete plan (%d tiles)", max_tiles);
+  TL_REQUIRE((!tile_group && !row_weight) || (tile_group && splits == 0), "mxfp4 product: groups and rows' weights in %d runs of k; the persistent form "
+             "alone has them", splits);
+  TL_REQUIRE(splits == 0 || bn == 16 || bn == 32 || bn == 64 || bn == 128, "mxfp4 product: token tiles of %d rows; 16, 32, 64 or 128", bn);
   mx::TcParams p = {};
   p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.bias = bias, p.C = out, p.ldc = ldc, p.M = M, p.N = N, p.K = K;
   p.matrices = act > 0 ? 2 : 1;
@@ -1003,7 +987,7 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
     TL_MX_MANY(256);
 #undef TL_MX_MANY
   }
-  const dim3 grid(ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS), tile_group ? max_tiles : ceil_div(M, bn), splits);
+  const dim3 grid(ceil_div(N, act > 0 ? mx::ROWS / 2 : mx::ROWS), ceil_div(M, bn), splits);
   TL_REQUIRE(grid.y <= 65535, "mxfp4 product: %d token tiles exceed the grid limit", (int)grid.y);
   CUtensorMap tmX;
   const int r = tensor_map(x, x_rows, K, ldx, bn, &tmX);
@@ -1022,7 +1006,6 @@ extern "C" int tl_mxfp4_tc(const void* x, long long ldx, long long x_rows, const
   if (bn == 16) TL_MX_TC(16);
   if (bn == 32) TL_MX_TC(32);
   if (bn == 64) TL_MX_TC(64);
-  TL_REQUIRE(bn == 128, "mxfp4 product: token tiles of %d rows; 16, 32, 64 or 128", bn);
   TL_MX_TC(128);
 #undef TL_MX_TC
 #undef TL_MX_TC_

@@ -46,7 +46,7 @@ _SIGNATURES = {
                                 c_void_p, c_void_p],
     "tl_mxfp4_tc": [c_void_p, c_longlong, c_longlong, c_void_p, c_void_p, c_void_p, c_void_p, c_longlong, c_int, c_int, c_int, c_int, c_float,
                     c_float, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p],
-    "tl_mxfp4_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
+    "tl_mxfp4_plan": [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
     "tl_mxfp4_gather": [c_void_p, c_longlong, c_void_p, c_int, c_void_p, c_longlong, c_int, c_int, c_void_p],
     "tl_mxfp4_sum": [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p],
 }
@@ -343,13 +343,12 @@ def _sorted(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first,
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
     tile = 64 if pairs <= 48 * E else 160
     tiles = min(pairs // tile + E, pairs)
-    ints = x.new_empty(E + 2 * pairs + 3 * tiles + 1, dtype=torch.int32)
-    counts = ints.data_ptr()
-    order = counts + 4 * E
+    ints = x.new_empty(2 * pairs + 3 * tiles + 1, dtype=torch.int32)
+    order = ints.data_ptr()
     place = order + 4 * pairs
     group, row0, n_rows = (place + 4 * (pairs + i * tiles) for i in range(3))
     n_tiles = n_rows + 4 * tiles
-    _check(lib().tl_mxfp4_plan(ids.data_ptr(), pairs, E, tile, counts, order, place, group, row0, n_rows, n_tiles, status, stream), "mxfp4_plan")
+    _check(lib().tl_mxfp4_plan(ids.data_ptr(), pairs, E, tile, order, place, group, row0, n_rows, n_tiles, status, stream), "mxfp4_plan")
     xs, ld = _boxed(x, pairs, w_first.k, ld, order, top)
     wide = -(-inter // 8) * 8
     a = x.new_empty(pairs, wide)
@@ -360,7 +359,7 @@ def _sorted(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first,
     _check(lib().tl_mxfp4_tc(a.data_ptr(), wide, pairs, w_down.codes, w_down.scales, None, y.data_ptr(), hidden, pairs, hidden, inter, 0, 0.0, 0.0,
                              ops.FP32, *tail, None, None, status, stream), "mxfp4_tc")
     if defer:
-        return ops.ExpertRows(y, ints[E + pairs:E + 2 * pairs], ids, None if before else wts)
+        return ops.ExpertRows(y, ints[pairs:2 * pairs], ids, None if before else wts)
     out = x.new_empty(rows, hidden, dtype=dtype)
     _check(lib().tl_mxfp4_sum(y.data_ptr(), place, ids.data_ptr(), None if before else w, out.data_ptr(), ops.dtype_code(dtype), rows, hidden, top,
                               E, stream), "mxfp4_sum")
