@@ -202,9 +202,10 @@ def _vector(v: torch.Tensor | None, size: int, name: str, index: int) -> int | N
 def _output(out, rows: int, n: int, dtype: torch.dtype, x: torch.Tensor) -> torch.Tensor:
     if out is None:
         return x.new_empty(rows, n, dtype=dtype)
-    if tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != x.device or (out.stride(1) != 1 and n > 1):
-        raise ops.KernelError(f"mxfp4 product: an output of {out.dtype} {tuple(out.shape)} on {out.device}; {dtype} ({rows}, {n}) with unit inner "
-                              f"stride on {x.device}")
+    if tuple(out.shape) != (rows, n) or out.dtype != dtype or out.device != x.device or (out.stride(1) != 1 and n > 1) or \
+            (out.stride(0) < n and rows > 1):
+        raise ops.KernelError(f"mxfp4 product: an output of {out.dtype} {tuple(out.shape)}, strides {out.stride()}, on {out.device}; {dtype} ({rows}, "
+                              f"{n}) with unit inner stride, a row behind the other, on {x.device} is wanted")
     return out
 
 
@@ -261,7 +262,7 @@ def _product(runtime, x, rows: int, ld: int, w: Mxfp4Matrix, bias: int | None, o
 def linear(runtime, x: torch.Tensor, w: Mxfp4Matrix, bias: torch.Tensor | None = None, out_dtype: torch.dtype | None = None,
            out: torch.Tensor | None = None, act: str | int | None = None) -> torch.Tensor:
     """x [rows, k] times the one matrix w [n, k], plus `bias` (32-bit, [n]), through the activation `act` (silu, gelu, relu2 or identity, by
-    name or code; None: as it is), in `out_dtype` (default: `out`'s, else x's)."""
+    name or code; None: as it is), in `out_dtype` (default: `out`'s, else x's). `out`, where it is given, shares no memory with the inputs."""
     if w.groups != 1:
         raise ops.KernelError(f"mxfp4 product: a stack of {w.groups} matrices where one is wanted")
     rows, ld = _rows(runtime, x, w)
