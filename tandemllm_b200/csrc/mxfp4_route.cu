@@ -45,8 +45,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(const int* ids, int 
                                                             int* tile_group, int* tile_row0, int* tile_rows, int* n_tiles, int* status) {
   __shared__ int at[PLAN_EXPERTS + 1];
   __shared__ long long scratch[33];
+  chain_wait();               // (first: what comes behind takes tensor memory before it waits, so nothing in front of the layer may still need any)
   chain_next();
-  chain_wait();
   const int tid = threadIdx.x;
   // Eight ids a thread at once, on their way together; up to 8192 pairs they stay for the second pass. -1: none, else what names no expert is `experts`.
   constexpr int HELD = 8;

@@ -34,3 +34,10 @@ def test_the_next_kernel_comes_when_this_one_has_its_tensor_memory():
         assert taken < body.index("chain_next();"), kernel
         found += 1
     assert found == 2
+
+
+def test_a_layer_of_experts_begins_when_everything_in_front_of_it_has_ended():
+    """With all launches chained, the products behind the plan would else take tensor memory while a kernel in front of the plan, that has yet
+    to take its own, waits."""
+    body = kernels("mxfp4_route.cu")["plan_kernel"][1]
+    assert body.index("chain_wait();") < body.index("chain_next();")
