@@ -34,9 +34,8 @@ constexpr int GROUPS = 4;
 constexpr int GROUP_WARPS = 4;
 constexpr int WARPS = GROUPS * GROUP_WARPS;           // that multiply; a group has one more that copies and one that finishes
 constexpr int THREADS = (WARPS + 2 * GROUPS) * 32;
-constexpr int MAX_TOKENS = 16;
 constexpr int MAX_PAIRS = 256;                        // of the experts' form
-constexpr int MAX_ROWS = 8;
+constexpr int MAX_ROWS = 8;                           // token rows: the N side of the MMA
 
 // Token rows in shared memory: a row's length is 64 modulo 128 bytes, so that the 16 bytes of eight lanes (two rows, four quarters of a
 // block) fall on all banks. Eight numbers lie as the codes' conversion leaves theirs: 0 2, 4 6, 1 3, 5 7. (64 bits: it is asked of any length.)
@@ -66,17 +65,13 @@ __device__ __forceinline__ int row_exponent(uint32_t top) { return max((int)(top
 __device__ __forceinline__ float to_half(uint32_t top) { return power(14 - row_exponent(top)); }
 __device__ __forceinline__ float from_half(uint32_t top) { return power(row_exponent(top) - 15); }
 
-// acc[j] += 16 weight rows by 128 k times the token rows of every tile j of eight. `lo` and `hi`: a lane's words of the four blocks in row g and
-// in row g + 8; `s_lo` and `s_hi` these rows' scales.
-template <int NT>
-__device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4& lo4, const uint4& hi4, uint32_t s_lo, uint32_t s_hi,
-                                         const uint8_t* const (&rows)[NT], int at) {
+// acc += 16 weight rows by 128 k times eight token rows. `lo` and `hi`: a lane's words of the four blocks in row g and in row g + 8; `s_lo` and `s_hi`
+// these rows' scales.
+__device__ __forceinline__ void multiply(float (&acc)[4], const uint4& lo4, const uint4& hi4, uint32_t s_lo, uint32_t s_hi, const uint8_t* row) {
   const uint32_t lo[4] = {lo4.x, lo4.y, lo4.z, lo4.w}, hi[4] = {hi4.x, hi4.y, hi4.z, hi4.w};
-  uint4 x[4][NT];
+  uint4 x[4];
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
-#pragma unroll
-    for (int j = 0; j < NT; ++j) x[b][j] = *reinterpret_cast<const uint4*>(rows[j] + at + 64 * b);
+  for (int b = 0; b < 4; ++b) x[b] = *reinterpret_cast<const uint4*>(row + 64 * b);
   // two blocks side by side: an MMA's sum is there 30 cycles later
 #pragma unroll
   for (int b0 = 0; b0 < 4; b0 += 2) {
@@ -86,25 +81,18 @@ __device__ __forceinline__ void multiply(float (&acc)[NT][4], const uint4& lo4, 
       values16(lo[b0 + b], u[b]);
       values16(hi[b0 + b], v[b]);
     }
-    float c[2][NT][4];
+    float c[2][4];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+    for (int b = 0; b < 2; ++b) mma_16816_first(c[b], u[b][0], v[b][0], u[b][1], v[b][1], x[b0 + b].x, x[b0 + b].y);
 #pragma unroll
-      for (int j = 0; j < NT; ++j) mma_16816_first(c[b][j], u[b][0], v[b][0], u[b][1], v[b][1], x[b0 + b][j].x, x[b0 + b][j].y);
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) mma_16816(c[b][j], u[b][2], v[b][2], u[b][3], v[b][3], x[b0 + b][j].z, x[b0 + b][j].w);
+    for (int b = 0; b < 2; ++b) mma_16816(c[b], u[b][2], v[b][2], u[b][3], v[b][3], x[b0 + b].z, x[b0 + b].w);
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
       const float f_lo = scale32(s_lo, b0 + b), f_hi = scale32(s_hi, b0 + b);
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        acc[j][0] = fmaf(c[b][j][0], f_lo, acc[j][0]);
-        acc[j][1] = fmaf(c[b][j][1], f_lo, acc[j][1]);
-        acc[j][2] = fmaf(c[b][j][2], f_hi, acc[j][2]);
-        acc[j][3] = fmaf(c[b][j][3], f_hi, acc[j][3]);
-      }
+      acc[0] = fmaf(c[b][0], f_lo, acc[0]);
+      acc[1] = fmaf(c[b][1], f_lo, acc[1]);
+      acc[2] = fmaf(c[b][2], f_hi, acc[2]);
+      acc[3] = fmaf(c[b][3], f_hi, acc[3]);
     }
   }
 }
@@ -242,8 +230,8 @@ __host__ __device__ __forceinline__ int stage_bytes(int slice) { return 2 * slic
 // Dynamic shared memory: token rows (SECOND: and one of zeros), rings, two sets of the warps' sums, barriers (full and empty ones of the rings,
 // of the sums two each a group, and one of SECOND's rows), the rows' largest numbers.
 __host__ __device__ __forceinline__ long long rows_bytes(Kind kind, int m, int k_tiles) { return (m + (kind == SECOND ? 1 : 0)) * row_bytes(k_tiles); }
-inline long long few_bytes(Kind kind, int nt, int m, int k_tiles, int slice, int stages) {
-  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (8 * nt + 1) * 4 + (GROUPS * (2 * stages + 4) + 1) * 8 +
+inline long long few_bytes(Kind kind, int m, int k_tiles, int slice, int stages) {
+  return rows_bytes(kind, m, k_tiles) + GROUPS * stages * stage_bytes(slice) + 2 * WARPS * 16 * (MAX_ROWS + 1) * 4 + (GROUPS * (2 * stages + 4) + 1) * 8 +
          m * 4;
 }
 
@@ -272,9 +260,9 @@ __device__ __forceinline__ uint4 load_piece(const bf16* row, int k, int K, bool 
   return v;
 }
 
-template <int NT, bool GATED, Kind KIND, bool ALIGNED, typename TOut>
+template <bool GATED, Kind KIND, bool ALIGNED, typename TOut>
 __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
-  constexpr int OUTS = GATED ? 8 : 16, COLS = 8 * NT;
+  constexpr int OUTS = GATED ? 8 : 16, COLS = MAX_ROWS;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ typename Place<KIND>::Type place;
   __shared__ int aborted_;
@@ -523,31 +511,27 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
   const unsigned lane_codes = lane * 16;
   int it = 0, nth = 0;
   for (int unit = first_unit; unit < units; unit += teams, ++nth) {
-    float acc[NT][4] = {};
+    float acc[4] = {};
     bool ok = true;
     for (int sl = member; sl < slices; sl += p.team, ++it) {
       const int item = KIND == SECOND ? sl / parts : 0, tile0 = (sl - (KIND == SECOND ? item * parts : 0)) * p.slice;
       const int n = min(p.slice, k_tiles - tile0), s = it % p.stages;
       const uint8_t* from = ring + s * one_stage;
-      const uint8_t* rows[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        int m = min(j * 8 + g, p.M - 1);
-        if (KIND == SECOND) {
-          const int pair = items->pair[item][g];
-          m = pair >= 0 ? pair : p.M;
-        }
-        rows[j] = xs + m * x_bytes + tile0 * (TILE_K * 2) + t * 16;
+      int m = min(g, p.M - 1);
+      if (KIND == SECOND) {
+        const int pair = items->pair[item][g];
+        m = pair >= 0 ? pair : p.M;
       }
+      const uint8_t* row = xs + m * x_bytes + tile0 * (TILE_K * 2) + t * 16;
       ok = __all_sync(0xffffffffu, !*aborted && mbar_wait(&full[s * GROUPS + group], (it / p.stages) & 1));
       if (!ok) break;
-      float sum[NT][4] = {};
+      float sum[4] = {};
       for (int c = (w + it) & (GROUP_WARPS - 1); c < n; c += GROUP_WARPS) {
         const uint8_t* codes = from + c * TILE_CODES + lane_codes;
         const uint8_t* scales = from + p.slice * 2 * TILE_CODES + c * TILE_SCALES + g * 4;
-        multiply<NT>(KIND == SECOND ? sum : acc, *reinterpret_cast<const uint4*>(codes), *reinterpret_cast<const uint4*>(codes + p.slice * TILE_CODES),
-                     *reinterpret_cast<const uint32_t*>(scales), *reinterpret_cast<const uint32_t*>(scales + p.slice * TILE_SCALES), rows,
-                     c * (TILE_K * 2));
+        multiply(KIND == SECOND ? sum : acc, *reinterpret_cast<const uint4*>(codes), *reinterpret_cast<const uint4*>(codes + p.slice * TILE_CODES),
+                 *reinterpret_cast<const uint32_t*>(scales), *reinterpret_cast<const uint32_t*>(scales + p.slice * TILE_SCALES),
+                 row + c * (TILE_K * 2));
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&empty[s * GROUPS + group]);
@@ -557,8 +541,8 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
           const int pair = items->pair[item][2 * t + c];
           if (pair >= 0) {
             const float f = from_half(tops[pair]);
-            acc[0][c] = fmaf(sum[0][c], f, acc[0][c]);
-            acc[0][c + 2] = fmaf(sum[0][c + 2], f, acc[0][c + 2]);
+            acc[c] = fmaf(sum[c], f, acc[c]);
+            acc[c + 2] = fmaf(sum[c + 2], f, acc[c + 2]);
           }
         }
       }
@@ -571,13 +555,10 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const FewParams p) {
       break;
     }
     float (&mine)[16][COLS + 1] = part[buffer][warp];
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      mine[g][8 * j + 2 * t] = acc[j][0];
-      mine[g][8 * j + 2 * t + 1] = acc[j][1];
-      mine[g + 8][8 * j + 2 * t] = acc[j][2];
-      mine[g + 8][8 * j + 2 * t + 1] = acc[j][3];
-    }
+    mine[g][2 * t] = acc[0];
+    mine[g][2 * t + 1] = acc[1];
+    mine[g + 8][2 * t] = acc[2];
+    mine[g + 8][2 * t + 1] = acc[3];
     __syncwarp();
     if (lane == 0) mbar_arrive(&summed[buffer * GROUPS + team0]);
   }
@@ -600,12 +581,12 @@ constexpr int few_dynamic(mx::Kind kind) { return FEW_SMEM - (kind == mx::DENSE 
 
 // Tiles a stage and stages a ring that fit beside the token rows, or false. Stages of 16 tiles where a slice is as long, so that a wait and an
 // arrival serve four tiles a warp, else of 8 or 4.
-bool few_fits(mx::Kind kind, int nt, int m, int k_tiles, mx::FewParams& p) {
+bool few_fits(mx::Kind kind, int m, int k_tiles, mx::FewParams& p) {
   const int share = kind == mx::SECOND ? k_tiles : ceil_div(k_tiles, p.team);
   for (int slice = 16; slice >= 4; slice /= 2) {
     if (slice > 4 && slice / 2 >= share) continue;
     for (int stages = 6; stages >= 2; --stages)
-      if (mx::few_bytes(kind, nt, m, k_tiles, slice, stages) <= few_dynamic(kind) && (stages <= 3 || stages * slice <= 32)) {
+      if (mx::few_bytes(kind, m, k_tiles, slice, stages) <= few_dynamic(kind) && (stages <= 3 || stages * slice <= 32)) {
         p.slice = slice, p.stages = stages;
         return true;
       }
@@ -614,7 +595,7 @@ bool few_fits(mx::Kind kind, int nt, int m, int k_tiles, mx::FewParams& p) {
 }
 
 template <auto kernel>
-int launch_few(mx::FewParams& p, mx::Kind kind, int nt, long long units, cudaStream_t stream) {
+int launch_few(mx::FewParams& p, mx::Kind kind, long long units, cudaStream_t stream) {
   p.skip = mx::skip_stage_for_test();
   static thread_local int set_on = -1;              // the device whose function has its shared memory
   int dev = 0;
@@ -626,7 +607,7 @@ int launch_few(mx::FewParams& p, mx::Kind kind, int nt, long long units, cudaStr
     set_on = dev;
   }
   const long long ctas = ceil_div64(units, mx::GROUPS / p.team);
-  const int bytes = (int)mx::few_bytes(kind, nt, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);        // (few_fits has passed it)
+  const int bytes = (int)mx::few_bytes(kind, p.M, ceil_div(p.K, mx::TILE_K), p.slice, p.stages);        // (few_fits has passed it)
   const dim3 grid((unsigned)(ctas < sm_count() ? ctas : sm_count()));
   return mx::launch_behind(kind == mx::SECOND, kernel, grid, mx::THREADS, bytes, stream, p);
 }
@@ -645,41 +626,35 @@ bool a_few(int rows, int top, int experts) {
 
 // Whether `M` rows of K elements go through the form below.
 extern "C" int tl_mxfp4_few_fits(int M, int N, int K, int act) {
-  if (M < 1 || M > mx::MAX_TOKENS || N < 1 || K < 1) return 0;
+  if (M < 1 || M > mx::MAX_ROWS || N < 1 || K < 1) return 0;
   mx::FewParams p = {};
   p.team = team_of(ceil_div(N, act > 0 ? 8 : 16));
-  return few_fits(mx::DENSE, M <= 8 ? 1 : 2, M, ceil_div(K, mx::TILE_K), p);
+  return few_fits(mx::DENSE, M, ceil_div(K, mx::TILE_K), p);
 }
 
-// x [M, K] bfloat16 (row stride ldx), M <= 16; the matrix N x K (gated: two, gate and up); bias [N] (gated: [2 N]) 32-bit or null; out [M, N]
+// x [M, K] bfloat16 (row stride ldx), M <= 8; the matrix N x K (gated: two, gate and up); bias [N] (gated: [2 N]) 32-bit or null; out [M, N]
 // (row stride ldc) bfloat16 or 32-bit. `act`: the gate's activation TL_ACT_*, 0 for a plain product, negated an activation on its results.
 extern "C" int tl_mxfp4_few(const void* x, long long ldx, const void* codes, const void* scales, const float* bias, void* out, long long ldc,
                             int M, int N, int K, int act, float a0, float a1, int out_dtype, int* status, cudaStream_t stream) {
   if (M == 0 || N == 0) return 0;
-  TL_REQUIRE(M >= 1 && M <= mx::MAX_TOKENS && N >= 1 && K >= 1, "mxfp4 product of few rows: %d rows x (%d x %d)", M, N, K);
+  TL_REQUIRE(M >= 1 && M <= mx::MAX_ROWS && N >= 1 && K >= 1, "mxfp4 product of few rows: %d rows x (%d x %d)", M, N, K);
   TL_REQUIRE(act <= 0 ? act >= -TL_ACT_IDENTITY : tl_is_gate(act), "mxfp4 product: gate activation %d is none (nor an ungated one, negated)", act);
   TL_REQUIRE(act <= 0 || out_dtype == TL_BF16, "mxfp4 product: gated outputs of type %d", out_dtype);
   mx::FewParams p = {};
   p.x = x, p.ldx = ldx, p.codes = (const uint8_t*)codes, p.scales = (const uint8_t*)scales, p.bias = bias, p.out = out, p.ldc = ldc;
   p.M = M, p.N = N, p.K = K, p.act = act, p.ga0 = a0, p.ga1 = a1, p.status = status;
   const bool aligned = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
-  const int nt = M <= 8 ? 1 : 2, units = ceil_div(N, act > 0 ? 8 : 16);
+  const int units = ceil_div(N, act > 0 ? 8 : 16);
   p.team = team_of(units);
-  TL_REQUIRE(few_fits(mx::DENSE, nt, M, ceil_div(K, mx::TILE_K), p), "mxfp4 product of few rows: %d rows of %d elements are too many", M, K);
-#define TL_FEW(NT_, G_, T_)                                                                                            \
-  do {                                                                                                                 \
-    if (aligned) return launch_few<mx::few_kernel<NT_, G_, mx::DENSE, true, T_>>(p, mx::DENSE, NT_, units, stream);    \
-    return launch_few<mx::few_kernel<NT_, G_, mx::DENSE, false, T_>>(p, mx::DENSE, NT_, units, stream);                \
+  TL_REQUIRE(few_fits(mx::DENSE, M, ceil_div(K, mx::TILE_K), p), "mxfp4 product of few rows: %d rows of %d elements are too many", M, K);
+#define TL_FEW(G_, T_)                                                                                       \
+  do {                                                                                                       \
+    if (aligned) return launch_few<mx::few_kernel<G_, mx::DENSE, true, T_>>(p, mx::DENSE, units, stream);    \
+    return launch_few<mx::few_kernel<G_, mx::DENSE, false, T_>>(p, mx::DENSE, units, stream);                \
   } while (0)
-#define TL_FEW_(NT_)                                     \
-  do {                                                   \
-    if (act > 0) TL_FEW(NT_, true, bf16);                \
-    if (out_dtype == TL_FP32) TL_FEW(NT_, false, float); \
-    TL_FEW(NT_, false, bf16);                            \
-  } while (0)
-  if (nt == 1) TL_FEW_(1);
-  TL_FEW_(2);
-#undef TL_FEW_
+  if (act > 0) TL_FEW(true, bf16);
+  if (out_dtype == TL_FP32) TL_FEW(false, float);
+  TL_FEW(false, bf16);
 #undef TL_FEW
 }
 
@@ -689,7 +664,7 @@ extern "C" int tl_mxfp4_experts_fit(int rows, int top, int K, int inter) {
   if (!a_few(rows, top, 1) || K < 1 || inter < 1) return 0;
   mx::FewParams p = {};
   p.team = 4;
-  return few_fits(mx::FIRST, 1, rows, ceil_div(K, mx::TILE_K), p) && few_fits(mx::SECOND, 1, rows * top, ceil_div(inter, mx::TILE_K), p);
+  return few_fits(mx::FIRST, rows, ceil_div(K, mx::TILE_K), p) && few_fits(mx::SECOND, rows * top, ceil_div(inter, mx::TILE_K), p);
 }
 static int between_row(int inter) { return ceil_div(inter, mx::TILE_K) * mx::TILE_K; }
 extern "C" long long tl_mxfp4_experts_between(int pairs, int inter) {
@@ -713,11 +688,11 @@ extern "C" int tl_mxfp4_experts_first(const void* x, long long ldx, const void* 
   const bool aligned = K % 8 == 0 && ldx % 8 == 0 && ((uintptr_t)x % 16) == 0;
   const long long units = (long long)p.parts * (top < experts ? top : experts);       // (at least so many)
   p.team = team_of(units);
-  TL_REQUIRE(few_fits(mx::FIRST, 1, rows, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d rows of %d elements are too many", rows, K);
+  TL_REQUIRE(few_fits(mx::FIRST, rows, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d rows of %d elements are too many", rows, K);
 #define TL_FIRST(G_)                                                                                                     \
   do {                                                                                                                   \
-    if (aligned) return launch_few<mx::few_kernel<1, G_, mx::FIRST, true, bf16>>(p, mx::FIRST, 1, units * rows, stream); \
-    return launch_few<mx::few_kernel<1, G_, mx::FIRST, false, bf16>>(p, mx::FIRST, 1, units * rows, stream);             \
+    if (aligned) return launch_few<mx::few_kernel<G_, mx::FIRST, true, bf16>>(p, mx::FIRST, units * rows, stream); \
+    return launch_few<mx::few_kernel<G_, mx::FIRST, false, bf16>>(p, mx::FIRST, units * rows, stream);             \
   } while (0)
   if (act > 0) TL_FIRST(true);
   TL_FIRST(false);
@@ -738,9 +713,9 @@ extern "C" int tl_mxfp4_experts_second(void* between, const void* codes, const v
   p.ids = ids, p.rows = rows, p.top = top, p.experts = experts, p.status = status;
   const int units = ceil_div(N, 16);
   p.team = team_of(units);
-  TL_REQUIRE(few_fits(mx::SECOND, 1, p.M, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d pairs of %d elements are too many", p.M, K);
-  if (out_dtype == TL_FP32) return launch_few<mx::few_kernel<1, false, mx::SECOND, true, float>>(p, mx::SECOND, 1, units, stream);
-  return launch_few<mx::few_kernel<1, false, mx::SECOND, true, bf16>>(p, mx::SECOND, 1, units, stream);
+  TL_REQUIRE(few_fits(mx::SECOND, p.M, ceil_div(K, mx::TILE_K), p), "mxfp4 experts: %d pairs of %d elements are too many", p.M, K);
+  if (out_dtype == TL_FP32) return launch_few<mx::few_kernel<false, mx::SECOND, true, float>>(p, mx::SECOND, units, stream);
+  return launch_few<mx::few_kernel<false, mx::SECOND, true, bf16>>(p, mx::SECOND, units, stream);
 }
 
 // For tests of the bounded waits: the polls after which a wait of this file's kernels gives up (0 puts the default back), and the stage of

@@ -9,7 +9,7 @@
 Rows are bfloat16 and every sum is 32-bit: the weights are exact in bfloat16, so a product is what the bfloat16 path would give for the
 rounded weights. The compute happens on the device of the rows, which has to be the current one, on its current stream; nothing is kept
 between calls but what the caller passes in. There is no 32-bit product: a 32-bit runtime takes the values as a plain matrix. Products of
-up to 16 rows take a row relative to its largest number: what is below 2^-31 of it loses bits, what is below 2^-39 counts as zero, and weights
+up to 8 rows take a row relative to its largest number: what is below 2^-31 of it loses bits, what is below 2^-39 counts as zero, and weights
 beyond 2^95 can make their sums infinite.
 """
 
@@ -27,8 +27,13 @@ from .build import Launchers, load
 BLOCK = 32                      # values a scale
 BYTES_A_VALUE = 17 / 32         # half a byte, and a scale's share
 TILE_ROWS, TILE_K = 8, 128      # the layout's tiles
-FEW_ROWS = 16                   # rows up to which a product goes to the register-only kernel
-EXPERT_ROWS, EXPERT_TOP = 8, 32     # rows of the experts' two-kernel form, experts a row
+# Rows up to which a product goes to the register-only kernel. Its and the tensor cores' us at 8 rows: 12000 outputs of 4096 15.3 and 16.9, 7168 gated
+# ones of 2048 9.9 and 14.2, 2048 of 2048 5.2 and 6.0, but 2048 of 7168 10.9 and 9.4. A form of it for 16 rows, which is gone, took at 12 rows 21.4
+# (17.3), 14.4 (14.1), 7.6 (6.4) and 9.6 (9.7), and was ahead only where there is little to do (1000 of 600 5.2 and 5.8).
+FEW_ROWS = 8
+# Rows up to which, and experts a row with which, a layer of experts goes to the two-kernel form. Its us and the sorted form's at 8 rows: top-4 of 32
+# experts of 1792 x 2048 46 and 65, top-6 of 64 of 768 x 2048 42 and 47, top-2 of 8 of 4096 x 2048 41 and 53; at one row 17 and 26.
+EXPERT_ROWS, EXPERT_TOP = 8, 32
 TILE_CODES, TILE_BYTES = TILE_ROWS * TILE_K // 2, TILE_ROWS * TILE_K * 17 // 32
 
 ACTIVATIONS = tuple(ops.ACTIVATIONS[a] for a in ("silu", "gelu", "relu2", "identity"))     # those a plain product may end with
