@@ -34,6 +34,10 @@ FEW_ROWS = 8
 # Rows up to which, and experts a row with which, a layer of experts goes to the two-kernel form. Its us and the sorted form's at 8 rows: top-4 of 32
 # experts of 1792 x 2048 46 and 65, top-6 of 64 of 768 x 2048 42 and 47, top-2 of 8 of 4096 x 2048 41 and 53; at one row 17 and 26.
 EXPERT_ROWS, EXPERT_TOP = 8, 32
+# Pairs an expert, on average, up to which the sorted form's tiles are of 64 rows, else of 160. Us of 64 and of 160 at 4, 16, 32 and 48 pairs: top-4 of 32
+# experts of 1792 x 2048 84 and 87, 87 and 88, 94 and 92, 99 and 94; top-6 of 64 of 768 x 2048 76 and 79, 80 and 81, 86 and 85, 97 and 90. With half of
+# the rows at one expert the same to 3 us (up to 24 pairs; at 64 116 and 100).
+LOW_PAIRS = 20
 TILE_CODES, TILE_BYTES = TILE_ROWS * TILE_K // 2, TILE_ROWS * TILE_K * 17 // 32
 
 ACTIVATIONS = tuple(ops.ACTIVATIONS[a] for a in ("silu", "gelu", "relu2", "identity"))     # those a plain product may end with
@@ -347,7 +351,7 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_f
 def _sorted(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first, w_down, act: int, before: bool, constants, dtype, defer):
     """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
-    tile = 64 if pairs <= 48 * E else 160
+    tile = 64 if pairs <= LOW_PAIRS * E else 160
     tiles = min(pairs // tile + E, pairs)
     ints = x.new_empty(2 * pairs + 3 * tiles + 1, dtype=torch.int32)
     order = ints.data_ptr()
