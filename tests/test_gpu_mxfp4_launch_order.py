@@ -58,3 +58,19 @@ def test_routed_layers_behind_the_router_that_writes_their_ids(runtime, chained,
     got = layers()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert int(runtime.status.item()) == 0
+
+
+@pytest.mark.parametrize("name", ["c", "d"])
+def test_a_model_with_all_launches_chained(chained, name):
+    from tests import test_gpu_mxfp4_models as models
+    from tests import test_gpu_puripel as puripel
+    from tests import tiny_configs as T
+    cfg, spec, W = models.lfm2(name)
+    requests = {"a": T.long_tokens(name, 100), "b": T.long_tokens(name, 31, seed=8)}
+    schedule = [[("a", 64), ("b", 1)], [("a", 9), ("b", 20)], [("a", 2), ("b", 3)]] + [[("a", 1), ("b", 1)]] * 7 + [[("a", 18)]]
+    engine = models.engine_on(spec, W, "bfloat16")
+    want = puripel.run_schedule(engine, requests, schedule)
+    chained(1)
+    for _ in range(3):
+        got = puripel.run_schedule(engine, requests, schedule)
+        assert all(torch.equal(got[r], want[r]) for r in requests)
