@@ -4,6 +4,9 @@
 //   FIRST   the experts' first half for up to 8 rows: a[p] = act(G_e x) * (U_e x) of every (row, slot) pair p, times the pair's weight
 //   SECOND  their second half: out[r] = sum over r's pairs of D_e a[p], all experts in one sum
 //
+// a[p] is rounded to bfloat16 between the halves, as the bfloat16 path's rows are: in 32 bits a step's rows would not fit shared memory beside the
+// weights' stages, and a layer's result, which is rounded to bfloat16 itself (1.7e-3 of it), is off by 2.3e-3 so.
+//
 // Such a product reads every weight once and does little with it: its bounds are the weights' stream and their conversion. Codes become float16
 // numbers two at a time by a conversion of the GPU's, and a block's 32 products are two mma.sync m16n8k16 whose sum joins the others times the block's
 // scale, in 32 bits. (As bfloat16 numbers made of bits and times their scale, a word of eight codes takes 32 cycles of a scheduler with its MMA;

@@ -256,13 +256,15 @@ __device__ __forceinline__ void convert(const RowTile& q, uint32_t (&v)[32]) {
   }
 }
 
-// A tile's values to a stage of tensor memory, once the products of the tile that had it (`before`; negative: none) are done; `then` runs when
-// the tile's codes are used up. False where the wait ran out or somebody gave up.
+// A box from (x, y) where `one` is true: predicated, because behind a branch the operands would be made uniform first (see `elected`).
 __device__ __forceinline__ void tma_load_if(bool one, void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y) {
   asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %5, 0;\n\t"
       "@p cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n\t}"
       ::"r"(smem_u32(dst)), "l"(map), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"((int)one) : "memory");
 }
+
+// A tile's values to a stage of tensor memory, once the products of the tile that had it (`before`; negative: none) are done; `then` runs when
+// the tile's codes are used up. False where the wait ran out or somebody gave up.
 template <typename Then>
 __device__ __forceinline__ bool give_tile(uint32_t taddr, const RowTile& q, uint64_t* full, uint64_t* done, int before, volatile uint32_t* aborted,
                                           Then then) {

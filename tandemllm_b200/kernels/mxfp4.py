@@ -225,10 +225,10 @@ def shape_of(rows: int, row_tiles: int, k: int, sms: int, gated: bool) -> tuple[
 
     The form with the smallest estimated time, in us: `blocks` (of 128 k) one after the other in every round of CTAs, each as long as its
     weights take to convert or, persistent, as its tokens take to multiply; a round's start and end; and, where CTAs share a tile's k, adding
-    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows; over these the choice is 1.1 % slower than the
-    fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14 us in one persistent tile, 18 where two CTAs share
-    its k; 2048 rows 92 in tiles of 160, 106 in tiles of 192. At 2048 outputs of 7168: 256 rows 17 with eight CTAs a tile, 29 without;
-    700 rows 30 without, 35 with two."""
+    their sums. The numbers are fitted to 2800 timings of 8 products with 17 to 4096 rows (9 to 16 take what they give); over these the
+    choice is 1.1 % slower than the fastest form on average. What decides, at 7168 gated outputs of 2048: 100 rows 14 us in one persistent
+    tile, 18 where two CTAs share its k; 2048 rows 92 in tiles of 160, 106 in tiles of 192. At 2048 outputs of 7168: 256 rows 17 with
+    eight CTAs a tile, 29 without; 700 rows 30 without, 35 with two."""
     blocks = -(-k // TILE_K)
     best = None
     for h in range(64, min(256, max(64, -(-rows // 16) * 16)) + 1, 16):
@@ -349,7 +349,8 @@ def _two_kernels(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_f
 
 
 def _sorted(runtime, x, rows: int, ld: int, ids, top: int, w: int, wts, w_first, w_down, act: int, before: bool, constants, dtype, defer):
-    """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums."""
+    """The experts' token rows side by side, a tensor-core product over tiles of them for each half, and the rows' weighed sums. Between the halves
+    a row is bfloat16, as the second product's rows have to be; what the second half makes is 32-bit until it is added."""
     E, inter, hidden, pairs, status, stream = w_down.groups, w_down.k, w_down.n, rows * top, runtime.status.data_ptr(), ops.stream()
     tile = 64 if pairs <= LOW_PAIRS * E else 160
     tiles = min(pairs // tile + E, pairs)

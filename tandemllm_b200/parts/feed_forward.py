@@ -141,6 +141,7 @@ class DenseActivation(Part):
     def forward(self, x, step):
         tc = self.runtime.tensorcore
         if isinstance(self.w_up, mxfp4.Mxfp4Matrix):
+            # (an activation that the product does not end with acts on rows rounded to bfloat16, as in decode steps with stored weights)
             fused = self.act in mxfp4.ACTIVATIONS
             act = mxfp4.linear(self.runtime, x, self.w_up, act=self.act if fused else None)
             if not fused:
