@@ -51,3 +51,24 @@ def test_experts_with_such_blocks_among_others(runtime, m):
     want, off = P.experts(x, ids, wts, P.rounded(first).view(5, 1, 40, 96), P.rounded(down), "identity")
     assert float(want.abs().max()) > 2.0 ** -24
     P.hold(got, want, off)
+
+
+@pytest.mark.parametrize("size,weight", [(-125, 60), (-112, 50), (-111, 0), (-60, -30), (110, -60), (124, -124)])
+@pytest.mark.parametrize("m", [1, 8, 9])
+def test_rows_of_any_size(runtime, m, size, weight):
+    """Token rows from below the smallest normal number to next to the largest one, with weights that bring their products back."""
+    from tandemllm_b200.kernels import mxfp4
+    g = torch.Generator().manual_seed(m)
+    x = torch.ldexp(M.rows(g, m, 264).float().clamp(-7, 7), torch.tensor(size)).to(torch.bfloat16)
+    x[0, 100:] = 0                              # (a row's largest number may lie anywhere, or there may be none)
+    x[m - 1, :] *= 0 if m > 1 else 1
+    w = torch.ldexp(M.weights(g, 2, 48, 264).clamp(-0.9, 0.9), torch.tensor(weight))
+    v = P.rounded(w)
+    want, off = P.product(x, v[0])
+    assert float(want.abs().max()) > 2.0 ** (size + weight - 6)
+    P.hold(mxfp4.linear(runtime, x.to(DEV), mxfp4.quantize(w[0].to(DEV)), out_dtype=torch.float32), want, off)
+    down = torch.ldexp(M.weights(g, 2, 264, 48), torch.tensor(-weight))
+    ids, wts = M.routed(g, m, 2, 2)
+    got = mxfp4.experts(runtime, x.to(DEV), ids.to(DEV), wts.to(DEV), mxfp4.quantize(w.to(DEV)), mxfp4.quantize(down.to(DEV)), "identity",
+                        out_dtype=torch.float32)
+    P.hold(got, *P.experts(x, ids, wts, v.view(2, 1, 48, 264), P.rounded(down), "identity"))
