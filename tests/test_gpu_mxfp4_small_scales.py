@@ -67,6 +67,8 @@ def test_rows_of_any_size(runtime, m, size, weight):
     want, off = P.product(x, v[0])
     assert float(want.abs().max()) > 2.0 ** (size + weight - 6)
     P.hold(mxfp4.linear(runtime, x.to(DEV), mxfp4.quantize(w[0].to(DEV)), out_dtype=torch.float32), want, off)
+    if weight < -90 and m <= mxfp4.EXPERT_ROWS:
+        return                                  # (the second half's weights would be beyond 2^95, where sums of up to 8 rows can be infinite)
     down = torch.ldexp(M.weights(g, 2, 264, 48), torch.tensor(-weight))
     ids, wts = M.routed(g, m, 2, 2)
     got = mxfp4.experts(runtime, x.to(DEV), ids.to(DEV), wts.to(DEV), mxfp4.quantize(w.to(DEV)), mxfp4.quantize(down.to(DEV)), "identity",
